@@ -1,0 +1,144 @@
+// Label-wise attention over packed notes, forward and backward, for fp32 and bf16 tensors (gfx950).
+//
+//     x[l,t] = <q_l, k_t>;   y = cap tanh(x / cap)  (cap = 0: y = x);   P[l,t] = softmax of y[l,.] over the note's own tokens
+//     O[b,l] = sum_t drop(P[l,t]) v_t;   lse[b,l] = log sum_t exp y[l,t]           (a note of no tokens: O = 0, lse = -inf)
+//     backward, with delta = <dO, O>:  dV_t += drop(P) dO_l;   dS = P (drop(<dO_l, v_t>) - delta) (1 - (y / cap)^2);
+//                                      dK_t = sum_l dS q_l;    dQ_l = sum_{b,t} dS k_t
+//
+// One set of kernels serves both types.  A "fragment" is 16 bytes per lane: eight bf16 (one v_mfma_f32_16x16x32_bf16) or
+// four fp32 (four v_mfma_f32_16x16x4_f32, exact), so a k step of 64 bytes and every LDS offset are the same for both.
+//   row fragment of an image [row][k]:   lane (n = lane & 15, g = lane >> 4) holds row n, bytes 64 s + 16 g .. + 15
+//   column fragment of the same image (k down the rows): bf16 by ds_read_b64_tr_b16 (k order 16 h + 4 g + j), fp32 by four
+//   ds_read_b32 (k = 4 g + j): exactly the order in which the accumulator registers of two (one) 16 x 16 score tiles hold
+//   their rows, so P and dS go from accumulator to operand without touching LDS.
+// Sums are fp32.  P and dS are rounded to the tensors' type for the second product (bf16: half a step of 2^-8 each, as the
+// inputs' own rounding; nothing for fp32); the softmax sum uses P before that rounding.
+//
+// A pre-pass writes the operands as TILE IMAGES of 32 rows that are byte for byte the LDS layout (row pitch 64 s + 32 bytes:
+// conflict-free for both ways of reading), zero-filled past the note's end, past the last label and past E / F.  The sweeps
+// then copy whole tiles by LDS-DMA, and odd widths, row pitches, alignment and whatever lies between the notes
+// (NaN included) end in the pre-pass.
+#pragma once
+#include "packed.h"
+#include "rng.h"
+#include "../../include/gzsl_hip.h"
+
+#define PA_ROWS 32  // rows (tokens or labels) of a tile image
+#define PA_LOG2E 1.4426950408889634f
+#define PA_LN2 0.6931471805599453f
+
+template <typename T>
+struct PaTy;
+template <>
+struct PaTy<float> {
+    typedef f32x4 frag;
+};
+template <>
+struct PaTy<bf16> {
+    typedef bf16x8 frag;
+};
+
+// NE / NF: 16-wide tiles of the key / value width (E <= 16 NE, F <= 16 NF).
+template <typename T, int NE_, int NF_>
+struct PaGeo {
+    static constexpr int NE = NE_, NF = NF_, SZ = sizeof(T), KF = 16 / SZ, KK = 4 * KF, KS = PA_ROWS / KK;
+    static constexpr int SE = (NE * 16 * SZ + 63) / 64, SF = (NF * 16 * SZ + 63) / 64;  // 64-byte k steps over e / f
+    static constexpr int PE = 64 * SE + 32, PF = 64 * SF + 32;                          // row pitches in bytes
+    static constexpr int EB = PA_ROWS * PE, FB = PA_ROWS * PF;                          // image bytes (whole KB)
+    static constexpr int KV = EB + FB;                                                  // token tile: keys, values
+    static constexpr int OB = FB + 1024;                                                // label tile of dO: rows, lse[32], delta[32]
+};
+
+__device__ __forceinline__ f32x4 pa_mma(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = mfma16(a[j], b[j], c);
+    return c;
+}
+__device__ __forceinline__ f32x4 pa_mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ typename PaTy<T>::frag pa_row(const char* img, int pitch, int row0, int s, int n, int g) {
+    return *reinterpret_cast<const typename PaTy<T>::frag*>(img + (row0 + n) * pitch + 64 * s + 16 * g);
+}
+template <typename T>
+__device__ __forceinline__ typename PaTy<T>::frag pa_col(const char* img, int pitch, int row0, int col0, int n, int g);
+template <>
+__device__ __forceinline__ f32x4 pa_col<float>(const char* img, int pitch, int row0, int col0, int n, int g) {
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(img + (row0 + 4 * g + j) * pitch + 4 * (col0 + n));
+    return v;
+}
+template <>
+__device__ __forceinline__ bf16x8 pa_col<bf16>(const char* img, int pitch, int row0, int col0, int n, int g) {
+    const char* p = img + (row0 + 4 * g + (n >> 2)) * pitch + 2 * col0 + 8 * (n & 3);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(p + 16 * pitch));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// accumulator registers of the two 16-row score tiles -> operand fragment of k step ks
+__device__ __forceinline__ void pa_pack(const float (&p)[2][4], int ks, f32x4& out) {
+    out = f32x4{p[ks][0], p[ks][1], p[ks][2], p[ks][3]};
+}
+__device__ __forceinline__ void pa_pack(const float (&p)[2][4], int, bf16x8& out) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = (bf16)p[j >> 2][j & 3];
+}
+
+struct PaCap {
+    float cap, k1, c2;  // cap, 2 log2(e) / cap, cap log2(e)
+};
+__device__ __forceinline__ PaCap pa_cap(float cap) {
+    return {cap, cap > 0.f ? 2.f * PA_LOG2E / cap : 0.f, cap * PA_LOG2E};
+}
+// Score in units of log 2, and th = tanh(x / cap).  tanh u = 1 - 2 / (1 + e^{2u}): exact limits at +-inf, absolute error of a
+// few 2^-24.  fp32 tensors take the odd series below |u| = 0.35 (the next term is below 2^-26 of the value there), where the
+// difference would lose relative accuracy that the products of the gradient still have.
+template <typename T>
+__device__ __forceinline__ float pa_score2(float x, const PaCap& c, float& th) {
+    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1));
+    if (sizeof(T) == 2) {
+        th = fmaf(-2.f, r, 1.f);
+    } else {
+        const float u = x * (c.k1 * (0.5f * PA_LN2)), w = u * u;
+        const float s = u * fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+        th = fabsf(u) < 0.35f ? s : fmaf(-2.f, r, 1.f);
+    }
+    return th * c.c2;
+}
+
+// Copies `bytes` (whole KB) of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  The
+// caller waits with pa_arrive() before anyone reads.
+template <int WAVES>
+__device__ __forceinline__ void pa_dma(const char* src, char* dst, int bytes, int wave, int lane) {
+    for (int o = wave * 1024; o < bytes; o += WAVES * 1024)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + 16 * lane), (GZ_LDS void*)(dst + o), 16, 0, 0);
+}
+// this wave's copies have landed and every wave is past its reads of the other buffer
+__device__ __forceinline__ void pa_arrive() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+struct PaArgs {
+    const void *keys, *values, *queries;
+    const int64_t* spans;
+    long long rows, ldk, ldv, ldq;
+    int B, max_len, L, E, F, nT, nQ;  // nT: token tiles of the longest note, nQ: label tiles
+    float cap;
+    uint32_t l_offset, L_total, seed, thresh;
+    float scale;
+    // workspace
+    char *KV, *Q, *DO;
+    float *part, *ml;    // forward, split over tokens: unnormalised O [split][B][L][F] and (max, sum) [split][B][L][2]
+    float *dq, *dkv;     // backward: [slab][L][E]; [split][rows][E + F]
+    int nsplit;          // token splits (forward, dQ) or label splits (dK / dV) of a launch
+    // results and the backward's inputs
+    void* O;
+    float* LSE;
+    const void *cO, *dO;
+    const float* cLSE;
+    void *dK, *dV, *dQ;
+};

@@ -13,6 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('GZSL_HIP_LIB') or os.path.join(_HERE, 'lib', 'libgzsl_hip.so')  # env: diagnostic builds
 
 ACT_NONE, ACT_RELU, ACT_TANH, ACT_LRELU = 0, 1, 2, 3
+F32, BF16 = 0, 1
 EINVAL = 1001
 ETOOBIG = 1002
 
@@ -29,6 +30,21 @@ class GzslGemm(ctypes.Structure):
                 ('ldc', c_int), ('act', c_int), ('accumulate', c_int), ('alpha', c_float),
                 ('split_k', c_int), ('k_per_split', c_int), ('slab_stride', c_ll),
                 ('dot_w', c_void_p), ('dot_out', c_void_p), ('dot_period', c_int), ('dot_no_store', c_int)]
+
+class GzslPackedAttn(ctypes.Structure):
+    """Mirror of `struct GzslPackedAttn` (include/gzsl_hip.h)."""
+    _fields_ = [('keys', c_void_p), ('values', c_void_p), ('queries', c_void_p), ('spans', c_void_p),
+                ('rows', c_ll), ('ldk', c_ll), ('ldv', c_ll), ('ldq', c_ll),
+                ('B', c_int), ('max_len', c_int), ('L', c_int), ('E', c_int), ('F', c_int), ('dtype', c_int),
+                ('cap', c_float), ('l_offset', c_int), ('L_total', c_int), ('seed', c_u32), ('drop_thresh', c_u32),
+                ('drop_scale', c_float)]
+
+
+class GzslGatedScan(ctypes.Structure):
+    """Mirror of `struct GzslGatedScan` (include/gzsl_hip.h)."""
+    _fields_ = [('gates', c_void_p), ('cands', c_void_p), ('spans', c_void_p), ('h0', c_void_p),
+                ('rows', c_ll), ('ldg', c_ll), ('ldc', c_ll),
+                ('B', c_int), ('max_len', c_int), ('H', c_int), ('reverse', c_int), ('dtype', c_int)]
 
 
 # name -> argtypes (every entry point include/gzsl_hip.h declares; tests check the export list against the header)
@@ -81,6 +97,16 @@ _PROTOS = {
     'gzsl_gan_critic_head': [c_void_p] * 11 + [c_int, c_int, c_void_p],
     'gzsl_gan_gen_head': [c_void_p] * 7 + [c_int, c_int, c_void_p],
     'gzsl_adam_flat_step': [c_void_p] * 4 + [c_ll] + [c_float] * 4 + [c_void_p, c_void_p],
+    'gzsl_packed_attn_work_bytes': [ctypes.POINTER(GzslPackedAttn), c_int],
+    'gzsl_packed_attn_fwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 3 + [c_ll, c_void_p],
+    'gzsl_packed_attn_bwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 7 + [c_ll, c_void_p],
+    'gzsl_gated_scan_work_bytes': [ctypes.POINTER(GzslGatedScan), c_int],
+    'gzsl_gated_scan_fwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 3 + [c_ll, c_void_p],
+    'gzsl_gated_scan_bwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 7 + [c_ll, c_void_p],
+    'gzsl_gated_scan_step': [c_void_p] * 4 + [c_int, c_int, c_ll, c_ll, c_int, c_void_p],
+    'gzsl_clip_work_bytes': [c_void_p, c_int],
+    'gzsl_clip_grad_norm': [c_void_p] * 3 + [c_int, c_float, c_void_p, c_void_p, c_ll, c_void_p],
+    'gzsl_adamw_clip_step': [c_void_p] * 5 + [c_int] + [c_float] * 6 + [c_void_p, c_void_p, c_ll, c_void_p],
 }
 
 _lib = None
@@ -103,8 +129,7 @@ def load():
     for name, argtypes in _PROTOS.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
-        fn.restype = c_ll if name in ('gzsl_label_attn_bwd_det_work_floats', 'gzsl_label_attn_fwd_bf16x6_work_bytes',
-                                        'gzsl_label_attn_bwd_bf16x6_work_bytes') else c_int
+        fn.restype = c_ll if name.endswith(('_work_floats', '_work_bytes')) else c_int
     lib.gzsl_build_info.restype = ctypes.c_char_p
     lib.gzsl_build_info.argtypes = []
     _lib = lib

@@ -79,16 +79,24 @@ class EmbLayer(nn.Module):
 class AdamW(Optimizer):
     """The reference's hand-rolled AdamW (common_module.py:126-182): no bias correction, eps added to sqrt(v),
     weight decay applied to the parameter; per-parameter state keys `step`, `next_m`, `next_v`.  One fused kernel per
-    parameter tensor (`gzsl_adamw_nobias_step`)."""
+    parameter tensor (`gzsl_adamw_nobias_step`).
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), e=1e-6, weight_decay=0.0, ops=None):
+    Extra, not in the reference: `max_grad_norm` clips the gradients to that global norm on
+    their way into the update; the gradients themselves are left as they are, and `grad_norm` holds the norm of the last
+    step as a 0-dim device tensor.  One parameter group only; the whole step is two launches (`gzsl_adamw_clip_step`)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), e=1e-6, weight_decay=0.0, ops=None, max_grad_norm=None):
         for which, beta in enumerate(betas):
             if not 0.0 <= beta < 1.0:
                 raise ValueError(f'Invalid beta parameter at index {which}: {beta} - should be in [0.0, 1.0[')
         if e < 0.0 or e != e:
             raise ValueError(f'Invalid epsilon value: {e} - should be >= 0.0')
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f'Invalid max_grad_norm: {max_grad_norm} - should be > 0.0')
         super().__init__(params, dict(lr=lr, betas=betas, e=e, weight_decay=weight_decay))
         self._ops = ops
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
 
     def _moments(self, p):
         st = self.state[p]
@@ -101,6 +109,9 @@ class AdamW(Optimizer):
         if self._ops is None:
             from ..ops_hip import HipOps
             self._ops = HipOps()
+        if self.max_grad_norm is not None:
+            self._clipped_step()
+            return loss
         for group in self.param_groups:
             b1, b2 = group['betas']
             for p in group['params']:
@@ -113,3 +124,29 @@ class AdamW(Optimizer):
                                       group['e'], group['weight_decay'])
                 st['step'] += 1
         return loss
+
+    def _clipped_step(self):
+        if len(self.param_groups) != 1:
+            raise NotImplementedError('max_grad_norm needs one parameter group: clip with clip_grad_norm_ first, then step')
+        group = self.param_groups[0]
+        ps = [p for p in group['params'] if p.grad is not None]
+        if any(p.grad.is_sparse for p in ps):
+            raise RuntimeError('Adam does not support sparse gradients, please consider SparseAdam instead')
+        sts = [self._moments(p) for p in ps]
+        self.grad_norm = self._ops.adamw_clip_step_([p.data for p in ps], [p.grad.data.contiguous() for p in ps],
+                                                    [st['next_m'] for st in sts], [st['next_v'] for st in sts],
+                                                    self.max_grad_norm, group['lr'], *group['betas'], group['e'],
+                                                    group['weight_decay'])
+        for st in sts:
+            st['step'] += 1
+
+
+def clip_grad_norm_(parameters, max_norm, ops=None):
+    """torch.nn.utils.clip_grad_norm_(parameters, max_norm) of the 2-norm on the HIP kernels: the global norm (0-dim device
+    tensor, before clipping) of all gradients, which are scaled in place by min(1, max_norm / (norm + 1e-6)); two launches,
+    nothing is read back.  fp32 and bf16 gradients; a gradient must be contiguous."""
+    if ops is None:
+        from ..ops_hip import HipOps
+        ops = HipOps()
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    return ops.clip_grad_norm_([p.grad for p in parameters if p.grad is not None], max_norm)

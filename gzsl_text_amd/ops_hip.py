@@ -464,6 +464,197 @@ class HipOps:
              ptr(loss), ptr(dlogits), ptr(probs), B, L)
         return loss, dlogits, probs
 
+    # ------------------------------------------------------------------------------------ packed notes
+    @staticmethod
+    def _dtype(*ts):
+        t = ts[0].dtype
+        if t not in (torch.float32, torch.bfloat16) or any(x is not None and x.dtype != t for x in ts):
+            raise RuntimeError(f'expected tensors of one type, float32 or bfloat16, got {[str(x.dtype) for x in ts if x is not None]}')
+        return hip.F32 if t == torch.float32 else hip.BF16
+
+    @staticmethod
+    def _rows(t, what):
+        """A [rows, width] tensor whose rows are contiguous (any row pitch)."""
+        if t.dim() != 2:
+            raise RuntimeError(f'{what}: expected [rows, width], got {tuple(t.shape)}')
+        ok = t.stride(1) == 1 or t.shape[1] <= 1
+        return t if ok and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+    @staticmethod
+    def _ld(t):
+        return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+    @staticmethod
+    def _spans(spans, max_len):
+        if spans.dtype != torch.int64 or spans.dim() != 2 or spans.shape[1] != 2 or not spans.is_contiguous():
+            raise RuntimeError(f'spans: expected contiguous int64 [B, 2], got {spans.dtype} {tuple(spans.shape)}')
+        if not 0 <= max_len < 2 ** 31:
+            raise RuntimeError(f'max_len {max_len} out of range')
+
+    def _packed_attn(self, keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p):
+        dt = self._dtype(keys, values, queries)
+        keys, values, queries = self._rows(keys, 'keys'), self._rows(values, 'values'), self._rows(queries, 'queries')
+        self._spans(spans, max_len)
+        if keys.shape[0] != values.shape[0] or keys.shape[1] != queries.shape[1]:
+            raise RuntimeError(f'keys {tuple(keys.shape)}, values {tuple(values.shape)}, queries {tuple(queries.shape)} do not fit')
+        if not 0.0 <= p < 1.0:
+            raise RuntimeError(f'drop probability {p} outside [0, 1)')
+        L = queries.shape[0]
+        L_total = L_total or L
+        if l_offset < 0 or l_offset + L > L_total:
+            raise RuntimeError(f'labels {l_offset} .. {l_offset + L} outside of {L_total}')
+        th, sc = drop_params(p)
+        d = hip.GzslPackedAttn(dptr(keys), dptr(values), dptr(queries), ptr(spans), keys.shape[0], self._ld(keys), self._ld(values),
+                               self._ld(queries), spans.shape[0], max_len, L, keys.shape[1], values.shape[1], dt, float(cap),
+                               l_offset, L_total, seed & 0xFFFFFFFF, th, sc)
+        return d, (keys, values, queries)  # (the tensors: a contiguous copy must outlive the launch)
+
+    def attn_packed_fwd(self, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0):
+        """(O [B,L,F], lse [B,L]): label attention over packed notes (gzsl_packed_attn_fwd).  keys [R,E], values [R,F],
+        queries [L,E], all fp32 or all bf16; spans [B,2] int64 = (first row, rows) per note, ascending and disjoint."""
+        d, hold = self._packed_attn(keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p)
+        O = torch.empty((d.B, d.L, d.F), dtype=values.dtype, device=values.device)
+        lse = torch.empty((d.B, d.L), dtype=torch.float32, device=values.device)
+        work = self._work('gzsl_packed_attn_work_bytes', d, 0, values.device)
+        call('gzsl_packed_attn_fwd', d, ptr(O), ptr(lse), ptr(work), work.numel())
+        del hold
+        return O, lse
+
+    def attn_packed_bwd(self, dO, O, lse, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0):
+        """(dkeys [R,E], dvalues [R,F], dqueries [L,E]) of attn_packed_fwd; rows of no note get zeros."""
+        d, hold = self._packed_attn(keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p)
+        self._dtype(keys, dO, O)
+        if tuple(dO.shape) != (d.B, d.L, d.F) or dO.shape != O.shape or tuple(lse.shape) != (d.B, d.L):
+            raise RuntimeError(f'dO {tuple(dO.shape)}, O {tuple(O.shape)}, lse {tuple(lse.shape)} do not fit {(d.B, d.L, d.F)}')
+        _check_f32(lse)
+        dK, dV, dQ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (keys, values, queries))
+        if d.B == 0 or d.L == 0:
+            return dK.zero_(), dV.zero_(), dQ.zero_()
+        work = self._work('gzsl_packed_attn_work_bytes', d, 1, dO.device)
+        call('gzsl_packed_attn_bwd', d, ptr(O), ptr(lse), ptr(dO), ptr(dK), ptr(dV), ptr(dQ), ptr(work), work.numel())
+        del hold
+        return dK, dV, dQ
+
+    @staticmethod
+    def _work(name, d, backward, device):
+        n = getattr(hip.load(), name)(d, backward)
+        if n < 0:
+            raise RuntimeError(f'{name[:-len("_work_bytes")]}: unsupported arguments (GZSL_EINVAL)')
+        return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+    def _gated_scan(self, gates, cands, spans, max_len, h0, reverse):
+        dt = self._dtype(gates, cands)
+        gates, cands = self._rows(gates, 'gates'), self._rows(cands, 'cands')
+        self._spans(spans, max_len)
+        if gates.shape != cands.shape:
+            raise RuntimeError(f'gates {tuple(gates.shape)} and cands {tuple(cands.shape)} do not fit')
+        _check_f32(h0)
+        if h0 is not None and tuple(h0.shape) != (spans.shape[0], gates.shape[1]):
+            raise RuntimeError(f'h0 {tuple(h0.shape)} does not fit {(spans.shape[0], gates.shape[1])}')
+        d = hip.GzslGatedScan(dptr(gates), dptr(cands), ptr(spans), ptr(h0), gates.shape[0], self._ld(gates), self._ld(cands),
+                              spans.shape[0], max_len, gates.shape[1], int(bool(reverse)), dt)
+        return d, (gates, cands)
+
+    def gated_scan_fwd(self, gates, cands, spans, max_len, h0=None, reverse=False):
+        """(h [R,H], h_last [B,H] fp32): h_t = (1 - z_t) h_{t-1} + z_t cands_t with z = sigmoid(gates), through every note's
+        rows (backwards when `reverse`) from h0 [B,H] fp32 (None: zeros).  Rows of no note get zeros."""
+        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse)
+        h = torch.empty(gates.shape, dtype=gates.dtype, device=gates.device)
+        last = torch.empty((d.B, d.H), dtype=torch.float32, device=gates.device)
+        if d.B == 0:
+            return h.zero_(), last
+        work = self._work('gzsl_gated_scan_work_bytes', d, 0, gates.device)
+        call('gzsl_gated_scan_fwd', d, ptr(h), ptr(last), ptr(work), work.numel())
+        del hold
+        return h, last
+
+    def gated_scan_bwd(self, dh, dlast, h, gates, cands, spans, max_len, h0=None, reverse=False):
+        """(dgates, dcands, dh0) of gated_scan_fwd; dh [R,H] or dlast [B,H] may be None (zeros)."""
+        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse)
+        self._dtype(gates, h, dh)
+        _check_f32(dlast)
+        if h.shape != gates.shape or (dh is not None and dh.shape != h.shape) or (dlast is not None and tuple(dlast.shape) != (d.B, d.H)):
+            raise RuntimeError('gated_scan_bwd: h / dh / dlast do not fit the gates')
+        dg, dc = (torch.empty(gates.shape, dtype=gates.dtype, device=gates.device) for _ in range(2))
+        dh0 = torch.empty((d.B, d.H), dtype=torch.float32, device=gates.device)
+        if d.B == 0:
+            return dg.zero_(), dc.zero_(), dh0
+        work = self._work('gzsl_gated_scan_work_bytes', d, 1, gates.device)
+        call('gzsl_gated_scan_bwd', d, ptr(h), ptr(dh), ptr(dlast), ptr(dg), ptr(dc), ptr(dh0), ptr(work), work.numel())
+        del hold
+        return dg, dc, dh0
+
+    def gated_scan_step_(self, gates, cands, state, active=None):
+        """One token of every running note: state [B,H] fp32 <- (1 - z) state + z cands, z = sigmoid(gates); rows whose
+        `active` [B] (bool) is False keep theirs."""
+        dt = self._dtype(gates, cands)
+        _check_f32(state)
+        gates, cands = self._rows(gates, 'gates'), self._rows(cands, 'cands')
+        if gates.shape != cands.shape or state.shape != gates.shape:
+            raise RuntimeError(f'gates {tuple(gates.shape)}, cands {tuple(cands.shape)}, state {tuple(state.shape)} do not fit')
+        if active is not None and (active.dtype != torch.bool or tuple(active.shape) != (state.shape[0],)):
+            raise RuntimeError(f'active: expected bool [{state.shape[0]}], got {active.dtype} {tuple(active.shape)}')
+        if state.numel():
+            call('gzsl_gated_scan_step', dptr(gates), dptr(cands), ptr(state), ptr(active), state.shape[0], state.shape[1],
+                 self._ld(gates), self._ld(cands), dt)
+            torch.autograd.graph.increment_version(state)
+        return state
+
+    # ------------------------------------------------------------------------------------ gradient clipping
+    @staticmethod
+    def _pointers(ts):
+        """Host array of the tensors' addresses; a tensor given twice would be updated twice at once."""
+        import ctypes
+        a = [ptr(t) for t in ts]
+        held = [x for x in a if x]
+        if len(set(held)) != len(held):
+            raise RuntimeError('the same tensor appears twice in the list')
+        return (ctypes.c_void_p * max(len(a), 1))(*a)
+
+    @staticmethod
+    def _sizes(ts):
+        import ctypes
+        return (ctypes.c_longlong * max(len(ts), 1))(*[t.numel() for t in ts])
+
+    def clip_grad_norm_(self, grads, max_norm):
+        """Global 2-norm of the gradients (fp32 or bf16 tensors) as a 0-dim fp32 tensor; every gradient is multiplied by
+        min(1, max_norm / (norm + 1e-6)) in place.  Nothing is read back to the host."""
+        import ctypes
+        grads = list(grads)
+        if not max_norm > 0:
+            raise RuntimeError(f'max_norm must be positive, got {max_norm}')
+        for t in grads:
+            self._dtype(t)
+        dev = grads[0].device if grads else torch.device('cuda', torch.cuda.current_device())
+        sizes, n = self._sizes(grads), len(grads)
+        types = (ctypes.c_int * max(n, 1))(*[self._dtype(t) for t in grads])
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(max(hip.load().gzsl_clip_work_bytes(sizes, n), 16), dtype=torch.uint8, device=dev)
+        call('gzsl_clip_grad_norm', self._pointers(grads), sizes, types, n, float(max_norm), ptr(norm), ptr(work), work.numel())
+        torch.autograd.graph.increment_version(grads)
+        return norm
+
+    def adamw_clip_step_(self, params, grads, m, v, max_norm, lr, beta1, beta2, eps, wd):
+        """adamw_step_ over a list of tensors, every gradient multiplied by min(1, max_norm / (norm + 1e-6)) on the way (norm:
+        of all of them together, returned as a 0-dim fp32 tensor).  The gradients are left as they are."""
+        lists = [list(x) for x in (params, grads, m, v)]
+        if not max_norm > 0:
+            raise RuntimeError(f'max_norm must be positive, got {max_norm}')
+        n = len(lists[0])
+        if any(len(x) != n for x in lists) or any(t.shape != p.shape for x in lists for p, t in zip(lists[0], x)):
+            raise RuntimeError('params, grads and moments do not fit')
+        for x in lists:
+            _check_f32(*x)
+        dev = lists[0][0].device if n else torch.device('cuda', torch.cuda.current_device())
+        sizes = self._sizes(lists[0])
+        self._pointers(lists[0] + lists[2] + lists[3])  # (no tensor may be written twice, across the lists either)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(max(hip.load().gzsl_clip_work_bytes(sizes, n), 16), dtype=torch.uint8, device=dev)
+        call('gzsl_adamw_clip_step', *[self._pointers(x) for x in lists], sizes, n, float(max_norm), lr, beta1, beta2, eps, wd,
+             ptr(norm), ptr(work), work.numel())
+        torch.autograd.graph.increment_version(lists[0] + lists[2] + lists[3])
+        return norm
+
     # ------------------------------------------------------------------------------------ batching / eval scoring
     def multihot(self, y_indices, L):
         """[B,W] int64 label lists padded with -1 -> dense fp32 [B,L] targets (utils/helper.py:117-123)."""

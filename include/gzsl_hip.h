@@ -266,6 +266,73 @@ int gzsl_gan_gen_head(const float* hf, const float* lh, const float* w2, const f
 int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long n, float lr, float beta1, float beta2,
                         float eps, int* state, void* stream);
 
+/* ---- packed notes -----------------------------------------------------------------------------------------------
+ * Notes of unequal length in one [rows, width] tensor: note b owns rows spans[2b] .. spans[2b] + spans[2b+1] - 1 (int64, on
+ * the device, ascending and disjoint; a padded [B,T,width] batch is spans (b*T, length)).  `max_len` is at least the longest
+ * count.  The kernels clamp every span to [0, rows) and max_len.  Tensors are fp32 or bf16 (`dtype`), their rows `ld*`
+ * elements apart with consecutive elements inside a row; sums, softmax statistics and states are fp32 for both. */
+#define GZSL_F32 0
+#define GZSL_BF16 1
+/* Label-wise attention over packed notes (icd_modules.py:137-142 for notes of unequal length; the reference attends its
+ * padding):  x = <q_l, k_t>, y = cap*tanh(x/cap) (cap = 0: y = x), softmax of y over the note's own tokens, dropout on the
+ * weights (the masks of gzsl_label_attn_fwd, keyed on (b*L_total + l_offset + l, token index in the note)), pooling of the
+ * values.  O [B,L,F] of the tensors' type, LSE [B,L] fp32 (natural units); a note of no tokens gives O = 0, LSE = -inf.
+ * E, F <= 208.  `work`: 16-byte aligned device scratch of gzsl_packed_attn_work_bytes(d, backward) bytes (-1: bad arguments),
+ * its contents undefined before and after. */
+typedef struct GzslPackedAttn {
+    const void* keys;    /* [rows, E] */
+    const void* values;  /* [rows, F] */
+    const void* queries; /* [L, E] */
+    const int64_t* spans;
+    long long rows, ldk, ldv, ldq;
+    int B, max_len, L, E, F, dtype;
+    float cap;
+    int l_offset, L_total;
+    uint32_t seed, drop_thresh;
+    float drop_scale;
+} GzslPackedAttn;
+long long gzsl_packed_attn_work_bytes(const GzslPackedAttn* d, int backward);
+int gzsl_packed_attn_fwd(const GzslPackedAttn* d, void* O, float* LSE, void* work, long long work_bytes, void* stream);
+/* autograd of the above from its O, LSE and dO [B,L,F]: dkeys [rows,E], dvalues [rows,F], dqueries [L,E] are WRITTEN (not
+ * accumulated), of the tensors' type and contiguous, zero in rows of no note; sums are taken in a fixed order, without atomics. */
+int gzsl_packed_attn_bwd(const GzslPackedAttn* d, const void* O, const float* LSE, const void* dO, void* dkeys, void* dvalues,
+                         void* dqueries, void* work, long long work_bytes, void* stream);
+/* Gated linear recurrence over packed notes:  z = sigmoid(gates), h_t = (1 - z_t) h_{t-1} + z_t cands_t, from h0 [B,H] fp32
+ * (NULL: 0) through each note's rows, backwards when `reverse`.  h [rows,H] of the tensors' type, contiguous, zero in rows of
+ * no note; h_last [B,H] fp32 the state behind each note's last step (h0 for a note of no tokens). */
+typedef struct GzslGatedScan {
+    const void* gates; /* [rows, H] */
+    const void* cands; /* [rows, H] */
+    const int64_t* spans;
+    const float* h0;
+    long long rows, ldg, ldc;
+    int B, max_len, H, reverse, dtype;
+} GzslGatedScan;
+long long gzsl_gated_scan_work_bytes(const GzslGatedScan* d, int backward);
+int gzsl_gated_scan_fwd(const GzslGatedScan* d, void* h, float* h_last, void* work, long long work_bytes, void* stream);
+/* dgates, dcands [rows,H] written (zero in rows of no note), dh0 [B,H] written (may be NULL), from dh [rows,H] and dlast [B,H]
+ * fp32 (either may be NULL: zero) and the forward's h. */
+int gzsl_gated_scan_bwd(const GzslGatedScan* d, const void* h, const void* dh, const float* dlast, void* dgates, void* dcands,
+                        float* dh0, void* work, long long work_bytes, void* stream);
+/* One token of every running note: state [B,H] fp32 <- (1 - z) state + z cands; rows with active[b] == 0 keep theirs (active may
+ * be NULL).  The recurrence's counterpart of gzsl_gru_seq_step. */
+int gzsl_gated_scan_step(const void* gates, const void* cands, float* state, const uint8_t* active, int B, int H, long long ldg,
+                         long long ldc, int dtype, void* stream);
+
+/* ---- gradient clipping -------------------------------------------------------------------------------------------
+ * norm = sqrt(sum of squares over the n tensors) (*norm, fp32 on the device), f = min(1, max_norm / (norm + 1e-6)); every
+ * gradient is multiplied by f.  The pointer, size and type (GZSL_F32 / GZSL_BF16) arrays are HOST memory, read during the call;
+ * the tensors are contiguous.  max_norm > 0 (infinity: the norm alone).  A norm that is not a number makes every gradient one.
+ * `work`: 8-byte aligned device scratch of gzsl_clip_work_bytes(sizes, n) bytes. */
+long long gzsl_clip_work_bytes(const long long* sizes, int n);
+int gzsl_clip_grad_norm(void* const* grads, const long long* sizes, const int* dtypes, int n, float max_norm, float* norm,
+                        void* work, long long work_bytes, void* stream);
+/* gzsl_adamw_nobias_step (common_module.py:138-182) over n tensors with the gradients clipped on the way: f as above, the
+ * update of every tensor from f*g.  The gradients are left as they are. */
+int gzsl_adamw_clip_step(float* const* p, const float* const* g, float* const* m, float* const* v, const long long* sizes, int n,
+                         float max_norm, float lr, float beta1, float beta2, float eps, float wd, float* norm, void* work,
+                         long long work_bytes, void* stream);
+
 /* library self-description: number of exported compute entry points and build target string */
 const char* gzsl_build_info(void);
 

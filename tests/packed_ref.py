@@ -1,0 +1,146 @@
+"""64-bit references of the packed-note operators with ELEMENTWISE error bounds, for tests/test_gpu_packed_*.py.
+
+Every bound counts roundings: u = 2^-24 is half a step of fp32, `step` half a step of the tensors' type (2^-24 or 2^-8,
+torch.finfo(t).eps / 2).  A sum of n products in fp32 is off by at most n u times the sum of their magnitudes."""
+import torch
+
+from oracle.rng import attn_dropout_scale
+
+U = 2.0 ** -24
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None):
+    """keys [R,E], values [R,F], queries [L,E] (any type, used as the numbers they hold), spans list of (start, n);
+    keep: list of [L,n] dropout factors or None.  Returns dict of name -> (value, bound): O, lse and, with dout [B,L,F],
+    dK, dV, dQ."""
+    step = half_step(values.dtype)
+    k, v, q = (x.detach().cpu().double() for x in (keys, values, queries))
+    B, L, E, F, R = len(spans), q.shape[0], k.shape[1], v.shape[1], k.shape[0]
+    z = lambda *s: torch.zeros(s, dtype=torch.float64)  # noqa: E731
+    out = {n: [z(*s), z(*s)] for n, s in (('O', (B, L, F)), ('lse', (B, L)), ('dK', (R, E)), ('dV', (R, F)), ('dQ', (L, E)))}
+    out['lse'][0].fill_(float('-inf'))
+    slabs = 0
+    for b, (s0, n) in enumerate(spans):
+        if n == 0:
+            continue
+        kb, vb = k[s0:s0 + n], v[s0:s0 + n]
+        x = q @ kb.T
+        dx = (E + 2) * U * (q.abs() @ kb.T.abs())         # the product's sum
+        if cap > 0:
+            th = torch.tanh(x / cap)
+            y, slope = cap * th, 1 - th * th
+            dy = dx + 8 * U * cap                          # tanh from exp and reciprocal, a few roundings of values below 2
+        else:
+            th, y, slope, dy = None, x, 1.0, dx
+        dy = dy + 4 * U * y.abs() + 4 * U                  # into units of log 2, and the exponential itself
+        lse = torch.logsumexp(y, 1, keepdim=True)
+        P = torch.exp(y - lse)
+        dlse = (P * dy).sum(1, keepdim=True) + (n + 4) * U + 4 * U * lse.abs()
+        out['lse'][0][b], out['lse'][1][b] = lse[:, 0], dlse[:, 0]
+        rel = dy + dlse + 2 * U * (y - lse).abs() + 4 * U  # relative error of a weight
+        D = 1.0 if keep is None else keep[b]
+        Pd = P * D
+        O = Pd @ vb
+        dO_ = (Pd * (rel + step * (step > U) + (n + 4) * U)) @ vb.abs()   # P is rounded to the tensors' type for the product
+        out['O'][0][b] = O
+        out['O'][1][b] = dO_ + (O.abs() + dO_) * step
+        if dout is None:
+            continue
+        g = dout[b].detach().cpu().double()
+        slabs += 1
+        out['dV'][0][s0:s0 + n] = Pd.T @ g
+        out['dV'][1][s0:s0 + n] = (Pd * (rel + step * (step > U) + (L + 4) * U)).T @ g.abs()
+        dP = g @ vb.T
+        ddP = (F + 2) * U * (g.abs() @ vb.T.abs())
+        delta = (g * O).sum(1, keepdim=True)
+        ddelta = (g.abs() * (out['O'][1][b] + (F + 2) * U * O.abs())).sum(1, keepdim=True)
+        inner = dP * D - delta
+        dS = P * inner * slope
+        ddS = P * ((rel + 4 * U) * inner.abs() + ddP * D + ddelta) * (1.0 if cap == 0 else slope.abs())
+        if cap > 0:
+            dth = (dx / cap + 8 * U) * slope + 4 * U       # error of tanh, from x's error and its own
+            ddS = ddS + P * inner.abs() * 2 * (th.abs() * dth + dth * dth + U)
+        ddS = ddS + dS.abs() * step * (step > U)
+        out['dQ'][0] += dS @ kb
+        out['dQ'][1] += (ddS + (n + 4) * U * dS.abs()) @ kb.abs()
+        out['dK'][0][s0:s0 + n] = dS.T @ q
+        out['dK'][1][s0:s0 + n] = (ddS + (L + 4) * U * dS.abs()).T @ q.abs()
+    for name in ('dK', 'dV', 'dQ'):
+        val, err = out[name]
+        err += (slabs + 256) * U * err + (val.abs() + err) * step          # joining the shares; the last rounding
+    return {n: tuple(x) for n, x in out.items()}
+
+
+def dropout_keep(spans, L, seed, p, l_offset=0, L_total=0):
+    """The counter hash's factors, as oracle/rng.py defines them, per note: [L, n]."""
+    L_total = L_total or L
+    return [torch.from_numpy(attn_dropout_scale(seed, [b], range(l_offset, l_offset + L), L_total, range(n), p)[0]).double()
+            for b, (_, n) in enumerate(spans)]
+
+
+TINY = 2.0 ** -120  # what lies below fp32's smallest normal number, 2^-126, may be flushed to zero; magnitudes it meets here: < 64
+
+
+def within(got, want, what):
+    val, tol = want
+    tol = tol + TINY
+    got = got.detach().cpu().double()
+    assert got.shape == val.shape, (what, got.shape, val.shape)
+    same = (got == val) | (torch.isnan(got) & torch.isnan(val))
+    bad = ~same & ~((got - val).abs() <= tol)
+    if bad.any():
+        i = torch.nonzero(bad)[0].tolist()
+        raise AssertionError(f'{what}: {int(bad.sum())} of {bad.numel()} outside the bound; first at {i}: got {got[tuple(i)].item()!r}, '
+                             f'want {val[tuple(i)].item()!r} +- {tol[tuple(i)].item():.3e}')
+
+
+def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
+    """dict of name -> (value, bound): h, last and, with dh / dlast (either may be None), dg, dc, dh0."""
+    step = half_step(gates.dtype)
+    g, c = gates.detach().cpu().double(), cands.detach().cpu().double()
+    R, H = g.shape
+    B = len(spans)
+    z = lambda *s: torch.zeros(s, dtype=torch.float64)  # noqa: E731
+    out = {n: [z(*s), z(*s)] for n, s in (('h', (R, H)), ('last', (B, H)), ('dg', (R, H)), ('dc', (R, H)), ('dh0', (B, H)))}
+    zz, aa = torch.sigmoid(g), torch.sigmoid(-g)
+    for b, (s0, n) in enumerate(spans):
+        rows = list(range(s0, s0 + n))
+        if reverse:
+            rows.reverse()
+        h = z(H) if h0 is None else h0[b].detach().cpu().double()
+        e = z(H)
+        before, ebefore = z(R, H), z(R, H)
+        for r in rows:
+            before[r], ebefore[r] = h, e
+            t1, t2 = aa[r] * h, zz[r] * c[r]
+            # each gate is off by a few roundings of the exponential and the division, each product by one more
+            e = aa[r] * e + 8 * U * (t1.abs() + t2.abs())
+            h = t1 + t2
+            out['h'][0][r], out['h'][1][r] = h, e + (h.abs() + e) * step
+        out['last'][0][b], out['last'][1][b] = h, e + U * h.abs()
+        if dh is None and dlast is None:
+            continue
+        carry = z(H) if dlast is None else dlast[b].detach().cpu().double()
+        ec = z(H)
+        for r in reversed(rows):
+            lam = carry + (0 if dh is None else dh[r].detach().cpu().double())
+            el = ec + U * lam.abs()
+            out['dc'][0][r] = lam * zz[r]
+            out['dc'][1][r] = (el + 8 * U * lam.abs()) * zz[r]
+            d = c[r] - before[r]
+            w = zz[r] * aa[r]
+            # the backward reads h as it was stored: one rounding to the tensors' type on top of its error
+            ed = ebefore[r] + (before[r].abs() + ebefore[r]) * step + U * (c[r].abs() + before[r].abs())
+            out['dg'][0][r] = lam * d * w
+            out['dg'][1][r] = w * ((el + 20 * U * lam.abs()) * (d.abs() + ed) + lam.abs() * ed)
+            ec = aa[r] * el + 8 * U * (aa[r] * lam).abs()
+            carry = aa[r] * lam
+        out['dh0'][0][b], out['dh0'][1][b] = carry, ec + U * carry.abs()
+    for name in ('dg', 'dc'):
+        val, err = out[name]
+        err += (val.abs() + err) * step
+    return {n: tuple(x) for n, x in out.items()}
