@@ -2,6 +2,14 @@
 //     z = sigmoid(g);   h_t = (1 - z_t) h_{t-1} + z_t c_t          (t runs through a note's rows, or back through them)
 //     backward:  lam_t = dh_t + (1 - z_{t+1}) lam_{t+1};   dc = lam z;   dg = lam (c - h_{t-1}) z (1 - z);   dh_0 = (1 - z_1) lam_1
 // The states are fp32 throughout; tensors of 16 bits are widened when read and rounded once when written.
+//
+// Both directions are the recurrence x <- A x + B, whose steps join: (A1, B1) then (A2, B2) = (A2 A1, A2 B1 + B2).  The time axis is
+// cut into chunks, one workgroup each (a thread owns V channels and S consecutive steps of a tile, all in registers):
+//   1. gs_chunk_kernel reduces every chunk to its (A, B)         reads g and c (g and dh)
+//   2. gs_apply_kernel joins the pairs of the chunks before its own into the state it starts from, then runs through its tiles:
+//      each thread's steps to a pair, a scan of the pairs over the tile's threads in LDS, the steps again from the state in front.
+// Memory-bound: 3 (6) tensors forward (backward), of which the first pass reads two once more (from the 256 MB last-level cache
+// where they fit).  The pairs meet in a fixed order, so results repeat bit for bit; tokens in front of a step never see it.
 #include "packed.h"
 #include "../../include/gzsl_hip.h"
 
@@ -17,55 +25,281 @@ struct GsArgs {
     const float* dlast;
     void *dg, *dc;
     float* dh0;
+    float* pair;                             // [B][nch][2][H]
+    int ncg, nblk, TS, tiles, chunk, nch;    // channel groups of a workgroup, workgroups over the channels, threads over time, tiles of a chunk
 };
 
 // z = sigmoid(g) and a = 1 - z = sigmoid(-g), both to full relative accuracy (e^-|g| never overflows)
 __device__ __forceinline__ void gs_gate(float g, float& z, float& a) {
-    const float e = expf(-fabsf(g)), big = 1.f / (1.f + e), small = e * big;
+    const float e = expf(-fabsf(g)), big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
     z = g >= 0.f ? big : small;
     a = g >= 0.f ? small : big;
     if (g != g) z = a = g;
 }
 
-// one thread per (note, channel)
+template <typename T, int V>
+struct GsVec {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
 template <typename T>
-__global__ __launch_bounds__(64) void gs_fwd_kernel(GsArgs a) {
-    const int ch = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-    if (ch >= a.H) return;
-    const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
-    const T *g = (const T*)a.g + ch, *c = (const T*)a.c + ch;
-    T* out = (T*)a.h + ch;
-    float h = a.h0 ? a.h0[(long long)b * a.H + ch] : 0.f;
-    for (int t = 0; t < sp.len; ++t) {
-        const long long row = sp.start + (a.reverse ? sp.len - 1 - t : t);
-        float z, k;
-        gs_gate((float)g[row * a.ldg], z, k);
-        h = fmaf(k, h, z * (float)c[row * a.ldc]);
-        out[row * a.H] = (T)h;
-    }
-    a.last[(long long)b * a.H + ch] = h;
+struct GsVec<T, 1> {
+    typedef T type;
+};
+template <typename T, int V>
+__device__ __forceinline__ void gs_load(const T* p, float (&v)[V]) {
+    typedef typename GsVec<T, V>::type vec;
+    const vec x = *reinterpret_cast<const vec*>(p);
+    if constexpr (V == 1) v[0] = (float)x;
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (float)x[i];
+}
+template <typename T, int V>
+__device__ __forceinline__ void gs_store(T* p, const float (&v)[V]) {
+    typedef typename GsVec<T, V>::type vec;
+    vec x;
+    if constexpr (V == 1) x = (T)v[0];
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = (T)v[i];
+    *reinterpret_cast<vec*>(p) = x;
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void gs_bwd_kernel(GsArgs a) {
-    const int ch = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-    if (ch >= a.H) return;
-    const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
-    const T *g = (const T*)a.g + ch, *c = (const T*)a.c + ch, *h = (const T*)a.ch + ch, *dh = (const T*)a.dh + ch;
-    T *dg = (T*)a.dg + ch, *dc = (T*)a.dc + ch;
-    const long long at = (long long)b * a.H + ch;
-    const float h0 = a.h0 ? a.h0[at] : 0.f;
-    float carry = a.dlast ? a.dlast[at] : 0.f;
-    for (int t = sp.len - 1; t >= 0; --t) {
-        const long long row = sp.start + (a.reverse ? sp.len - 1 - t : t), prev = a.reverse ? row + 1 : row - 1;
-        float z, k;
-        gs_gate((float)g[row * a.ldg], z, k);
-        const float lam = carry + (a.dh ? (float)dh[row * a.H] : 0.f), before = t > 0 ? (float)h[prev * a.H] : h0;
-        dc[row * a.H] = (T)(lam * z);
-        dg[row * a.H] = (T)(lam * ((float)c[row * a.ldc] - before) * (z * k));
-        carry = lam * k;
+// Inclusive scan of the threads' pairs along time (thread j of TS per channel group); returns the pair of the threads in front
+// in (Ae, Be) and the whole tile's in (At, Bt).
+template <int V>
+__device__ __forceinline__ void gs_scan(float (&A)[V], float (&B)[V], float (&Ae)[V], float (&Be)[V], float (&At)[V], float (&Bt)[V], float* sh, int tid,
+                                        int j, int TS, int ncg, int nt) {
+    auto put = [&]() {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sh[i * nt + tid] = A[i], sh[(V + i) * nt + tid] = B[i];
+    };
+    for (int d = 1; d < TS; d <<= 1) {
+        put();
+        __syncthreads();
+        if (j >= d) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float pa = sh[i * nt + tid - d * ncg], pb = sh[(V + i) * nt + tid - d * ncg];
+                B[i] = fmaf(A[i], pb, B[i]);
+                A[i] *= pa;
+            }
+        }
+        __syncthreads();
     }
-    if (a.dh0) a.dh0[at] = carry;
+    put();
+    __syncthreads();
+    const int lastt = tid - j * ncg + (TS - 1) * ncg;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        Ae[i] = j > 0 ? sh[i * nt + tid - ncg] : 1.f;
+        Be[i] = j > 0 ? sh[(V + i) * nt + tid - ncg] : 0.f;
+        At[i] = sh[i * nt + lastt];
+        Bt[i] = sh[(V + i) * nt + lastt];
+    }
+    __syncthreads();
+}
+
+// Where step i (in the order of the recurrence: forward from a note's first step, backward from its last) has its row.
+template <bool BWD>
+__device__ __forceinline__ long long gs_row(const NoteSpan& sp, int reverse, int i) {
+    return (BWD != (reverse != 0)) ? sp.start + sp.len - 1 - i : sp.start + i;
+}
+
+struct GsPlace {
+    int tid, nt, j, ch, b, k;
+    bool on;
+};
+__device__ __forceinline__ GsPlace gs_place(const GsArgs& a, int V) {
+    GsPlace p;
+    p.tid = threadIdx.x, p.nt = blockDim.x;
+    p.j = p.tid / a.ncg;
+    p.k = blockIdx.x % a.nch;
+    p.b = blockIdx.x / a.nch;
+    p.ch = (blockIdx.y * a.ncg + p.tid % a.ncg) * V;
+    p.on = p.ch < a.H;
+    if (!p.on) p.ch = 0;
+    return p;
+}
+
+template <typename T, int V, int S, bool BWD>
+__global__ __launch_bounds__(512) void gs_chunk_kernel(GsArgs a) {
+    extern __shared__ float sh[];
+    const GsPlace p = gs_place(a, V);
+    const NoteSpan sp = note_span(a.spans, p.b, a.rows, a.max_len);
+    const long long first = (long long)p.k * a.chunk;
+    if (first + a.chunk >= sp.len) return;  // nothing behind this chunk starts from it
+    // this thread's share of the chunk: tiles * S consecutive steps, all inside the note
+    const int n = a.tiles * S, i0 = (int)first + p.j * n;
+    const T *x = (const T*)a.g + p.ch, *y = (BWD ? (const T*)a.dh : (const T*)a.c) + p.ch;
+    const long long ldy = BWD ? a.H : a.ldc;
+    float A[V], B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+    for (int s0 = 0; s0 < n; s0 += S) {
+        float g[S][V], u[S][V];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const long long row = gs_row<BWD>(sp, a.reverse, i0 + s0 + s);
+            gs_load<T, V>(x + row * a.ldg, g[s]);
+            if (!BWD || a.dh) gs_load<T, V>(y + row * ldy, u[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float z, k;
+                gs_gate(g[s][v], z, k);
+                if (BWD) B[v] = k * (B[v] + (a.dh ? u[s][v] : 0.f));
+                else B[v] = fmaf(k, B[v], z * u[s][v]);
+                A[v] *= k;
+            }
+    }
+    float Ae[V], Be[V], At[V], Bt[V];
+    gs_scan<V>(A, B, Ae, Be, At, Bt, sh, p.tid, p.j, a.TS, a.ncg, p.nt);
+    if (p.on && p.j == 0) {
+        float* out = a.pair + ((long long)p.b * a.nch + p.k) * 2 * a.H + p.ch;
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] = At[v], out[a.H + v] = Bt[v];
+    }
+}
+
+template <typename T, int V, int S, bool BWD>
+__global__ __launch_bounds__(512) void gs_apply_kernel(GsArgs a) {
+    extern __shared__ float sh[];
+    const GsPlace p = gs_place(a, V);
+    const NoteSpan sp = note_span(a.spans, p.b, a.rows, a.max_len);
+    const long long first = (long long)p.k * a.chunk;
+    {   // rows of no note: those behind this note, shared out like its own rows, and those in front of note 0
+        const long long next = p.b + 1 < a.B ? note_span(a.spans, p.b + 1, a.rows, a.max_len).start : a.rows;
+        const long long lo = max(first, (long long)sp.len), hi = p.k == a.nch - 1 ? next - sp.start : min(first + a.chunk, next - sp.start);
+        float zero[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) zero[v] = 0.f;
+        auto clear = [&](long long r0, long long r1) {
+            for (long long r = r0 + p.j; r < r1; r += a.TS) {
+                if (!p.on) break;
+                if (BWD) {
+                    gs_store<T, V>((T*)a.dg + r * a.H + p.ch, zero);
+                    gs_store<T, V>((T*)a.dc + r * a.H + p.ch, zero);
+                } else {
+                    gs_store<T, V>((T*)a.h + r * a.H + p.ch, zero);
+                }
+            }
+        };
+        clear(sp.start + lo, sp.start + hi);
+        if (p.b == 0 && p.k == 0) clear(0, sp.start);
+    }
+    if (first >= sp.len && p.k > 0) return;
+    const long long at = (long long)p.b * a.H + p.ch;
+    const float* init = BWD ? a.dlast : a.h0;
+    float x[V];  // the state in front of the current tile
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = init ? init[at + v] : 0.f;
+    float Ae[V], Be[V], At[V], Bt[V];
+    if (p.k > 0) {
+        // the pairs of the chunks in front, shared out over the threads along time
+        const int per = (p.k + a.TS - 1) / a.TS, q0 = p.j * per, q1 = min(p.k, q0 + per);
+        const float* pr = a.pair + (long long)p.b * a.nch * 2 * a.H + p.ch;
+        float A[V], B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll 4
+        for (int q = q0; q < q1; ++q) {
+            float ka[V], kb[V];
+            gs_load<float, V>(pr + (long long)q * 2 * a.H, ka);
+            gs_load<float, V>(pr + (long long)q * 2 * a.H + a.H, kb);
+#pragma unroll
+            for (int v = 0; v < V; ++v) B[v] = fmaf(ka[v], B[v], kb[v]), A[v] *= ka[v];
+        }
+        gs_scan<V>(A, B, Ae, Be, At, Bt, sh, p.tid, p.j, a.TS, a.ncg, p.nt);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = fmaf(At[v], x[v], Bt[v]);
+    }
+    const T *pg = (const T*)a.g + p.ch, *pc = (const T*)a.c + p.ch;
+    for (int t = 0; t < a.tiles; ++t) {
+        const long long base = first + (long long)t * a.TS * S;
+        if (base >= sp.len) break;
+        const int i0 = (int)base + p.j * S;
+        float k[S][V], z[S][V], c[S][V], u[S][V];  // u: dh (backward)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const bool in = i0 + s < sp.len;
+            const long long row = gs_row<BWD>(sp, a.reverse, in ? i0 + s : sp.len - 1);  // (past the end: read the last row, use nothing of it)
+            gs_load<T, V>(pg + row * a.ldg, k[s]);
+            gs_load<T, V>(pc + row * a.ldc, c[s]);
+            if (BWD) {
+                if (a.dh) gs_load<T, V>((const T*)a.dh + p.ch + row * a.H, u[s]);
+                else
+#pragma unroll
+                    for (int v = 0; v < V; ++v) u[s][v] = 0.f;
+                float before[V];
+                const bool start = row == (a.reverse ? sp.start + sp.len - 1 : sp.start);  // the note's first step
+                if (start) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) before[v] = a.h0 ? a.h0[at + v] : 0.f;
+                } else {
+                    gs_load<T, V>((const T*)a.ch + p.ch + (a.reverse ? row + 1 : row - 1) * a.H, before);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) c[s][v] -= before[v];
+            }
+        }
+        float A[V], B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gs_gate(k[s][v], z[s][v], k[s][v]);
+                if (i0 + s >= sp.len) k[s][v] = 1.f, u[s][v] = c[s][v] = z[s][v] = 0.f;
+                if (BWD) {
+                    B[v] = k[s][v] * (B[v] + u[s][v]);
+                } else {
+                    z[s][v] *= c[s][v];
+                    B[v] = fmaf(k[s][v], B[v], z[s][v]);
+                }
+                A[v] *= k[s][v];
+            }
+        // (a step past the end multiplies by 1 and adds nothing: in the backward that leaves k (B + u) = B)
+        gs_scan<V>(A, B, Ae, Be, At, Bt, sh, p.tid, p.j, a.TS, a.ncg, p.nt);
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            y[v] = fmaf(Ae[v], x[v], Be[v]);
+            x[v] = fmaf(At[v], x[v], Bt[v]);
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            if (i0 + s >= sp.len) break;
+            const long long row = gs_row<BWD>(sp, a.reverse, i0 + s);
+            float o[V], w[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (BWD) {
+                    const float lam = y[v] + u[s][v];
+                    o[v] = lam * z[s][v];
+                    w[v] = lam * c[s][v] * (z[s][v] * k[s][v]);
+                    y[v] = lam * k[s][v];
+                } else {
+                    y[v] = fmaf(k[s][v], y[v], z[s][v]);
+                    o[v] = y[v];
+                }
+            }
+            if (!p.on) continue;
+            if (BWD) {
+                gs_store<T, V>((T*)a.dc + row * a.H + p.ch, o);
+                gs_store<T, V>((T*)a.dg + row * a.H + p.ch, w);
+            } else {
+                gs_store<T, V>((T*)a.h + row * a.H + p.ch, o);
+            }
+        }
+    }
+    float* end = BWD ? a.dh0 : a.last;
+    if (p.on && p.j == 0 && end && first + a.chunk >= sp.len)
+#pragma unroll
+        for (int v = 0; v < V; ++v) end[at + v] = x[v];
 }
 
 template <typename T>
@@ -83,7 +317,7 @@ __global__ __launch_bounds__(256) void gs_step_kernel(const T* g, const T* c, fl
 static int gs_check(const GzslGatedScan* d) {
     if (!d || d->B < 0 || d->rows < 0 || d->max_len < 0 || d->H < 1 || d->ldg < d->H || d->ldc < d->H) return GZSL_EINVAL;
     if (d->dtype != GZSL_F32 && d->dtype != GZSL_BF16) return GZSL_EINVAL;
-    if (d->B > 65534) return GZSL_ETOOBIG;
+    if (d->B > 65534 || d->max_len > 0x7FF00000) return GZSL_ETOOBIG;  // (positions of a last, partial tile stay below 2^31)
     if (d->B > 0 && !d->spans) return GZSL_EINVAL;
     if (d->rows > 0 && (!d->gates || !d->cands)) return GZSL_EINVAL;
     return 0;
@@ -95,45 +329,83 @@ static GsArgs gs_args(const GzslGatedScan& d) {
     return a;
 }
 
-template <typename T>
-static int gs_fwd(const GsArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(gs_fwd_kernel<T>, dim3(cdiv(a.H, 64), a.B), dim3(64), 0, st, a);
-    hipLaunchKernelGGL(zero_gaps_kernel<T>, dim3(16, a.B + 1), dim3(256), 0, st, a.spans, a.rows, a.B, a.max_len, (T*)a.h, a.H, (T*)nullptr, 0);
+// Vectors of 16 bytes where the width and every address allow it, 8 bytes for bf16 of a width divisible by 4 only, else elements.
+static int gs_width(const GzslGatedScan& d, uintptr_t addresses) {
+    const int sz = d.dtype == GZSL_F32 ? 4 : 2;
+    for (int V = 16 / sz; V >= 4; V >>= 1)
+        if (d.H % V == 0 && d.ldg % V == 0 && d.ldc % V == 0 && addresses % (uintptr_t)(V * sz) == 0) return V;
+    return 1;
+}
+// S V = 32 values of each operand in a thread's registers; up to 512 threads of at most 64 channel groups.
+static int gs_steps(int V) { return V == 8 ? 4 : 8; }
+static int gs_shape(GsArgs& a, int V) {
+    const int groups = (a.H + V - 1) / V;
+    a.ncg = groups < 64 ? groups : 64;
+    a.nblk = (groups + a.ncg - 1) / a.ncg;
+    a.TS = 512 / a.ncg;
+    const long long tile = (long long)a.TS * gs_steps(V), all = (a.max_len + tile - 1) / tile, wgs = all * a.B * a.nblk;
+    // a chunk is one tile until that makes over 1024 workgroups (four to a compute unit) or over 256 chunks to look back at
+    long long m = wgs / 1024;
+    if (m < (all + 255) / 256) m = (all + 255) / 256;
+    if (m < 1) m = 1;
+    a.tiles = (int)m, a.chunk = (int)(m * tile);
+    a.nch = (int)((a.max_len + a.chunk - 1) / a.chunk);
+    if (a.nch < 1) a.nch = 1;
+    return (long long)a.nch * a.B > 0x7FFFFFFF || a.nblk > 65535 ? GZSL_ETOOBIG : 0;
+}
+
+template <typename T, int V, bool BWD>
+static int gs_go(GsArgs& a, void* work, long long work_bytes, hipStream_t st) {
+    constexpr int S = V == 8 ? 4 : 8;
+    if (int e = gs_shape(a, V)) return e;
+    if (a.nch > 1 && (!work || ((uintptr_t)work & 15) || work_bytes < 8LL * a.B * a.nch * a.H)) return GZSL_EINVAL;
+    a.pair = (float*)work;
+    const dim3 grid(a.nch * a.B, a.nblk), block(a.ncg * a.TS);
+    const size_t lds = sizeof(float) * 2 * V * block.x;
+    if (a.nch > 1) hipLaunchKernelGGL((gs_chunk_kernel<T, V, S, BWD>), grid, block, lds, st, a);
+    hipLaunchKernelGGL((gs_apply_kernel<T, V, S, BWD>), grid, block, lds, st, a);
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <typename T>
-static int gs_bwd(const GsArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(gs_bwd_kernel<T>, dim3(cdiv(a.H, 64), a.B), dim3(64), 0, st, a);
-    hipLaunchKernelGGL(zero_gaps_kernel<T>, dim3(16, a.B + 1), dim3(256), 0, st, a.spans, a.rows, a.B, a.max_len, (T*)a.dg, a.H, (T*)a.dc, a.H);
-    GZSL_CHECK_LAUNCH();
-    return 0;
+template <bool BWD>
+static int gs_run(const GzslGatedScan& d, GsArgs& a, int V, void* work, long long work_bytes, hipStream_t st) {
+    if (d.dtype == GZSL_F32) return V == 4 ? gs_go<float, 4, BWD>(a, work, work_bytes, st) : gs_go<float, 1, BWD>(a, work, work_bytes, st);
+    if (V == 8) return gs_go<bf16, 8, BWD>(a, work, work_bytes, st);
+    return V == 4 ? gs_go<bf16, 4, BWD>(a, work, work_bytes, st) : gs_go<bf16, 1, BWD>(a, work, work_bytes, st);
 }
 
 extern "C" long long gzsl_gated_scan_work_bytes(const GzslGatedScan* d, int backward) {
     (void)backward;
-    return gs_check(d) ? -1 : 0;
+    if (gs_check(d)) return -1;
+    long long most = 0;  // over the vector widths, which the addresses decide
+    for (int V = 1; V <= 8; V <<= 1) {
+        GsArgs a = gs_args(*d);
+        if (V == 2 || gs_shape(a, V)) continue;
+        const long long n = a.nch > 1 ? 8LL * a.B * a.nch * a.H : 0;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" int gzsl_gated_scan_fwd(const GzslGatedScan* d, void* h, float* h_last, void* work, long long work_bytes, void* stream) {
-    (void)work, (void)work_bytes;
     if (int e = gs_check(d)) return e;
     if (d->B == 0) return d->rows == 0 ? 0 : GZSL_EINVAL;
     if (!h_last || (d->rows > 0 && !h)) return GZSL_EINVAL;
     GsArgs a = gs_args(*d);
     a.h = h, a.last = h_last;
-    return d->dtype == GZSL_F32 ? gs_fwd<float>(a, (hipStream_t)stream) : gs_fwd<bf16>(a, (hipStream_t)stream);
+    const int V = gs_width(*d, (uintptr_t)d->gates | (uintptr_t)d->cands | (uintptr_t)h);
+    return gs_run<false>(*d, a, V, work, work_bytes, (hipStream_t)stream);
 }
 
 extern "C" int gzsl_gated_scan_bwd(const GzslGatedScan* d, const void* h, const void* dh, const float* dlast, void* dgates, void* dcands, float* dh0,
                                    void* work, long long work_bytes, void* stream) {
-    (void)work, (void)work_bytes;
     if (int e = gs_check(d)) return e;
     if (d->B == 0) return d->rows == 0 ? 0 : GZSL_EINVAL;
     if (d->rows > 0 && (!h || !dgates || !dcands)) return GZSL_EINVAL;
     GsArgs a = gs_args(*d);
     a.ch = h, a.dh = dh, a.dlast = dlast, a.dg = dgates, a.dc = dcands, a.dh0 = dh0;
-    return d->dtype == GZSL_F32 ? gs_bwd<float>(a, (hipStream_t)stream) : gs_bwd<bf16>(a, (hipStream_t)stream);
+    const int V = gs_width(*d, (uintptr_t)d->gates | (uintptr_t)d->cands | (uintptr_t)h | (uintptr_t)dh | (uintptr_t)dgates | (uintptr_t)dcands);
+    return gs_run<true>(*d, a, V, work, work_bytes, (hipStream_t)stream);
 }
 
 extern "C" int gzsl_gated_scan_step(const void* gates, const void* cands, float* state, const uint8_t* active, int B, int H, long long ldg,

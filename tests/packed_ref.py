@@ -99,7 +99,13 @@ def within(got, want, what):
 
 
 def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
-    """dict of name -> (value, bound): h, last and, with dh / dlast (either may be None), dg, dc, dh0."""
+    """dict of name -> (value, bound): h, last and, with dh / dlast (either may be None), dg, dc, dh0.
+
+    The state is a sum of terms (a product of gates) * (z c) or * h0.  A kernel may run through the steps or join pieces
+    (A2 A1, A2 B1 + B2); either way a term passes through each of its gates once (every gate a few roundings off, 8 u with the
+    product) and through one addition per step or join, so its error is at most the number of its steps times 10 u, relative to
+    the TERM: cancellation between terms does not shrink it.  The bound is therefore the recurrence of the terms' magnitudes,
+    m_t = a_t m_{t-1} + |z_t c_t|, with e_t = a_t e_{t-1} + 10 u m_t; 30 u m on top for the joins (at most 30 levels)."""
     step = half_step(gates.dtype)
     g, c = gates.detach().cpu().double(), cands.detach().cpu().double()
     R, H = g.shape
@@ -112,23 +118,25 @@ def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
         if reverse:
             rows.reverse()
         h = z(H) if h0 is None else h0[b].detach().cpu().double()
-        e = z(H)
+        e, m = z(H), h.abs()
         before, ebefore = z(R, H), z(R, H)
         for r in rows:
-            before[r], ebefore[r] = h, e
+            before[r], ebefore[r] = h, e + 30 * U * m
             t1, t2 = aa[r] * h, zz[r] * c[r]
-            # each gate is off by a few roundings of the exponential and the division, each product by one more
-            e = aa[r] * e + 8 * U * (t1.abs() + t2.abs())
+            m = aa[r] * m + t2.abs()
+            e = aa[r] * e + 10 * U * m
             h = t1 + t2
-            out['h'][0][r], out['h'][1][r] = h, e + (h.abs() + e) * step
-        out['last'][0][b], out['last'][1][b] = h, e + U * h.abs()
+            out['h'][0][r], out['h'][1][r] = h, e + 30 * U * m + (h.abs() + e) * step
+        out['last'][0][b], out['last'][1][b] = h, e + 30 * U * m
         if dh is None and dlast is None:
             continue
         carry = z(H) if dlast is None else dlast[b].detach().cpu().double()
-        ec = z(H)
+        ec, m = z(H), carry.abs()
         for r in reversed(rows):
-            lam = carry + (0 if dh is None else dh[r].detach().cpu().double())
-            el = ec + U * lam.abs()
+            up = z(H) if dh is None else dh[r].detach().cpu().double()
+            lam = carry + up
+            m = m + up.abs()
+            el = ec + 31 * U * m
             out['dc'][0][r] = lam * zz[r]
             out['dc'][1][r] = (el + 8 * U * lam.abs()) * zz[r]
             d = c[r] - before[r]
@@ -137,9 +145,10 @@ def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
             ed = ebefore[r] + (before[r].abs() + ebefore[r]) * step + U * (c[r].abs() + before[r].abs())
             out['dg'][0][r] = lam * d * w
             out['dg'][1][r] = w * ((el + 20 * U * lam.abs()) * (d.abs() + ed) + lam.abs() * ed)
-            ec = aa[r] * el + 8 * U * (aa[r] * lam).abs()
+            m = aa[r] * m
+            ec = aa[r] * ec + 10 * U * m
             carry = aa[r] * lam
-        out['dh0'][0][b], out['dh0'][1][b] = carry, ec + U * carry.abs()
+        out['dh0'][0][b], out['dh0'][1][b] = carry, ec + 30 * U * m
     for name in ('dg', 'dc'):
         val, err = out[name]
         err += (val.abs() + err) * step
