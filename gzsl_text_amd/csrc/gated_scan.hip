@@ -13,6 +13,9 @@
 #include "packed.h"
 #include "../../include/gzsl_hip.h"
 
+#define GS_THREADS 256
+#define GS_LOG2E 1.4426950408889634f
+
 struct GsArgs {
     const void *g, *c;
     const int64_t* spans;
@@ -29,12 +32,19 @@ struct GsArgs {
     int ncg, nblk, TS, tiles, chunk, nch;    // channel groups of a workgroup, workgroups over the channels, threads over time, tiles of a chunk
 };
 
-// z = sigmoid(g) and a = 1 - z = sigmoid(-g), both to full relative accuracy (e^-|g| never overflows)
+// z = sigmoid(g), a = 1 - z = sigmoid(-g).  fp32: both to a few roundings of their own size (e^-|g| never overflows; its exponent
+// |g| log2(e) is rounded once: |g| half steps), which the backward's z a needs.  The forward of
+// bf16 tensors takes a as the difference, off by a few half steps of 1: it only multiplies the state.
+template <typename T, bool BWD>
 __device__ __forceinline__ void gs_gate(float g, float& z, float& a) {
-    const float e = expf(-fabsf(g)), big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
-    z = g >= 0.f ? big : small;
-    a = g >= 0.f ? small : big;
-    if (g != g) z = a = g;
+    if (sizeof(T) == 2 && !BWD) {
+        z = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -GS_LOG2E));
+        a = 1.f - z;
+    } else {
+        const float e = __builtin_amdgcn_exp2f(fabsf(g) * -GS_LOG2E), big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
+        z = g >= 0.f ? big : small;
+        a = g >= 0.f ? small : big;
+    }
 }
 
 template <typename T, int V>
@@ -123,7 +133,7 @@ __device__ __forceinline__ GsPlace gs_place(const GsArgs& a, int V) {
 }
 
 template <typename T, int V, int S, bool BWD>
-__global__ __launch_bounds__(512) void gs_chunk_kernel(GsArgs a) {
+__global__ __launch_bounds__(GS_THREADS) void gs_chunk_kernel(GsArgs a) {
     extern __shared__ float sh[];
     const GsPlace p = gs_place(a, V);
     const NoteSpan sp = note_span(a.spans, p.b, a.rows, a.max_len);
@@ -149,7 +159,7 @@ __global__ __launch_bounds__(512) void gs_chunk_kernel(GsArgs a) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float z, k;
-                gs_gate(g[s][v], z, k);
+                gs_gate<T, BWD>(g[s][v], z, k);
                 if (BWD) B[v] = k * (B[v] + (a.dh ? u[s][v] : 0.f));
                 else B[v] = fmaf(k, B[v], z * u[s][v]);
                 A[v] *= k;
@@ -165,7 +175,7 @@ __global__ __launch_bounds__(512) void gs_chunk_kernel(GsArgs a) {
 }
 
 template <typename T, int V, int S, bool BWD>
-__global__ __launch_bounds__(512) void gs_apply_kernel(GsArgs a) {
+__global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
     extern __shared__ float sh[];
     const GsPlace p = gs_place(a, V);
     const NoteSpan sp = note_span(a.spans, p.b, a.rows, a.max_len);
@@ -252,7 +262,7 @@ __global__ __launch_bounds__(512) void gs_apply_kernel(GsArgs a) {
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gs_gate(k[s][v], z[s][v], k[s][v]);
+                gs_gate<T, BWD>(k[s][v], z[s][v], k[s][v]);
                 if (i0 + s >= sp.len) k[s][v] = 1.f, u[s][v] = c[s][v] = z[s][v] = 0.f;
                 if (BWD) {
                     B[v] = k[s][v] * (B[v] + u[s][v]);
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(256) void gs_step_kernel(const T* g, const T* c, fl
     const int ch = (int)(i - b * H);
     if (active && !active[b]) return;
     float z, k;
-    gs_gate((float)g[b * ldg + ch], z, k);
+    gs_gate<T, false>((float)g[b * ldg + ch], z, k);
     state[i] = fmaf(k, state[i], z * (float)c[b * ldc + ch]);
 }
 
@@ -336,13 +346,13 @@ static int gs_width(const GzslGatedScan& d, uintptr_t addresses) {
         if (d.H % V == 0 && d.ldg % V == 0 && d.ldc % V == 0 && addresses % (uintptr_t)(V * sz) == 0) return V;
     return 1;
 }
-// S V = 32 values of each operand in a thread's registers; up to 512 threads of at most 64 channel groups.
+// S V = 32 values of each operand in a thread's registers; up to GS_THREADS threads of at most 64 channel groups.
 static int gs_steps(int V) { return V == 8 ? 4 : 8; }
 static int gs_shape(GsArgs& a, int V) {
     const int groups = (a.H + V - 1) / V;
     a.ncg = groups < 64 ? groups : 64;
     a.nblk = (groups + a.ncg - 1) / a.ncg;
-    a.TS = 512 / a.ncg;
+    a.TS = GS_THREADS / a.ncg;
     const long long tile = (long long)a.TS * gs_steps(V), all = (a.max_len + tile - 1) / tile, wgs = all * a.B * a.nblk;
     // a chunk is one tile until that makes over 1024 workgroups (four to a compute unit) or over 256 chunks to look back at
     long long m = wgs / 1024;

@@ -102,10 +102,10 @@ def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
     """dict of name -> (value, bound): h, last and, with dh / dlast (either may be None), dg, dc, dh0.
 
     The state is a sum of terms (a product of gates) * (z c) or * h0.  A kernel may run through the steps or join pieces
-    (A2 A1, A2 B1 + B2); either way a term passes through each of its gates once (every gate a few roundings off, 8 u with the
-    product) and through one addition per step or join, so its error is at most the number of its steps times 10 u, relative to
+    (A2 A1, A2 B1 + B2); either way a term passes through each of its gates once (a gate is off by a few roundings of its
+    own size, and by |g| u where it is the small one of the two, from the rounded exponent) and through one addition per step or join, so its error is at most the number of its steps times 10 u, relative to
     the TERM: cancellation between terms does not shrink it.  The bound is therefore the recurrence of the terms' magnitudes,
-    m_t = a_t m_{t-1} + |z_t c_t|, with e_t = a_t e_{t-1} + 10 u m_t; 30 u m on top for the joins (at most 30 levels)."""
+    m_t = a_t m_{t-1} + |z_t c_t|, with e_t = a_t e_{t-1} + (10 + |g_t|) u m_t; 30 u m on top for the joins (at most 30 levels)."""
     step = half_step(gates.dtype)
     g, c = gates.detach().cpu().double(), cands.detach().cpu().double()
     R, H = g.shape
@@ -123,8 +123,9 @@ def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
         for r in rows:
             before[r], ebefore[r] = h, e + 30 * U * m
             t1, t2 = aa[r] * h, zz[r] * c[r]
+            coarse = 5 * U * m if step > U else 0  # (bf16 tensors: the forward takes 1 - z, off by a few u of 1)
             m = aa[r] * m + t2.abs()
-            e = aa[r] * e + 10 * U * m
+            e = aa[r] * e + (10 + g[r].abs().nan_to_num(0, 0, 0)) * U * m + coarse
             h = t1 + t2
             out['h'][0][r], out['h'][1][r] = h, e + 30 * U * m + (h.abs() + e) * step
         out['last'][0][b], out['last'][1][b] = h, e + 30 * U * m
@@ -138,15 +139,16 @@ def scan_ref(gates, cands, spans, h0=None, reverse=False, dh=None, dlast=None):
             m = m + up.abs()
             el = ec + 31 * U * m
             out['dc'][0][r] = lam * zz[r]
-            out['dc'][1][r] = (el + 8 * U * lam.abs()) * zz[r]
+            gr = g[r].abs().nan_to_num(0, 0, 0)
+            out['dc'][1][r] = (el + (8 + gr) * U * lam.abs()) * zz[r]
             d = c[r] - before[r]
             w = zz[r] * aa[r]
             # the backward reads h as it was stored: one rounding to the tensors' type on top of its error
             ed = ebefore[r] + (before[r].abs() + ebefore[r]) * step + U * (c[r].abs() + before[r].abs())
             out['dg'][0][r] = lam * d * w
-            out['dg'][1][r] = w * ((el + 20 * U * lam.abs()) * (d.abs() + ed) + lam.abs() * ed)
+            out['dg'][1][r] = w * ((el + (20 + gr) * U * lam.abs()) * (d.abs() + ed) + lam.abs() * ed)
             m = aa[r] * m
-            ec = aa[r] * ec + 10 * U * m
+            ec = aa[r] * ec + (10 + gr) * U * m
             carry = aa[r] * lam
         out['dh0'][0][b], out['dh0'][1][b] = carry, ec + 30 * U * m
     for name in ('dg', 'dc'):

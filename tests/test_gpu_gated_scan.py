@@ -160,7 +160,9 @@ def test_step_form(ops, ext, dtype, B, H):
     gd, cd, s = g.cpu().double(), c.cpu().double(), old.cpu().double()
     t1, t2 = torch.sigmoid(-gd) * s, torch.sigmoid(gd) * cd
     on = active.cpu()
-    within(state[active], ((t1 + t2)[on], (8 * U * (t1.abs() + t2.abs()) + U * (t1 + t2).abs())[on]), 'state')
+    # the gates: a few roundings and the rounded exponent's |g| u; bf16 tensors take 1 - z, off by u of 1
+    tol = (8 + gd.abs()) * U * (t1.abs() + t2.abs()) + U * (t1 + t2).abs() + (2 * U * s.abs() if dtype == torch.bfloat16 else 0)
+    within(state[active], ((t1 + t2)[on], tol[on]), 'state')
     assert torch.equal(state[~active], old[~active])
     s2 = old.clone()
     ops.gated_scan_step_(g, c, s2, active)
