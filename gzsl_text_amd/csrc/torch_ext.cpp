@@ -414,7 +414,7 @@ Tensor adamw_clip_step_(at::TensorList params, at::TensorList grads, at::TensorL
     Tensor norm = at::empty({}, opt);
     const Tensor work = scratch(gzsl_clip_work_bytes(n.data(), (int)n.size()), norm, "adamw_clip_step_");
     check_rc(gzsl_adamw_clip_step((float* const*)p.data(), (const float* const*)g.data(), (float* const*)mm.data(), (float* const*)vv.data(), n.data(),
-                                  (int)n.size(), (float)max_norm, (float)lr, (float)beta1, (float)beta2, (float)eps, (float)wd, norm.data_ptr<float>(),
+                                  (int)n.size(), (float)max_norm, lr, beta1, beta2, eps, wd, norm.data_ptr<float>(),
                                   work.data_ptr(), work.numel(), cur_stream()),
              "gzsl_adamw_clip_step");
     for (const at::TensorList ts : {params, m, v})

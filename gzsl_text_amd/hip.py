@@ -106,7 +106,7 @@ _PROTOS = {
     'gzsl_gated_scan_step': [c_void_p] * 4 + [c_int, c_int, c_ll, c_ll, c_int, c_void_p],
     'gzsl_clip_work_bytes': [c_void_p, c_int],
     'gzsl_clip_grad_norm': [c_void_p] * 3 + [c_int, c_float, c_void_p, c_void_p, c_ll, c_void_p],
-    'gzsl_adamw_clip_step': [c_void_p] * 5 + [c_int] + [c_float] * 6 + [c_void_p, c_void_p, c_ll, c_void_p],
+    'gzsl_adamw_clip_step': [c_void_p] * 5 + [c_int, c_float] + [ctypes.c_double] * 5 + [c_void_p, c_void_p, c_ll, c_void_p],
 }
 
 _lib = None

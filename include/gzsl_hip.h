@@ -328,9 +328,9 @@ long long gzsl_clip_work_bytes(const long long* sizes, int n);
 int gzsl_clip_grad_norm(void* const* grads, const long long* sizes, const int* dtypes, int n, float max_norm, float* norm,
                         void* work, long long work_bytes, void* stream);
 /* gzsl_adamw_nobias_step (common_module.py:138-182) over n tensors with the gradients clipped on the way: f as above, the
- * update of every tensor from f*g.  The gradients are left as they are. */
+ * update of every tensor from f*g, with 1 - beta taken in 64 bits before it is rounded.  The gradients are left as they are. */
 int gzsl_adamw_clip_step(float* const* p, const float* const* g, float* const* m, float* const* v, const long long* sizes, int n,
-                         float max_norm, float lr, float beta1, float beta2, float eps, float wd, float* norm, void* work,
+                         float max_norm, double lr, double beta1, double beta2, double eps, double wd, float* norm, void* work,
                          long long work_bytes, void* stream);
 
 /* library self-description: number of exported compute entry points and build target string */
