@@ -24,19 +24,3 @@ __device__ __forceinline__ NoteSpan note_span(const int64_t* spans, int b, long 
     if (n > max_len) n = max_len;
     return {s, n < 0 ? 0 : (int)n};
 }
-
-// Rows that belong to no note read as zero: those before the first note and those behind each note (spans ascend).
-template <typename T>
-static __global__ __launch_bounds__(256) void zero_gaps_kernel(const int64_t* spans, long long rows, int B, int max_len, T* x, int Wx, T* y, int Wy) {
-    const int b = (int)blockIdx.y - 1;  // -1: in front of note 0
-    long long r0 = 0, r1 = rows;
-    if (b >= 0) {
-        const NoteSpan sp = note_span(spans, b, rows, max_len);
-        r0 = sp.start + sp.len;
-    }
-    if (b + 1 < B) r1 = note_span(spans, b + 1, rows, max_len).start;
-    const long long step = (long long)gridDim.x * 256, first = (long long)blockIdx.x * 256 + threadIdx.x;
-    for (long long i = r0 * Wx + first; i < r1 * Wx; i += step) x[i] = (T)0.f;
-    if (y)
-        for (long long i = r0 * Wy + first; i < r1 * Wy; i += step) y[i] = (T)0.f;
-}

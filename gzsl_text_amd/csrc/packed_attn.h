@@ -23,9 +23,9 @@
 #include "rng.h"
 #include "../../include/gzsl_hip.h"
 
-#define PA_ROWS 32  // rows (tokens or labels) of a tile image
 #define PA_LOG2E 1.4426950408889634f
 #define PA_LN2 0.6931471805599453f
+#define PA_TILE 64  // tokens of a workgroup in the dK / dV sweep
 
 template <typename T>
 struct PaTy;
@@ -38,15 +38,18 @@ struct PaTy<bf16> {
     typedef bf16x8 frag;
 };
 
-// NE / NF: 16-wide tiles of the key / value width (E <= 16 NE, F <= 16 NF).
+// NE / NF: 16-wide tiles of the key / value width (E <= 16 NE, F <= 16 NF).  A tile image holds one k step of the second
+// product: 32 rows of bf16, 16 of fp32.
 template <typename T, int NE_, int NF_>
 struct PaGeo {
-    static constexpr int NE = NE_, NF = NF_, SZ = sizeof(T), KF = 16 / SZ, KK = 4 * KF, KS = PA_ROWS / KK;
+    static constexpr int NE = NE_, NF = NF_, SZ = sizeof(T), KF = 16 / SZ, ROWS = 4 * KF, U = ROWS / 16;
     static constexpr int SE = (NE * 16 * SZ + 63) / 64, SF = (NF * 16 * SZ + 63) / 64;  // 64-byte k steps over e / f
     static constexpr int PE = 64 * SE + 32, PF = 64 * SF + 32;                          // row pitches in bytes
-    static constexpr int EB = PA_ROWS * PE, FB = PA_ROWS * PF;                          // image bytes (whole KB)
-    static constexpr int KV = EB + FB;                                                  // token tile: keys, values
-    static constexpr int OB = FB + 1024;                                                // label tile of dO: rows, lse[32], delta[32]
+    static constexpr int EB = ROWS * PE, FB = ROWS * PF;
+    static constexpr int KV = EB + FB;                                  // token tile: keys, values
+    static constexpr int QB = (EB + 1023) / 1024 * 1024;                // label tile: queries
+    static constexpr int OB = (FB + 12 * ROWS + 1023) / 1024 * 1024;    // label tile: dO rows, then off[], scale[], delta[] of its labels
+    static_assert(KV % 1024 == 0, "whole KB: the copies move 1 KB per wave instruction");
 };
 
 __device__ __forceinline__ f32x4 pa_mma(f32x4 a, f32x4 b, f32x4 c) {
@@ -78,11 +81,11 @@ __device__ __forceinline__ bf16x8 pa_col<bf16>(const char* img, int pitch, int r
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(p + 16 * pitch));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-// accumulator registers of the two 16-row score tiles -> operand fragment of k step ks
-__device__ __forceinline__ void pa_pack(const float (&p)[2][4], int ks, f32x4& out) {
-    out = f32x4{p[ks][0], p[ks][1], p[ks][2], p[ks][3]};
+// accumulator registers of the tile's 16-row score tiles -> operand fragment
+__device__ __forceinline__ void pa_pack(const float (&p)[1][4], f32x4& out) {
+    out = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]};
 }
-__device__ __forceinline__ void pa_pack(const float (&p)[2][4], int, bf16x8& out) {
+__device__ __forceinline__ void pa_pack(const float (&p)[2][4], bf16x8& out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = (bf16)p[j >> 2][j & 3];
 }
@@ -130,15 +133,136 @@ struct PaArgs {
     float cap;
     uint32_t l_offset, L_total, seed, thresh;
     float scale;
+    int nLT, extra;                   // label workgroups of a note; token chunks beyond one a note (0: notes are not cut)
+    int shares, slots;                // dK / dV: label shares of a token tile at most, slabs that the workspace has room for
     // workspace
     char *KV, *Q, *DO;
-    float *part, *ml;    // forward, split over tokens: unnormalised O [split][B][L][F] and (max, sum) [split][B][L][2]
-    float *dq, *dkv;     // backward: [slab][L][E]; [split][rows][E + F]
-    int nsplit;          // token splits (forward, dQ) or label splits (dK / dV) of a launch
+    float *part, *ml;  // forward, notes cut: unnormalised O [chunk][L][F] and (max, sum) [chunk][L][2]
+    float *dq, *dkv;   // backward: [chunk][L][E]; [unit][PA_TILE][E + F]
     // results and the backward's inputs
     void* O;
-    float* LSE;
+    float *LSE, *rest;  // rest: (max in log 2, 1 / sum) [B][L][2], then for bf16 what the rounding of O dropped, [B][L][F]
     const void *cO, *dO;
-    const float* cLSE;
+    const float *cLSE, *crest;
     void *dK, *dV, *dQ;
 };
+
+// ---- how the work is cut.  The host knows max_len, not the lengths: every wave works the cut out from the span table, so the
+// kernels agree on it without a table in memory.  Per 64 notes: one load and a few lane exchanges.
+struct PaUnit {
+    int b, c, nch;        // note, its chunk, the note's chunks
+    int chunk, ci, all;   // tokens of a chunk, number of this chunk among all, chunks in all
+    NoteSpan sp;
+};
+// Chunks of ROWS-aligned `chunk` tokens, about a.extra of them beyond one a note.  Up to 64 notes are taken longest first, so
+// that the last workgroups of the grid are the short ones; more notes are taken in their order.
+template <int ROWS>
+__device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = -1) {
+    const int lane = threadIdx.x & 63;
+    PaUnit u;
+    u.ci = ci;
+    u.b = -1;
+    int chunk = 0x7FFFFFC0;
+    auto length = [&](int b) { return b < a.B ? note_span(a.spans, b, a.rows, a.max_len).len : 0; };
+    int len = length(lane);
+    if (a.extra > 0) {
+        long long n = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) n += b0 ? length(b0 + lane) : len;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+        long long per = (n + a.extra - 1) / a.extra;
+        if (per < 256) per = 256;  // a share that pays for its own start and its part in the join
+        chunk = (int)min(per / ROWS * ROWS + ROWS, (long long)0x7FFFFFC0);
+    }
+    u.chunk = chunk;
+    int base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int note = b0 + lane;
+        if (b0) len = length(note);
+        if (a.B <= 64) {  // order by length, longest first (ties: lower note first)
+            int rank = 0;
+            for (int j = 0; j < a.B; ++j) {
+                const int other = __builtin_amdgcn_readlane(len, j);
+                rank += other > len || (other == len && j < lane);
+            }
+            if (lane >= a.B) rank = lane;
+            note = __builtin_amdgcn_ds_permute(rank << 2, note);
+            len = __builtin_amdgcn_ds_permute(rank << 2, len);
+        }
+        const int nch = note < a.B ? max(1, (len + chunk - 1) / chunk) : 0;
+        int incl = nch;  // chunks up to and with this lane
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(incl, o);
+            if (lane >= o) incl += x;
+        }
+        const unsigned long long hit = want_b >= 0 ? __ballot(note == want_b) : __ballot(base + incl > ci);
+        if (u.b < 0 && hit) {
+            const int src = __ffsll((long long)hit) - 1;
+            u.b = __shfl(note, src);
+            u.nch = __shfl(nch, src);
+            const int first = base + __shfl(incl, src) - u.nch;
+            u.c = ci - first;
+            if (want_b >= 0) u.c = 0, u.ci = first;
+        }
+        base += __shfl(incl, 63);
+    }
+    u.all = base;
+    if (u.b >= 0) u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+    return u;
+}
+// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  The parts are as many as fill the chip's 512 places
+// (two workgroups a compute unit) best, a slab written and read again counted as 1 % a part.
+struct PaTileUnit {
+    int b, tile, share, shares, unit, tiles;
+    NoteSpan sp;
+};
+__device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, int want_b = -1) {
+    const int lane = threadIdx.x & 63;
+    PaTileUnit u;
+    u.b = -1;
+    auto tiles_of = [&](int b) { return b < a.B ? (note_span(a.spans, b, a.rows, a.max_len).len + PA_TILE - 1) / PA_TILE : 0; };
+    int n = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) n += tiles_of(b0 + lane);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    u.tiles = n;
+    u.shares = 1;
+    float best = -1.f;
+    for (int s = 1; s <= a.shares && (s == 1 || (long long)n * s <= a.slots); ++s) {
+        const int all = n * s, rounds = (all + 511) / 512;
+        const float fill = rounds > 0 ? (float)all / (512.f * rounds) - 0.01f * s : 0.f;
+        if (fill > best) best = fill, u.shares = s;
+    }
+    u.unit = unit;
+    const int t = unit / u.shares;
+    u.share = unit % u.shares;
+    int base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int nt = tiles_of(b0 + lane);
+        int incl = nt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(incl, o);
+            if (lane >= o) incl += x;
+        }
+        const unsigned long long hit = want_b >= 0 ? __ballot(b0 + lane == want_b) : __ballot(base + incl > t);
+        if (u.b < 0 && hit) {
+            const int src = __ffsll((long long)hit) - 1, first = base + __shfl(incl, src) - __shfl(nt, src);
+            u.b = b0 + src;
+            u.tile = want_b >= 0 ? first : t - first;  // want_b: the note's first tile among all
+        }
+        base += __shfl(incl, 63);
+    }
+    if (u.b >= 0) u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+    return u;
+}
+
+struct PaPlan {
+    int nT, nQ, wide, waves, extra, shares, slots, nLT;
+    long long units;  // workgroups of the dK / dV sweep
+    long long kv, q, dO, part, ml, dq, dkv, bytes;
+};
+// packed_attn_f32.hip / packed_attn_bf16.hip
+int pa_run_f32(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);
+int pa_run_bf16(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);

@@ -218,7 +218,7 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         return d;
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& spans,
-                                 int64_t max_len, double cap, double p_drop, int64_t seed, int64_t l_offset, int64_t L_total) {
+                                 int64_t max_len, double cap, double p_drop, int64_t seed, int64_t l_offset, int64_t L_total, bool grad) {
         const int t = type_of(keys, "keys");
         TORCH_CHECK(type_of(values, "values") == t && type_of(queries, "queries") == t, "gzsl: keys, values and queries must have one type");
         const Tensor k = rows_of(keys, "keys"), v = rows_of(values, "values"), q = rows_of(queries, "queries");
@@ -235,20 +235,24 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         const GzslPackedAttn d = describe(k, v, q, spans, max_len, cap, p_drop, seed, l_offset, L_total);
         Tensor O = at::empty({d.B, d.L, d.F}, v.options()), lse = at::empty({d.B, d.L}, v.options().dtype(at::kFloat));
         const Tensor work = scratch(gzsl_packed_attn_work_bytes(&d, 0), k, "packed_label_attention");
-        check_rc(gzsl_packed_attn_fwd(&d, O.data_ptr(), lse.data_ptr<float>(), work.data_ptr(), work.numel(), cur_stream()), "gzsl_packed_attn_fwd");
-        ctx->save_for_backward({k, v, q, spans, O, lse});
+        Tensor rest;
+        if (grad) rest = scratch(gzsl_packed_attn_rest_bytes(&d), k, "packed_label_attention");
+        check_rc(gzsl_packed_attn_fwd(&d, O.data_ptr(), lse.data_ptr<float>(), grad ? rest.data_ptr() : nullptr, work.data_ptr(), work.numel(), cur_stream()),
+                 "gzsl_packed_attn_fwd");
+        ctx->mark_non_differentiable({lse});
+        if (!grad) return {O, lse};
+        ctx->save_for_backward({k, v, q, spans, O, lse, rest});
         ctx->saved_data["max_len"] = max_len;
         ctx->saved_data["cap"] = cap;
         ctx->saved_data["p"] = p_drop;
         ctx->saved_data["seed"] = seed;
         ctx->saved_data["l_offset"] = l_offset;
         ctx->saved_data["L_total"] = L_total;
-        ctx->mark_non_differentiable({lse});
         return {O, lse};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &k = saved[0], &v = saved[1], &q = saved[2], &spans = saved[3], &O = saved[4], &lse = saved[5];
+        const Tensor &k = saved[0], &v = saved[1], &q = saved[2], &spans = saved[3], &O = saved[4], &lse = saved[5], &rest = saved[6];
         const c10::DeviceGuard guard(k.device());
         const GzslPackedAttn d = describe(k, v, q, spans, ctx->saved_data["max_len"].toInt(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["p"].toDouble(),
                                           ctx->saved_data["seed"].toInt(), ctx->saved_data["l_offset"].toInt(), ctx->saved_data["L_total"].toInt());
@@ -258,16 +262,17 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         } else {
             const Tensor dO = grads[0].contiguous();
             const Tensor work = scratch(gzsl_packed_attn_work_bytes(&d, 1), k, "packed_label_attention");
-            check_rc(gzsl_packed_attn_bwd(&d, O.data_ptr(), lse.data_ptr<float>(), dO.data_ptr(), dK.data_ptr(), dV.data_ptr(), dQ.data_ptr(), work.data_ptr(),
+            check_rc(gzsl_packed_attn_bwd(&d, O.data_ptr(), lse.data_ptr<float>(), rest.data_ptr(), dO.data_ptr(), dK.data_ptr(), dV.data_ptr(), dQ.data_ptr(), work.data_ptr(),
                                           work.numel(), cur_stream()),
                      "gzsl_packed_attn_bwd");
         }
-        return {dK, dV, dQ, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dK, dV, dQ, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 std::tuple<Tensor, Tensor> packed_label_attention(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& spans, int64_t max_len,
                                                   double cap, double p_drop, int64_t seed, int64_t l_offset, int64_t L_total) {
-    auto out = PackedLabelAttention::apply(keys, values, queries, spans, max_len, cap, p_drop, seed, l_offset, L_total);
+    const bool grad = at::GradMode::is_enabled() && (keys.requires_grad() || values.requires_grad() || queries.requires_grad());
+    auto out = PackedLabelAttention::apply(keys, values, queries, spans, max_len, cap, p_drop, seed, l_offset, L_total, grad);
     return {out[0], out[1]};
 }
 

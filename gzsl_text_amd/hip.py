@@ -98,8 +98,9 @@ _PROTOS = {
     'gzsl_gan_gen_head': [c_void_p] * 7 + [c_int, c_int, c_void_p],
     'gzsl_adam_flat_step': [c_void_p] * 4 + [c_ll] + [c_float] * 4 + [c_void_p, c_void_p],
     'gzsl_packed_attn_work_bytes': [ctypes.POINTER(GzslPackedAttn), c_int],
-    'gzsl_packed_attn_fwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 3 + [c_ll, c_void_p],
-    'gzsl_packed_attn_bwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 7 + [c_ll, c_void_p],
+    'gzsl_packed_attn_rest_bytes': [ctypes.POINTER(GzslPackedAttn)],
+    'gzsl_packed_attn_fwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 4 + [c_ll, c_void_p],
+    'gzsl_packed_attn_bwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 8 + [c_ll, c_void_p],
     'gzsl_gated_scan_work_bytes': [ctypes.POINTER(GzslGatedScan), c_int],
     'gzsl_gated_scan_fwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 3 + [c_ll, c_void_p],
     'gzsl_gated_scan_bwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 7 + [c_ll, c_void_p],
@@ -129,7 +130,7 @@ def load():
     for name, argtypes in _PROTOS.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
-        fn.restype = c_ll if name.endswith(('_work_floats', '_work_bytes')) else c_int
+        fn.restype = c_ll if name.endswith(('_work_floats', '_work_bytes', '_rest_bytes')) else c_int
     lib.gzsl_build_info.restype = ctypes.c_char_p
     lib.gzsl_build_info.argtypes = []
     _lib = lib

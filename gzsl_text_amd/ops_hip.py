@@ -509,29 +509,37 @@ class HipOps:
                                l_offset, L_total, seed & 0xFFFFFFFF, th, sc)
         return d, (keys, values, queries)  # (the tensors: a contiguous copy must outlive the launch)
 
-    def attn_packed_fwd(self, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0):
-        """(O [B,L,F], lse [B,L]): label attention over packed notes (gzsl_packed_attn_fwd).  keys [R,E], values [R,F],
-        queries [L,E], all fp32 or all bf16; spans [B,2] int64 = (first row, rows) per note, ascending and disjoint."""
+    def attn_packed_fwd(self, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0,
+                        need_grad=True):
+        """(O [B,L,F], lse [B,L], rest): label attention over packed notes (gzsl_packed_attn_fwd).  keys [R,E], values [R,F],
+        queries [L,E], all fp32 or all bf16; spans [B,2] int64 = (first row, rows) per note, ascending and disjoint.  `rest`
+        is for attn_packed_bwd (softmax statistics; bf16: what the rounding of O dropped); None without need_grad."""
         d, hold = self._packed_attn(keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p)
         O = torch.empty((d.B, d.L, d.F), dtype=values.dtype, device=values.device)
         lse = torch.empty((d.B, d.L), dtype=torch.float32, device=values.device)
         work = self._work('gzsl_packed_attn_work_bytes', d, 0, values.device)
-        call('gzsl_packed_attn_fwd', d, ptr(O), ptr(lse), ptr(work), work.numel())
+        rest = None
+        if need_grad:
+            rest = torch.empty(max(hip.load().gzsl_packed_attn_rest_bytes(d), 16), dtype=torch.uint8, device=values.device)
+        call('gzsl_packed_attn_fwd', d, ptr(O), ptr(lse), ptr(rest), ptr(work), work.numel())
         del hold
-        return O, lse
+        return O, lse, rest
 
-    def attn_packed_bwd(self, dO, O, lse, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0):
-        """(dkeys [R,E], dvalues [R,F], dqueries [L,E]) of attn_packed_fwd; rows of no note get zeros."""
+    def attn_packed_bwd(self, dO, O, lse, rest, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0):
+        """(dkeys [R,E], dvalues [R,F], dqueries [L,E]) of attn_packed_fwd; rows of no note get zeros.  rest=None: from lse and
+        the rounded O alone."""
         d, hold = self._packed_attn(keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p)
         self._dtype(keys, dO, O)
         if tuple(dO.shape) != (d.B, d.L, d.F) or dO.shape != O.shape or tuple(lse.shape) != (d.B, d.L):
             raise RuntimeError(f'dO {tuple(dO.shape)}, O {tuple(O.shape)}, lse {tuple(lse.shape)} do not fit {(d.B, d.L, d.F)}')
         _check_f32(lse)
+        if rest is not None and rest.numel() * rest.element_size() < hip.load().gzsl_packed_attn_rest_bytes(d):
+            raise RuntimeError('rest is not that of this call\'s forward')
         dK, dV, dQ = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (keys, values, queries))
         if d.B == 0 or d.L == 0:
             return dK.zero_(), dV.zero_(), dQ.zero_()
         work = self._work('gzsl_packed_attn_work_bytes', d, 1, dO.device)
-        call('gzsl_packed_attn_bwd', d, ptr(O), ptr(lse), ptr(dO), ptr(dK), ptr(dV), ptr(dQ), ptr(work), work.numel())
+        call('gzsl_packed_attn_bwd', d, ptr(O), ptr(lse), ptr(rest), ptr(dO), ptr(dK), ptr(dV), ptr(dQ), ptr(work), work.numel())
         del hold
         return dK, dV, dQ
 

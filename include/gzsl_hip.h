@@ -292,11 +292,15 @@ typedef struct GzslPackedAttn {
     float drop_scale;
 } GzslPackedAttn;
 long long gzsl_packed_attn_work_bytes(const GzslPackedAttn* d, int backward);
-int gzsl_packed_attn_fwd(const GzslPackedAttn* d, void* O, float* LSE, void* work, long long work_bytes, void* stream);
-/* autograd of the above from its O, LSE and dO [B,L,F]: dkeys [rows,E], dvalues [rows,F], dqueries [L,E] are WRITTEN (not
+/* `rest` (may be NULL): 16-byte aligned, gzsl_packed_attn_rest_bytes(d) bytes that the backward takes: each row's softmax
+ * maximum and sum, and for bf16 what the rounding of O dropped.  Without it the backward works from LSE and the rounded O, whose
+ * rounding then enters the gradients (bf16: about twice their error). */
+long long gzsl_packed_attn_rest_bytes(const GzslPackedAttn* d);
+int gzsl_packed_attn_fwd(const GzslPackedAttn* d, void* O, float* LSE, void* rest, void* work, long long work_bytes, void* stream);
+/* autograd of the above from its O, LSE, rest (or NULL) and dO [B,L,F]: dkeys [rows,E], dvalues [rows,F], dqueries [L,E] are WRITTEN (not
  * accumulated), of the tensors' type and contiguous, zero in rows of no note; sums are taken in a fixed order, without atomics. */
-int gzsl_packed_attn_bwd(const GzslPackedAttn* d, const void* O, const float* LSE, const void* dO, void* dkeys, void* dvalues,
-                         void* dqueries, void* work, long long work_bytes, void* stream);
+int gzsl_packed_attn_bwd(const GzslPackedAttn* d, const void* O, const float* LSE, const void* rest, const void* dO, void* dkeys,
+                         void* dvalues, void* dqueries, void* work, long long work_bytes, void* stream);
 /* Gated linear recurrence over packed notes:  z = sigmoid(gates), h_t = (1 - z_t) h_{t-1} + z_t cands_t, from h0 [B,H] fp32
  * (NULL: 0) through each note's rows, backwards when `reverse`.  h [rows,H] of the tensors' type, contiguous, zero in rows of
  * no note; h_last [B,H] fp32 the state behind each note's last step (h0 for a note of no tokens). */

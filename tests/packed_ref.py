@@ -13,9 +13,9 @@ def half_step(t):
     return torch.finfo(t).eps / 2
 
 
-def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None):
+def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=True):
     """keys [R,E], values [R,F], queries [L,E] (any type, used as the numbers they hold), spans list of (start, n);
-    keep: list of [L,n] dropout factors or None.  Returns dict of name -> (value, bound): O, lse and, with dout [B,L,F],
+    keep: list of [L,n] dropout factors or None; rest: the backward has what the rounding of O dropped.  Returns dict of name -> (value, bound): O, lse and, with dout [B,L,F],
     dK, dV, dQ."""
     step = half_step(values.dtype)
     k, v, q = (x.detach().cpu().double() for x in (keys, values, queries))
@@ -57,7 +57,8 @@ def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None):
         dP = g @ vb.T
         ddP = (F + 2) * U * (g.abs() @ vb.T.abs())
         delta = (g * O).sum(1, keepdim=True)
-        ddelta = (g.abs() * (out['O'][1][b] + (F + 2) * U * O.abs())).sum(1, keepdim=True)
+        ofO = dO_ + (O.abs() + dO_) * step * step if rest else out['O'][1][b]
+        ddelta = (g.abs() * (ofO + (F + 2) * U * O.abs())).sum(1, keepdim=True)
         inner = dP * D - delta
         dS = P * inner * slope
         ddS = P * ((rel + 4 * U) * inner.abs() + ddP * D + ddelta) * (1.0 if cap == 0 else slope.abs())

@@ -53,9 +53,9 @@ SHAPES = [  # lengths, E, F, L: one token, one label, tiles of 32 and workgroups
 @pytest.mark.parametrize('cap', [0.0, 5.0, 50.0])
 def test_forward_and_backward_against_64_bits(ops, lens, E, F, L, dtype, cap):
     k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=len(lens) * 1000 + E + L)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
     assert O.dtype == dtype and lse.dtype == torch.float32
-    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, cap)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, cap)
     ref = attn_ref(k, v, q, sl, cap, do)
     for name, x in (('O', O), ('lse', lse), ('dV', dv), ('dK', dk), ('dQ', dq)):
         within(x, ref[name], name)
@@ -66,8 +66,8 @@ def test_forward_and_backward_against_64_bits(ops, lens, E, F, L, dtype, cap):
 def test_long_axis_is_shared_out_and_joined(ops, lens, L, E, F, dtype):
     """Few labels over many tokens (token shares, joined), few tokens under many labels (label shares, joined)."""
     k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=7)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 8.0)
-    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 8.0)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 8.0)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 8.0)
     ref = attn_ref(k, v, q, sl, 8.0, do)
     for name, x in (('O', O), ('lse', lse), ('dV', dv), ('dK', dk), ('dQ', dq)):
         within(x, ref[name], name)
@@ -81,8 +81,8 @@ def test_long_axis_is_shared_out_and_joined(ops, lens, L, E, F, dtype):
 def test_padded_batch_leaves_its_padding_out(ops, dtype, garbage):
     """A padded batch seen as rows, NaN, infinities or lowest values in the padding and behind the last note."""
     k, v, q, do, spans, max_len, sl = make([37, 0, 70, 1], 36, 52, 41, dtype, seed=3, pitch=75, tail=9, garbage=garbage)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
-    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 30.0)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 30.0)
     ref = attn_ref(k, v, q, sl, 30.0, do)
     for name, x in (('O', O), ('lse', lse), ('dV', dv), ('dK', dk), ('dQ', dq)):
         within(x, ref[name], name)
@@ -97,8 +97,8 @@ def test_padded_batch_leaves_its_padding_out(ops, dtype, garbage):
 def test_dropout_has_the_padded_operators_masks(ops, dtype):
     lens, E, F, L, L_total, l_off, seed, p = [50, 0, 97], 36, 52, 67, 120, 40, 77, 0.2
     k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=5)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 0.0, l_off, L_total, seed, p)
-    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 0.0, l_off, L_total, seed, p)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 0.0, l_off, L_total, seed, p)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 0.0, l_off, L_total, seed, p)
     ref = attn_ref(k, v, q, sl, 0.0, do, dropout_keep(sl, L, seed, p, l_off, L_total))
     for name, x in (('O', O), ('lse', lse), ('dV', dv), ('dK', dk), ('dQ', dq)):
         within(x, ref[name], name)
@@ -110,12 +110,12 @@ def test_full_notes_without_a_cap_agree_with_the_padded_operator(ops, p):
     64-bit value, so they differ by at most twice that."""
     B, T, E, F, L, seed = 3, 150, 100, 200, 90, 9
     k, v, q, do, spans, max_len, sl = make([T] * B, E, F, L, torch.float32, seed=11)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 0.0, 0, L, seed, p)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 0.0, 0, L, seed, p)
     O2, lse2 = ops.attn_fwd(k.view(B, T, E), v.view(B, T, F), q, 0, L, seed, p)
     ref = attn_ref(k, v, q, sl, 0.0, do, dropout_keep(sl, L, seed, p) if p else None)
     within(O, (O2.cpu().double(), 2 * ref['O'][1]), 'O')
     within(lse, (lse2.cpu().double(), 2 * ref['lse'][1]), 'lse')
-    g = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 0.0, 0, L, seed, p)
+    g = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 0.0, 0, L, seed, p)
     g2 = [torch.zeros(B, T, E, device=DEV), torch.zeros(B, T, F, device=DEV), torch.zeros(L, E, device=DEV)]
     ops.attn_bwd(do, O2, k.view(B, T, E), v.view(B, T, F), q, lse2, 0, L, seed, p, *g2)
     for x, y, name in zip(g, g2, ('dK', 'dV', 'dQ')):
@@ -127,8 +127,8 @@ def test_gradients_are_the_slopes_of_the_forward(ops, cap):
     """Central differences of the 64-bit forward along a random direction: their error is the third derivative times
     eps^2 / 6 plus 1e-16 / eps of cancellation, below 1e-6 of the sums of magnitudes here; the kernel's own is the bound."""
     k, v, q, do, spans, max_len, sl = make([19, 33], 20, 24, 17, torch.float32, seed=21)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
-    grads = dict(zip(('dK', 'dV', 'dQ'), ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, cap)))
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
+    grads = dict(zip(('dK', 'dV', 'dQ'), ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, cap)))
     ref = attn_ref(k, v, q, sl, cap, do)
     gen = torch.Generator().manual_seed(2)
     base = [x.cpu().double() for x in (k, v, q)]
@@ -161,12 +161,12 @@ def test_scores_far_outside_the_cap_and_rising_maxima(ops):
     from gzsl_text_amd.packed import note_spans
     spans, max_len, _ = note_spans([130], device=DEV)
     kc = (k * 1e4).to(DEV)
-    O, lse = ops.attn_packed_fwd(kc, v.to(DEV), q.to(DEV), spans, max_len, 3.0)
+    O, lse, rest = ops.attn_packed_fwd(kc, v.to(DEV), q.to(DEV), spans, max_len, 3.0)
     ref = attn_ref(kc, v, q, [(0, 130)], 3.0)
     within(O, ref['O'], 'O at saturation')
     ramp = (k * torch.linspace(0.0, 12.0, 130)[:, None]).to(DEV)
-    O, lse = ops.attn_packed_fwd(ramp, v.to(DEV), q.to(DEV), spans, max_len)
-    dk, dv, dq = ops.attn_packed_bwd(do.to(DEV), O, lse, ramp, v.to(DEV), q.to(DEV), spans, max_len)
+    O, lse, rest = ops.attn_packed_fwd(ramp, v.to(DEV), q.to(DEV), spans, max_len)
+    dk, dv, dq = ops.attn_packed_bwd(do.to(DEV), O, lse, rest, ramp, v.to(DEV), q.to(DEV), spans, max_len)
     ref = attn_ref(ramp, v, q, [(0, 130)], 0.0, do)
     for name, x in (('O', O), ('lse', lse), ('dV', dv), ('dK', dk), ('dQ', dq)):
         within(x, ref[name], name + ' with rising maxima')
@@ -182,8 +182,8 @@ def test_row_pitches_and_alignment(ops, ext, dtype):
         ks, vs, qs = (w[:, off:off + x.shape[1]] for w, x in zip((kw, vw, qw), (k, v, q)))
         for s, x in zip((ks, vs, qs), (k, v, q)):
             s.copy_(x)
-        O, lse = ops.attn_packed_fwd(ks, vs, qs, spans, max_len, 4.0)
-        got = (O, lse, *ops.attn_packed_bwd(do, O, lse, ks, vs, qs, spans, max_len, 4.0))
+        O, lse, rest = ops.attn_packed_fwd(ks, vs, qs, spans, max_len, 4.0)
+        got = (O, lse, *ops.attn_packed_bwd(do, O, lse, rest, ks, vs, qs, spans, max_len, 4.0))
         for name, x in zip(('O', 'lse', 'dK', 'dV', 'dQ'), got):
             within(x, ref[name], name)
     kt = k.t().contiguous().t()
@@ -192,8 +192,8 @@ def test_row_pitches_and_alignment(ops, ext, dtype):
 
 def test_torch_operator_and_autograd(ops, ext):
     k, v, q, do, spans, max_len, sl = make([30, 0, 45], 24, 40, 19, torch.float32, seed=13)
-    O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 6.0)
-    want = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 6.0)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 6.0)
+    want = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 6.0)
     a = [x.clone().requires_grad_(True) for x in (k, v, q)]
     O2, lse2 = ext.packed_label_attention(*a, spans, max_len, 6.0)
     assert torch.equal(O, O2) and torch.equal(lse, lse2) and not lse2.requires_grad
@@ -218,20 +218,20 @@ def test_captured_and_replayed_with_new_inputs(ops):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
-        ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 30.0)
+        O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
+        ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 30.0)
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        O, lse = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
-        g = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len, 30.0)
+        O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 30.0)
+        g = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 30.0)
     for seed in (1, 2, 3):
         k2, v2, q2, do2 = make([40, 33], 100, 200, 65, torch.bfloat16, seed=seed)[:4]
         for x, y in zip((k, v, q, do), (k2, v2, q2, do2)):
             x.copy_(y)
         graph.replay()
-        O2, lse2 = ops.attn_packed_fwd(k2, v2, q2, spans, max_len, 30.0)
-        g2 = ops.attn_packed_bwd(do2, O2, lse2, k2, v2, q2, spans, max_len, 30.0)
+        O2, lse2, rest2 = ops.attn_packed_fwd(k2, v2, q2, spans, max_len, 30.0)
+        g2 = ops.attn_packed_bwd(do2, O2, lse2, rest2, k2, v2, q2, spans, max_len, 30.0)
         torch.cuda.synchronize()
         for x, y in zip((O, lse, *g), (O2, lse2, *g2)):
             assert torch.equal(x, y)
@@ -248,7 +248,7 @@ def test_on_another_stream_and_two_at_once(ops):
         with torch.cuda.stream(s):
             got.append(ops.attn_packed_fwd(*x[:3], x[4], x[5], 9.0))
     torch.cuda.synchronize()
-    for (O, lse), (O2, lse2) in zip(want, got):
+    for (O, lse, _), (O2, lse2, _) in zip(want, got):
         assert torch.equal(O, O2) and torch.equal(lse, lse2)
 
 
@@ -256,7 +256,7 @@ def test_empty_extents(ops, ext):
     k, v, q, do, spans, max_len, _ = make([0, 0], 8, 8, 4, torch.float32, seed=1)
     O, lse = ext.packed_label_attention(k, v, q, spans, max_len)
     assert O.shape == (2, 4, 8) and not O.any() and torch.isneginf(lse).all()
-    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, k, v, q, spans, max_len)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, None, k, v, q, spans, max_len)
     assert dk.shape == (0, 8) and dv.shape == (0, 8) and not dq.any()
     none = torch.zeros((0, 2), dtype=torch.int64, device=DEV)
     x = torch.ones(3, 8, device=DEV, requires_grad=True)
@@ -268,10 +268,37 @@ def test_empty_extents(ops, ext):
     assert O.shape == (1, 0, 8)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('cap', [0.0, 30.0, 31.0])
+def test_backward_from_lse_and_output_alone(ops, dtype, cap):
+    """Without the forward's statistics: the rounding of lse and of O enters (their bounds, in attn_ref)."""
+    k, v, q, do, spans, max_len, sl = make([70, 33], 100, 200, 90, dtype, seed=17)
+    O, lse, none = ops.attn_packed_fwd(k, v, q, spans, max_len, cap, need_grad=False)
+    assert none is None
+    got = ops.attn_packed_bwd(do, O, lse, None, k, v, q, spans, max_len, cap)
+    ref = attn_ref(k, v, q, sl, cap, do, rest=False)
+    for name, x in zip(('dK', 'dV', 'dQ'), got):
+        within(x, ref[name], name)
+
+
+def test_many_notes(ops):
+    """More notes than a wave has lanes: 200 of them, some empty, both types of cut."""
+    gen = torch.Generator().manual_seed(4)
+    lens = [int(x) for x in torch.randint(0, 40, (200,), generator=gen)]
+    lens[77] = 700
+    for L in (9, 150):
+        k, v, q, do, spans, max_len, sl = make(lens, 20, 24, L, torch.float32, seed=5)
+        O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 4.0)
+        got = (O, lse, *ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 4.0))
+        ref = attn_ref(k, v, q, sl, 4.0, do)
+        for name, x in zip(('O', 'lse', 'dK', 'dV', 'dQ'), got):
+            within(x, ref[name], name)
+
+
 def test_a_wrong_table_is_clamped_to_the_rows(ops):
     """Counts and starts outside of the rows give other numbers, never an access out of range (the kernels clamp them)."""
     k, v, q, do, _, _, _ = make([40], 16, 16, 5, torch.float32, seed=2)
     bad = torch.tensor([[-5, 20], [30, 1000], [10 ** 12, 4], [3, -7]], dtype=torch.int64, device=DEV)
-    O, lse = ops.attn_packed_fwd(k, v, q, bad, 64)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, bad, 64)
     ref = attn_ref(k, v, q, [(0, 20), (30, 10), (40, 0), (3, 0)])
     within(O, ref['O'], 'O')

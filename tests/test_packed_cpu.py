@@ -95,8 +95,8 @@ def test_attention_refuses(bad):
     for backward in (0, 1):
         assert lib.gzsl_packed_attn_work_bytes(d, backward) == -1
     p = ctypes.c_void_p(4096)  # never dereferenced: the arguments are refused first
-    assert lib.gzsl_packed_attn_fwd(d, p, p, p, 1 << 40, None) == hip.EINVAL
-    assert lib.gzsl_packed_attn_bwd(d, p, p, p, p, p, p, p, 1 << 40, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(d, p, p, p, p, 1 << 40, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_bwd(d, p, p, p, p, p, p, p, p, 1 << 40, None) == hip.EINVAL
 
 
 @lib_built
@@ -106,13 +106,14 @@ def test_attention_refuses_missing_pointers_and_short_workspaces():
     d = attn()
     need = lib.gzsl_packed_attn_work_bytes(d, 0)
     assert need > 0
-    assert lib.gzsl_packed_attn_fwd(d, p, p, p, need, None) == hip.EINVAL  # no tensors
+    assert lib.gzsl_packed_attn_fwd(d, p, p, p, p, need, None) == hip.EINVAL  # no tensors
     d = attn(keys=4096, values=4096, queries=4096, spans=4096)
-    assert lib.gzsl_packed_attn_fwd(d, p, p, p, need - 1, None) == hip.EINVAL
-    assert lib.gzsl_packed_attn_fwd(d, p, p, ctypes.c_void_p(4097), need, None) == hip.EINVAL
-    assert lib.gzsl_packed_attn_fwd(d, None, p, p, need, None) == hip.EINVAL
-    assert lib.gzsl_packed_attn_bwd(d, p, p, None, p, p, p, p, 1 << 40, None) == hip.EINVAL
-    assert lib.gzsl_packed_attn_fwd(None, p, p, p, need, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(d, p, p, p, p, need - 1, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(d, p, p, None, ctypes.c_void_p(4097), need, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(d, None, p, None, p, need, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(d, p, p, ctypes.c_void_p(4100), p, need, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_bwd(d, p, p, p, None, p, p, p, p, 1 << 40, None) == hip.EINVAL
+    assert lib.gzsl_packed_attn_fwd(None, p, p, p, p, need, None) == hip.EINVAL
     assert lib.gzsl_packed_attn_work_bytes(attn(B=70000), 0) == -1
 
 
