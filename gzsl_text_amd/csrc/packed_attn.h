@@ -11,8 +11,9 @@
 //   column fragment of the same image (k down the rows): bf16 by ds_read_b64_tr_b16 (k order 16 h + 4 g + j), fp32 by four
 //   ds_read_b32 (k = 4 g + j): exactly the order in which the accumulator registers of two (one) 16 x 16 score tiles hold
 //   their rows, so P and dS go from accumulator to operand without touching LDS.
-// Sums are fp32.  P and dS are rounded to the tensors' type for the second product (bf16: half a step of 2^-8 each, as the
-// inputs' own rounding; nothing for fp32); the softmax sum uses P before that rounding.
+// Sums are fp32.  P is rounded to the tensors' type for its products (bf16: half a step of 2^-8, as the inputs' own rounding;
+// nothing for fp32); the softmax sum uses P before that rounding.  dS sums to zero over a row, so its products cancel: as one
+// bf16 piece it made dK and dQ 1.6 times as far off as rounded results are, so it goes in two (16 bits, one more product).
 //
 // A pre-pass writes the operands as TILE IMAGES of 32 rows that are byte for byte the LDS layout (row pitch 64 s + 32 bytes:
 // conflict-free for both ways of reading), zero-filled past the note's end, past the last label and past E / F.  The sweeps
@@ -88,6 +89,11 @@ __device__ __forceinline__ void pa_pack(const float (&p)[1][4], f32x4& out) {
 __device__ __forceinline__ void pa_pack(const float (&p)[2][4], bf16x8& out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = (bf16)p[j >> 2][j & 3];
+}
+// what that rounding dropped
+__device__ __forceinline__ void pa_pack_low(const float (&p)[2][4], bf16x8& out) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = (bf16)(p[j >> 2][j & 3] - (float)(bf16)p[j >> 2][j & 3]);
 }
 
 struct PaCap {

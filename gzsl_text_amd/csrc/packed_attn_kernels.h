@@ -381,8 +381,18 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_kv_kernel(PaArgs a) {
         pa_pack(ds, sf);
 #pragma unroll
         for (int j = 0; j < G::NF; ++j) dv[j] = pa_mma(pa_col<T>(D, G::PF, 0, 16 * j, n, g), pf, dv[j]);
+        if constexpr (sizeof(T) == 2) {
+            frag sl;
+            pa_pack_low(ds, sl);
 #pragma unroll
-        for (int j = 0; j < G::NE; ++j) dk[j] = pa_mma(pa_col<T>(Q, G::PE, 0, 16 * j, n, g), sf, dk[j]);
+            for (int j = 0; j < G::NE; ++j) {
+                const frag f = pa_col<T>(Q, G::PE, 0, 16 * j, n, g);
+                dk[j] = pa_mma(f, sf, pa_mma(f, sl, dk[j]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < G::NE; ++j) dk[j] = pa_mma(pa_col<T>(Q, G::PE, 0, 16 * j, n, g), sf, dk[j]);
+        }
         pa_arrive();
     }
     if (tok >= len) return;
@@ -400,35 +410,41 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_kv_kernel(PaArgs a) {
 #pragma unroll
     for (int j = 0; j < G::NF; ++j) pa_out<T>(dv[j], (T*)a.dV + row * a.F, nullptr, 16 * j + 4 * g, a.F);
 }
-// dK / dV from the label shares, in order; zeros in the rows of no note (in front of the first note: blockIdx.y = B; behind a
-// note: that note's blocks).
+// dK / dV from the label shares, in order, and zeros in the rows of no note: 16 rows a workgroup, counted from a note's first
+// (blockIdx.y = B: the rows in front of the first note), a wave to a row.
+#define PA_JOIN_ROWS 16
 template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
-    const int b = blockIdx.y, W = a.E + a.F;
-    const long long step = (long long)gridDim.x * 256, first = (long long)blockIdx.x * 256 + threadIdx.x;
-    long long r0 = 0, r1;
+    const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = threadIdx.x >> 6, last = gridDim.x - 1;
+    long long start = 0, len = 0, end;  // rows [start + len, end) belong to no note
+    PaTileUnit un;
+    un.shares = 1;
     if (b == a.B) {
-        r1 = note_span(a.spans, 0, a.rows, a.max_len).start;
+        end = note_span(a.spans, 0, a.rows, a.max_len).start;
     } else {
-        const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
-        r0 = sp.start + sp.len;
-        r1 = b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows;
-        const PaTileUnit un = pa_tile_unit(a, 0, b);
-        if (un.shares > 1) {
-            const long long all = (long long)sp.len * W;
-            for (long long i = first; i < all; i += step) {
-                const int tok = (int)(i / W), c = (int)(i - (long long)tok * W);
-                const float* slab = a.dkv + ((long long)(un.tile + tok / PA_TILE) * un.shares * PA_TILE + tok % PA_TILE) * W + c;
+        un = pa_tile_unit(a, 0, b);
+        start = un.sp.start, len = un.sp.len;
+        end = b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows;
+    }
+    // (the last workgroup of a note takes all that is left behind it)
+    const long long stop = (int)blockIdx.x == last ? max(end - start, len) : (long long)(blockIdx.x + 1) * PA_JOIN_ROWS;
+    for (long long r = (long long)blockIdx.x * PA_JOIN_ROWS + w; r < stop; r += 4) {
+        const long long row = start + r;
+        if (r < len) {
+            if (un.shares == 1) continue;
+            const float* slab = a.dkv + ((un.tile + r / PA_TILE) * un.shares * PA_TILE + r % PA_TILE) * W;
+            for (int c = lane; c < W; c += 64) {
                 float s = 0.f;
-                for (int k = 0; k < un.shares; ++k) s += slab[(long long)k * PA_TILE * W];
-                const long long row = sp.start + tok;
+#pragma unroll 4
+                for (int k = 0; k < un.shares; ++k) s += slab[(long long)k * PA_TILE * W + c];
                 if (c < a.E) ((T*)a.dK)[row * a.E + c] = (T)s;
                 else ((T*)a.dV)[row * a.F + c - a.E] = (T)s;
             }
+        } else if (row < end) {
+            for (int c = lane; c < a.E; c += 64) ((T*)a.dK)[row * a.E + c] = (T)0.f;
+            for (int c = lane; c < a.F; c += 64) ((T*)a.dV)[row * a.F + c] = (T)0.f;
         }
     }
-    for (long long i = r0 * a.E + first; i < r1 * a.E; i += step) ((T*)a.dK)[i] = (T)0.f;
-    for (long long i = r0 * a.F + first; i < r1 * a.F; i += step) ((T*)a.dV)[i] = (T)0.f;
 }
 
 // dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.
@@ -495,8 +511,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
         }
         frag sf;
         pa_pack(ds, sf);
+        if constexpr (sizeof(T) == 2) {
+            frag sl;
+            pa_pack_low(ds, sl);
 #pragma unroll
-        for (int j = 0; j < G::NE; ++j) dq[j] = pa_mma(pa_col<T>(K, G::PE, 0, 16 * j, n, g), sf, dq[j]);
+            for (int j = 0; j < G::NE; ++j) {
+                const frag f = pa_col<T>(K, G::PE, 0, 16 * j, n, g);
+                dq[j] = pa_mma(f, sf, pa_mma(f, sl, dq[j]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < G::NE; ++j) dq[j] = pa_mma(pa_col<T>(K, G::PE, 0, 16 * j, n, g), sf, dq[j]);
+        }
         pa_arrive();
     }
     const int l = l0 + n;
@@ -535,7 +561,7 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     hipLaunchKernelGGL((pa_pack_kernel<T, G>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_pack_do_kernel<T, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
     if (p.units > 0) hipLaunchKernelGGL((pa_bwd_kv_kernel<T, G, CAP, DROP>), dim3((unsigned)p.units), dim3(256), 2 * (G::QB + G::OB), st, a);
-    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(32, a.B + 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, PA_JOIN_ROWS) : 1, a.B + 1), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_bwd_q_kernel<T, G, W, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::KV, st, a);
     const long long n = (long long)a.L * a.E;
     hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS>), dim3((unsigned)(n < 256 * 4096 ? cdiv((long)n, 256) : 4096)), dim3(256), 0, st, a);
