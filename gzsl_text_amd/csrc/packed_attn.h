@@ -97,25 +97,65 @@ __device__ __forceinline__ void pa_pack_low(const float (&p)[2][4], bf16x8& out)
 }
 
 struct PaCap {
-    float cap, k1, c2;  // cap, 2 log2(e) / cap, cap log2(e)
+    float inv, k1, c2;  // 1 / cap, 2 log2(e) / cap, cap log2(e)
 };
 __device__ __forceinline__ PaCap pa_cap(float cap) {
-    return {cap, cap > 0.f ? 2.f * PA_LOG2E / cap : 0.f, cap * PA_LOG2E};
+    return {cap > 0.f ? 1.f / cap : 0.f, cap > 0.f ? 2.f * PA_LOG2E / cap : 0.f, cap * PA_LOG2E};
 }
-// Score in units of log 2, and th = tanh(x / cap).  tanh u = 1 - 2 / (1 + e^{2u}): exact limits at +-inf, absolute error of a
-// few 2^-24.  fp32 tensors take the odd series below |u| = 0.35 (the next term is below 2^-26 of the value there), where the
-// difference would lose relative accuracy that the products of the gradient still have.
-template <typename T>
-__device__ __forceinline__ float pa_score2(float x, const PaCap& c, float& th) {
-    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1));
-    if (sizeof(T) == 2) {
-        th = fmaf(-2.f, r, 1.f);
+// tanh u = 1 - 2 / (1 + e^{2u}): exact limits at +-inf, absolute error of a few 2^-24.  fp32 tensors take the odd series below
+// |u| = 0.35 (the next term is below 2^-26 of the value there), where the difference would lose relative accuracy that the
+// products of the gradient still have.  `far` (the same in the whole wave): some lane needs the exponential.
+__device__ __forceinline__ float pa_sech(float x, const PaCap& c) {  // 1 / (1 + e^{2 x / cap})
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1));
+}
+__device__ __forceinline__ float pa_series(float u) {
+    const float w = u * u;
+    return u * fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+}
+#define PA_NEAR 0.35f
+// Scores x of a tile -> y in units of log 2 (and th = tanh(x / cap) for the gradient).
+template <typename T, bool CAP, int U, bool TH>
+__device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, float (&y)[U][4], float (&th)[U][4]) {
+    if (!CAP) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[u][r] = x[u][r] * PA_LOG2E;
+    } else if (sizeof(T) == 2) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float q = pa_sech(x[u][r], c);
+                y[u][r] = fmaf(q, -2.f * c.c2, c.c2);
+                if (TH) th[u][r] = fmaf(q, -2.f, 1.f);
+            }
     } else {
-        const float u = x * (c.k1 * (0.5f * PA_LN2)), w = u * u;
-        const float s = u * fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-        th = fabsf(u) < 0.35f ? s : fmaf(-2.f, r, 1.f);
+        bool near = true;
+        float t[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float v = x[u][r] * c.inv;
+                near = near && fabsf(v) < PA_NEAR;  // (false for a NaN)
+                t[u][r] = pa_series(v);
+            }
+        if (!__all(near)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!(fabsf(x[u][r] * c.inv) < PA_NEAR)) t[u][r] = fmaf(pa_sech(x[u][r], c), -2.f, 1.f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                y[u][r] = t[u][r] * c.c2;
+                if (TH) th[u][r] = t[u][r];
+            }
     }
-    return th * c.c2;
 }
 
 // Copies `bytes` (whole KB) of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  The

@@ -1,6 +1,7 @@
 // Kernels of the packed label attention, instantiated for fp32 in packed_attn_f32.hip and for bf16 in packed_attn_bf16.hip; the
 // mathematics, the fragments, the tile images and the cut of the work are in packed_attn.h.
 #pragma once
+#include <type_traits>
 #include "packed_attn.h"
 
 // ------------------------------------------------------------------------------------------------------------- pre-pass
@@ -114,7 +115,7 @@ __device__ __forceinline__ void pa_out(const f32x4& v, T* row, bf16* low, int c,
 // -------------------------------------------------------------------------------------------------------------- forward
 // Workgroup = WAVES x 16 labels of one note (or of one chunk of it); labels on the lane axis.
 template <typename T, class G, int WAVES, bool CAP, bool DROP>
-__global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_kernel(PaArgs a) {
+__global__ __launch_bounds__(WAVES * 64, (sizeof(T) == 2 && G::NE == 7) ? 4 : (sizeof(T) == 2 ? 3 : 2)) void pa_fwd_kernel(PaArgs a) {
     typedef typename PaTy<T>::frag frag;
     constexpr int U = G::U;
     extern __shared__ __attribute__((aligned(16))) char sm[];
@@ -145,27 +146,21 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_kernel(PaArgs a) {
     const char* kv = a.KV + (long long)b * a.nT * G::KV;
     if (t0 < t1) pa_dma<WAVES>(kv + (long long)t0 * G::KV, sm, G::KV, wave, lane);
     pa_arrive();
-    for (int t = t0; t < t1; ++t) {
+    auto step = [&](int t, auto last) {  // last: the tile may end behind the note
         const char* K = sm + ((t - t0) & 1) * G::KV;
         const char* V = K + G::EB;
         if (t + 1 < t1) pa_dma<WAVES>(kv + (long long)(t + 1) * G::KV, sm + ((t - t0 + 1) & 1) * G::KV, G::KV, wave, lane);
-        float y[U][4];
+        f32x4 s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            f32x4 s0 = f32x4{0.f, 0.f, 0.f, 0.f}, s1 = s0;  // two chains: an accumulator takes its next product 8 cycles late
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < G::SE; ++k) {
-                f32x4& s = k & 1 ? s1 : s0;
-                s = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float th;
-                y[u][r] = CAP ? pa_score2<T>(s0[r] + s1[r], cap, th) : (s0[r] + s1[r]) * PA_LOG2E;
-            }
+            for (int k = 0; k < G::SE; ++k) s[u] = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s[u]);
         }
-        const int left = len - t * G::ROWS;  // tokens of this tile
-        if (left < G::ROWS) {
+        float y[U][4], th[U][4];
+        pa_scores<T, CAP, U, false>(s, cap, y, th);
+        if constexpr (decltype(last)::value) {
+            const int left = len - t * G::ROWS;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -209,7 +204,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_kernel(PaArgs a) {
 #pragma unroll
         for (int j = 0; j < G::NF; ++j) acc[j] = pa_mma(pa_col<T>(V, G::PF, 0, 16 * j, n, g), pf, acc[j]);
         pa_arrive();
-    }
+    };
+    for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
+    if (t0 < t1) step(t1 - 1, std::true_type{});
     const int l = l0 + n;
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -304,11 +301,9 @@ __global__ __launch_bounds__(256) void pa_join_kernel(PaArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- backward
-// P and dS of one score: weights w = exp2(y - off) * scale, dropout factor keep.
-template <typename T, bool CAP>
-__device__ __forceinline__ void pa_grad(float s, float dp, float off, float scale, float delta, float keep, const PaCap& c, float& p, float& ds) {
-    float th = 0.f;
-    const float y = CAP ? pa_score2<T>(s, c, th) : s * PA_LOG2E;
+// P and dS of a tile: weights w = exp2(y - off) * scale, dropout factor keep.
+template <bool CAP>
+__device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, float scale, float delta, float keep, float& p, float& ds) {
     const float w = __builtin_amdgcn_exp2f(y - off) * scale;
     p = w * keep;
     ds = w * fmaf(dp, keep, -delta);
@@ -354,15 +349,20 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_kv_kernel(PaArgs a) {
         const char* D = Q + G::QB;
         const float* aux = reinterpret_cast<const float*>(D + G::FB);
         if (q + 1 < q1) fetch(q + 1, sm + ((q - q0 + 1) & 1) * BUF);
-        float p[U][4], ds[U][4];
+        float p[U][4], ds[U][4], y[U][4], th[U][4];
+        f32x4 s[U], dp[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f}, dp = s;
+            s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < G::SF; ++k) {
-                if (k < G::SE) s = pa_mma(pa_row<T>(Q, G::PE, 16 * u, k, n, g), kf[k], s);
-                dp = pa_mma(pa_row<T>(D, G::PF, 16 * u, k, n, g), vf[k], dp);
+                if (k < G::SE) s[u] = pa_mma(pa_row<T>(Q, G::PE, 16 * u, k, n, g), kf[k], s[u]);
+                dp[u] = pa_mma(pa_row<T>(D, G::PF, 16 * u, k, n, g), vf[k], dp[u]);
             }
+        }
+        pa_scores<T, CAP, U, true>(s, cap, y, th);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
             const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
                         delta = *reinterpret_cast<const f32x4*>(aux + 2 * G::ROWS + 16 * u + 4 * g);
 #pragma unroll
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256, 2) void pa_bwd_kv_kernel(PaArgs a) {
                     const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
                     keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
                 }
-                pa_grad<T, CAP>(s[r], dp[r], off[r], scale[r], delta[r], keep, cap, p[u][r], ds[u][r]);
+                pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
             }
         }
         frag pf, sf;
@@ -433,6 +433,16 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
         if (r < len) {
             if (un.shares == 1) continue;
             const float* slab = a.dkv + ((un.tile + r / PA_TILE) * un.shares * PA_TILE + r % PA_TILE) * W;
+            if (((a.E | a.F) & 3) == 0) {
+                for (int c = 4 * lane; c < W; c += 256) {
+                    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                    for (int k = 0; k < un.shares; ++k) s += *reinterpret_cast<const f32x4*>(slab + (long long)k * PA_TILE * W + c);
+                    if (c < a.E) pa_out<T>(s, (T*)a.dK + row * a.E, nullptr, c, a.E);
+                    else pa_out<T>(s, (T*)a.dV + row * a.F, nullptr, c - a.E, a.F);
+                }
+                continue;
+            }
             for (int c = lane; c < W; c += 64) {
                 float s = 0.f;
 #pragma unroll 4
@@ -481,28 +491,32 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     const char* kv = a.KV + (long long)b * a.nT * G::KV;
     if (t0 < t1) pa_dma<WAVES>(kv + (long long)t0 * G::KV, sm, G::KV, wave, lane);
     pa_arrive();
-    for (int t = t0; t < t1; ++t) {
+    auto step = [&](int t, auto last) {  // last: the tile may end behind the note
         const char* K = sm + ((t - t0) & 1) * G::KV;
         const char* V = K + G::EB;
         if (t + 1 < t1) pa_dma<WAVES>(kv + (long long)(t + 1) * G::KV, sm + ((t - t0 + 1) & 1) * G::KV, G::KV, wave, lane);
-        float ds[U][4];
+        float ds[U][4], y[U][4], th[U][4];
+        f32x4 s[U], dp[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f}, dp = s;
+            s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < G::SF; ++k) {
-                if (k < G::SE) s = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s);
-                dp = pa_mma(pa_row<T>(V, G::PF, 16 * u, k, n, g), df[k], dp);
+                if (k < G::SE) s[u] = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s[u]);
+                dp[u] = pa_mma(pa_row<T>(V, G::PF, 16 * u, k, n, g), df[k], dp[u]);
             }
+        }
+        pa_scores<T, CAP, U, true>(s, cap, y, th);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float keep = 1.f, p;
                 if (DROP) keep = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? a.scale : 0.f;
-                pa_grad<T, CAP>(s[r], dp[r], off, scale, delta, keep, cap, p, ds[u][r]);
+                pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
             }
-        }
-        const int left = len - t * G::ROWS;
-        if (left < G::ROWS) {  // (a key of zeros has the score 0, which may be far above the note's own)
+        if constexpr (decltype(last)::value) {  // (a key of zeros has the score 0, which may be far above the note's own)
+            const int left = len - t * G::ROWS;
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -524,7 +538,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
             for (int j = 0; j < G::NE; ++j) dq[j] = pa_mma(pa_col<T>(K, G::PE, 0, 16 * j, n, g), sf, dq[j]);
         }
         pa_arrive();
-    }
+    };
+    for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
+    if (t0 < t1) step(t1 - 1, std::true_type{});
     const int l = l0 + n;
     if (l >= a.L) return;
     float* out = a.dq + ((long long)un.ci * a.L + l) * a.E;
