@@ -5,20 +5,27 @@
 //     backward, with delta = <dO, O>:  dV_t += drop(P) dO_l;   dS = P (drop(<dO_l, v_t>) - delta) (1 - (y / cap)^2);
 //                                      dK_t = sum_l dS q_l;    dQ_l = sum_{b,t} dS k_t
 //
-// One set of kernels serves both types.  A "fragment" is 16 bytes per lane: eight bf16 (one v_mfma_f32_16x16x32_bf16) or
-// four fp32 (four v_mfma_f32_16x16x4_f32, exact), so a k step of 64 bytes and every LDS offset are the same for both.
-//   row fragment of an image [row][k]:   lane (n = lane & 15, g = lane >> 4) holds row n, bytes 64 s + 16 g .. + 15
-//   column fragment of the same image (k down the rows): bf16 by ds_read_b64_tr_b16 (k order 16 h + 4 g + j), fp32 by four
-//   ds_read_b32 (k = 4 g + j): exactly the order in which the accumulator registers of two (one) 16 x 16 score tiles hold
-//   their rows, so P and dS go from accumulator to operand without touching LDS.
-// Sums are fp32.  P is rounded to the tensors' type for its products (bf16: half a step of 2^-8, as the inputs' own rounding;
-// nothing for fp32); the softmax sum uses P before that rounding.  dS sums to zero over a row, so its products cancel: as one
-// bf16 piece it made dK and dQ 1.6 times as far off as rounded results are, so it goes in two (16 bits, one more product).
+// One set of kernels, three kinds of product:
+//   PaBF   bf16 tensors: v_mfma_f32_16x16x32_bf16.
+//   PaX3   fp32 tensors, E <= 112: every operand is split exactly into three bf16 pieces (8 significant bits each) and a product is
+//          the six cross terms of weight >= 2^-16 of them (what is dropped is below 2^-24 of the product), each the same MFMA:
+//          6 x 16 cycles per 32 k against 8 x 32 of the fp32 MFMA.
+//   PaF32  fp32 tensors, E > 112 (three pieces of both tiles no longer fit LDS twice): v_mfma_f32_16x16x4_f32, exact.
+// Sums are fp32 in all of them.  P is rounded to bf16 for bf16 tensors' products (half a step of 2^-8, as the inputs' own
+// rounding); the softmax sum uses P before that.  dS sums to zero over a row, so its products cancel: as one bf16 piece it made
+// dK and dQ 1.6 times as far off as rounded results are, so it goes in two (16 bits, one more product).
 //
-// A pre-pass writes the operands as TILE IMAGES of 32 rows that are byte for byte the LDS layout (row pitch 64 s + 32 bytes:
-// conflict-free for both ways of reading), zero-filled past the note's end, past the last label and past E / F.  The sweeps
-// then copy whole tiles by LDS-DMA, and odd widths, row pitches, alignment and whatever lies between the notes
-// (NaN included) end in the pre-pass.
+// Everything is moved as FRAGMENTS: 1 KB, 16 bytes a lane, exactly one operand of one matrix instruction (eight bf16 of a lane;
+// four fp32, which feed four instructions).  With n = lane & 15, g = lane >> 4:
+//   row fragment (u, s) of a tile [row][k]:  row 16 u + n, 16 bytes of k from 64 s + 16 g (bytes)
+//   column fragment (j) of the same tile:    column 16 j + n, its rows 4 g + i (bf16: and 16 + 4 g + i): exactly the order in which
+//                                            the accumulator registers of the tile's 16 x 16 score tiles hold their rows, so P and
+//                                            dS go from accumulator to operand without touching LDS.
+// A pre-pass writes the operands as tile images made of such fragments (a tile: the rows of one k step of the second product, 32,
+// or 16 of PaF32), zero-filled past the note's end, past the last label and past E / F.  The sweeps copy images by LDS-DMA and read
+// them 16 bytes a lane at one address plus constants, free of bank conflicts without padding; odd widths, row pitches, alignment
+// and whatever lies between the notes (NaN included) end in the pre-pass.  PaX3's backward, for lack of LDS, takes its column
+// fragments out of the row fragments with ds_read_b64_tr_b16.
 #pragma once
 #include "packed.h"
 #include "rng.h"
@@ -26,31 +33,41 @@
 
 #define PA_LOG2E 1.4426950408889634f
 #define PA_LN2 0.6931471805599453f
-#define PA_TILE 64  // tokens of a workgroup in the dK / dV sweep
+#define PA_TILE 128  // tokens of a workgroup in the dK / dV sweep
 
-template <typename T>
-struct PaTy;
-template <>
-struct PaTy<float> {
+struct PaF32 {
+    typedef float T;
+    typedef float M;  // element of a fragment
     typedef f32x4 frag;
+    static constexpr int PL = 1;
 };
-template <>
-struct PaTy<bf16> {
+struct PaBF {
+    typedef bf16 T;
+    typedef bf16 M;
     typedef bf16x8 frag;
+    static constexpr int PL = 1;
+};
+struct PaPieces {
+    bf16x8 p[3];
+};
+struct PaX3 {
+    typedef float T;
+    typedef bf16 M;
+    typedef PaPieces frag;
+    static constexpr int PL = 3;
 };
 
-// NE / NF: 16-wide tiles of the key / value width (E <= 16 NE, F <= 16 NF).  A tile image holds one k step of the second
-// product: 32 rows of bf16, 16 of fp32.
-template <typename T, int NE_, int NF_>
+// NE / NF: 16-wide tiles of the key / value width (E <= 16 NE, F <= 16 NF).  Sizes in KB = fragments.
+template <class K, int NE_, int NF_>
 struct PaGeo {
-    static constexpr int NE = NE_, NF = NF_, SZ = sizeof(T), KF = 16 / SZ, ROWS = 4 * KF, U = ROWS / 16;
-    static constexpr int SE = (NE * 16 * SZ + 63) / 64, SF = (NF * 16 * SZ + 63) / 64;  // 64-byte k steps over e / f
-    static constexpr int PE = 64 * SE + 32, PF = 64 * SF + 32;                          // row pitches in bytes
-    static constexpr int EB = ROWS * PE, FB = ROWS * PF;
-    static constexpr int KV = EB + FB;                                  // token tile: keys, values
-    static constexpr int QB = (EB + 1023) / 1024 * 1024;                // label tile: queries
-    static constexpr int OB = (FB + 12 * ROWS + 1023) / 1024 * 1024;    // label tile: dO rows, then off[], scale[], delta[] of its labels
-    static_assert(KV % 1024 == 0, "whole KB: the copies move 1 KB per wave instruction");
+    static constexpr int NE = NE_, NF = NF_, PL = K::PL, SZ = sizeof(typename K::M), KF = 16 / SZ, KK = 4 * KF, ROWS = KK, U = ROWS / 16;
+    static constexpr int SE = (NE * 16 + KK - 1) / KK, SF = (NF * 16 + KK - 1) / KK;  // k steps over e / f
+    static constexpr int RE = U * SE, RF = U * SF;                                    // row fragments of a tile (one plane)
+    static constexpr bool TR = PL == 3;                                               // backward: columns by transposed reads
+    static constexpr int FWD = PL * (RE + NF);                                        // token tile, forward: keys by rows, values by columns
+    static constexpr int TOK = PL * (RE + RF) + (TR ? 0 : NE);                        // token tile, backward: keys, values by rows, keys by columns
+    static constexpr int QRY = PL * RE + (TR ? 0 : NE);                               // label tile: queries by rows (and columns)
+    static constexpr int OUT = PL * RF + (TR ? 0 : NF) + 1;                           // label tile: dO by rows (and columns), then off, scale, delta
 };
 
 __device__ __forceinline__ f32x4 pa_mma(f32x4 a, f32x4 b, f32x4 c) {
@@ -58,42 +75,85 @@ __device__ __forceinline__ f32x4 pa_mma(f32x4 a, f32x4 b, f32x4 c) {
     for (int j = 0; j < 4; ++j) c = mfma16(a[j], b[j], c);
     return c;
 }
-__device__ __forceinline__ f32x4 pa_mma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x4 pa_mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 pa_mma(const PaPieces& a, const PaPieces& b, f32x4 c) {  // smallest terms first
+    c = pa_mma(a.p[2], b.p[0], c);
+    c = pa_mma(a.p[0], b.p[2], c);
+    c = pa_mma(a.p[1], b.p[1], c);
+    c = pa_mma(a.p[1], b.p[0], c);
+    c = pa_mma(a.p[0], b.p[1], c);
+    return pa_mma(a.p[0], b.p[0], c);
 }
 
-template <typename T>
-__device__ __forceinline__ typename PaTy<T>::frag pa_row(const char* img, int pitch, int row0, int s, int n, int g) {
-    return *reinterpret_cast<const typename PaTy<T>::frag*>(img + (row0 + n) * pitch + 64 * s + 16 * g);
-}
-template <typename T>
-__device__ __forceinline__ typename PaTy<T>::frag pa_col(const char* img, int pitch, int row0, int col0, int n, int g);
-template <>
-__device__ __forceinline__ f32x4 pa_col<float>(const char* img, int pitch, int row0, int col0, int n, int g) {
-    f32x4 v;
+// Fragment i of `count` (a plane) at `img`; planes follow one another.
+template <class K, int COUNT>
+__device__ __forceinline__ typename K::frag pa_frag(const char* img, int i, int lane) {
+    if constexpr (K::PL == 1) {
+        return *reinterpret_cast<const typename K::frag*>(img + i * 1024 + lane * 16);
+    } else {
+        PaPieces f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(img + (row0 + 4 * g + j) * pitch + 4 * (col0 + n));
-    return v;
+        for (int p = 0; p < 3; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(img + (p * COUNT + i) * 1024 + lane * 16);
+        return f;
+    }
 }
-template <>
-__device__ __forceinline__ bf16x8 pa_col<bf16>(const char* img, int pitch, int row0, int col0, int n, int g) {
-    const char* p = img + (row0 + 4 * g + (n >> 2)) * pitch + 2 * col0 + 8 * (n & 3);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(p + 16 * pitch));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+// Column fragment j out of the row fragments (SK k steps, U = 2) of a tile.  Row r, columns 16 j + 4 q .. + 3 lie in k step j / 2, lane
+// (16 (2 (j & 1) + q / 2) + r), bytes 8 (q & 1); the transposed read gives lane n of a 16-lane group column n of its 4 x 16 block.
+template <int SK>
+__device__ __forceinline__ PaPieces pa_col_tr(const char* img, int j, int n, int g) {
+    const int r = 4 * g + (n >> 2), q = n & 3;
+    const char* at = img + (j >> 1) * 1024 + ((2 * (j & 1) + (q >> 1)) * 16 + r) * 16 + 8 * (q & 1);
+    PaPieces f;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(at + p * 2 * SK * 1024));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(at + (p * 2 + 1) * SK * 1024));
+        f.p[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return f;
 }
-// accumulator registers of the tile's 16-row score tiles -> operand fragment
-__device__ __forceinline__ void pa_pack(const float (&p)[1][4], f32x4& out) {
-    out = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]};
-}
+// accumulator registers of the tile's score tiles -> operand fragment
+__device__ __forceinline__ void pa_pack(const float (&p)[1][4], f32x4& out) { out = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]}; }
 __device__ __forceinline__ void pa_pack(const float (&p)[2][4], bf16x8& out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = (bf16)p[j >> 2][j & 3];
 }
-// what that rounding dropped
+__device__ __forceinline__ void pa_split(float x, bf16& h, bf16& m, bf16& l) {  // x = h + m + l
+    h = (bf16)x;
+    const float r = x - (float)h;
+    m = (bf16)r;
+    l = (bf16)(r - (float)m);
+}
+__device__ __forceinline__ void pa_pack(const float (&p)[2][4], PaPieces& out) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        bf16 h, m, l;
+        pa_split(p[j >> 2][j & 3], h, m, l);
+        out.p[0][j] = h, out.p[1][j] = m, out.p[2][j] = l;
+    }
+}
+// what rounding to bf16 dropped
 __device__ __forceinline__ void pa_pack_low(const float (&p)[2][4], bf16x8& out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = (bf16)(p[j >> 2][j & 3] - (float)(bf16)p[j >> 2][j & 3]);
+}
+
+// N fragments through a ring of D: a fragment's read is issued D products ahead of its use and kept there (left alone, the
+// compiler reads each one right before its product and waits for it).  ld(i) reads, use(i, f) multiplies.
+template <int N, int D, class F, class LD, class USE>
+__device__ __forceinline__ void pa_run_ring(F (&ring)[D], LD&& ld, USE&& use) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        use(i, ring[i % D]);
+        if (i + D < N) ring[i % D] = ld(i + D);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+template <int N, int D, class F, class LD>
+__device__ __forceinline__ void pa_fill_ring(F (&ring)[D], LD&& ld) {
+#pragma unroll
+    for (int i = 0; i < D && i < N; ++i) ring[i] = ld(i);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 struct PaCap {
@@ -114,14 +174,14 @@ __device__ __forceinline__ float pa_series(float u) {
 }
 #define PA_NEAR 0.35f
 // Scores x of a tile -> y in units of log 2 (and th = tanh(x / cap) for the gradient).
-template <typename T, bool CAP, int U, bool TH>
+template <class K, bool CAP, int U, bool TH>
 __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, float (&y)[U][4], float (&th)[U][4]) {
     if (!CAP) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[u][r] = x[u][r] * PA_LOG2E;
-    } else if (sizeof(T) == 2) {
+    } else if (sizeof(typename K::T) == 2) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -158,12 +218,16 @@ __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, f
     }
 }
 
-// Copies `bytes` (whole KB) of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  The
-// caller waits with pa_arrive() before anyone reads.
-template <int WAVES>
-__device__ __forceinline__ void pa_dma(const char* src, char* dst, int bytes, int wave, int lane) {
-    for (int o = wave * 1024; o < bytes; o += WAVES * 1024)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + 16 * lane), (GZ_LDS void*)(dst + o), 16, 0, 0);
+// Copies KB KB of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  The caller waits with
+// pa_arrive() before anyone reads.
+template <int WAVES, int KB>
+__device__ __forceinline__ void pa_dma(const char* src, char* dst, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < (KB + WAVES - 1) / WAVES; ++i) {
+        const int o = (wave + i * WAVES) * 1024;
+        if (KB % WAVES == 0 || i < KB / WAVES || o < KB * 1024)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + 16 * lane), (GZ_LDS void*)(dst + o), 16, 0, 0);
+    }
 }
 // this wave's copies have landed and every wave is past its reads of the other buffer
 __device__ __forceinline__ void pa_arrive() {
@@ -182,7 +246,7 @@ struct PaArgs {
     int nLT, extra;                   // label workgroups of a note; token chunks beyond one a note (0: notes are not cut)
     int shares, slots;                // dK / dV: label shares of a token tile at most, slabs that the workspace has room for
     // workspace
-    char *KV, *Q, *DO;
+    char *TK, *Q, *DO;  // images: token tiles [B][nT], queries [nQ], dO [B][nQ]
     float *part, *ml;  // forward, notes cut: unnormalised O [chunk][L][F] and (max, sum) [chunk][L][2]
     float *dq, *dkv;   // backward: [chunk][L][E]; [unit][PA_TILE][E + F]
     // results and the backward's inputs
@@ -257,8 +321,8 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
     if (u.b >= 0) u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
     return u;
 }
-// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  The parts are as many as fill the chip's 512 places
-// (two workgroups a compute unit) best, a slab written and read again counted as 1 % a part.
+// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  The parts are as many as fill the chip's 256 compute
+// units best, a slab written and read again counted as 2 % a part.
 struct PaTileUnit {
     int b, tile, share, shares, unit, tiles;
     NoteSpan sp;
@@ -276,8 +340,8 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
     u.shares = 1;
     float best = -1.f;
     for (int s = 1; s <= a.shares && (s == 1 || (long long)n * s <= a.slots); ++s) {
-        const int all = n * s, rounds = (all + 511) / 512;
-        const float fill = rounds > 0 ? (float)all / (512.f * rounds) - 0.01f * s : 0.f;
+        const int all = n * s, rounds = (all + 255) / 256;
+        const float fill = rounds > 0 ? (float)all / (256.f * rounds) - 0.02f * s : 0.f;
         if (fill > best) best = fill, u.shares = s;
     }
     u.unit = unit;
@@ -305,10 +369,11 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
 }
 
 struct PaPlan {
-    int nT, nQ, wide, waves, extra, shares, slots, nLT;
+    int nT, nQ, kind, waves, extra, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
     long long units;  // workgroups of the dK / dV sweep
     long long kv, q, dO, part, ml, dq, dkv, bytes;
 };
-// packed_attn_f32.hip / packed_attn_bf16.hip
-int pa_run_f32(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);
+// packed_attn_bf16.hip, packed_attn_x3.hip, packed_attn_f32.hip
 int pa_run_bf16(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);
+int pa_run_x3(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);
+int pa_run_f32(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st);

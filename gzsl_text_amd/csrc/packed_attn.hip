@@ -6,9 +6,9 @@ static inline long long up256(long long n) { return (n + 255) / 256 * 256; }
 template <class G>
 static void pa_sizes(PaPlan& p, const GzslPackedAttn& d, int backward) {
     p.nT = (int)(((long long)d.max_len + G::ROWS - 1) / G::ROWS), p.nQ = (int)(((long long)d.L + G::ROWS - 1) / G::ROWS);
-    p.kv = up256((long long)d.B * p.nT * G::KV);
-    p.q = up256((long long)p.nQ * G::QB);
-    p.dO = backward ? up256((long long)d.B * p.nQ * G::OB) : 0;
+    p.kv = 1024LL * d.B * p.nT * (backward ? G::TOK : G::FWD);
+    p.q = 1024LL * p.nQ * (backward ? G::QRY : G::PL * G::RE);
+    p.dO = backward ? 1024LL * d.B * p.nQ * G::OUT : 0;
 }
 static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     if (!d || d->B < 0 || d->rows < 0 || d->max_len < 0 || d->L < 0 || d->E < 1 || d->F < 1 || d->E > 208 || d->F > 208) return GZSL_EINVAL;
@@ -17,15 +17,16 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     if (d->ldk < d->E || d->ldv < d->F || d->ldq < d->E) return GZSL_EINVAL;
     if (d->B > 65534 || d->max_len > 0x7FFF0000 || d->L > 0x7FFF0000) return GZSL_ETOOBIG;
     p = PaPlan{};
-    p.wide = d->E > 112;
-    if (d->dtype == GZSL_F32) p.wide ? pa_sizes<PaGeo<float, 13, 13>>(p, *d, backward) : pa_sizes<PaGeo<float, 7, 13>>(p, *d, backward);
-    else p.wide ? pa_sizes<PaGeo<bf16, 13, 13>>(p, *d, backward) : pa_sizes<PaGeo<bf16, 7, 13>>(p, *d, backward);
-    // bf16 forward: 128 labels a workgroup read each token tile half as often as 64; taken where that leaves two rounds of work
-    p.waves = d->dtype == GZSL_BF16 && !backward && (long long)d->B * cdiv(d->L, 128) >= 512 ? 8 : 4;
+    p.kind = (d->dtype == GZSL_F32 ? 2 : 0) + (d->E > 112);
+    if (p.kind == 0) pa_sizes<PaGeo<PaBF, 7, 13>>(p, *d, backward);
+    else if (p.kind == 1) pa_sizes<PaGeo<PaBF, 13, 13>>(p, *d, backward);
+    else if (p.kind == 2) pa_sizes<PaGeo<PaX3, 7, 13>>(p, *d, backward);
+    else pa_sizes<PaGeo<PaF32, 13, 13>>(p, *d, backward);
+    p.waves = p.kind == 3 && !backward ? 4 : 8;
     p.nLT = cdiv(d->L, 16 * p.waves);
-    // notes are cut where (note, label) workgroups alone do not fill the chip's 512 places
-    const long long wgs = (long long)d->B * p.nLT;
-    p.extra = wgs > 0 && wgs < 512 && d->max_len > 256 ? cdiv(512, p.nLT) : 0;
+    // notes are cut where (note, label) workgroups alone do not fill the chip's places (one or two workgroups a compute unit)
+    const long long wgs = (long long)d->B * p.nLT, places = p.kind == 2 ? 256 : 512;
+    p.extra = wgs > 0 && wgs < places && d->max_len > 256 ? cdiv(places, p.nLT) : 0;
     if (p.extra > d->B * (d->max_len / 256 + 1)) p.extra = d->B * (d->max_len / 256 + 1);
     const long long chunks = d->B + p.extra;
     if ((long long)d->B * p.nT + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
@@ -55,7 +56,7 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
     a.nLT = p.nLT, a.extra = p.extra, a.shares = p.shares, a.slots = p.slots;
     char* w = (char*)work;
-    a.KV = w, w += p.kv;
+    a.TK = w, w += p.kv;
     a.Q = w, w += p.q;
     a.DO = w, w += p.dO;
     a.part = (float*)w, w += p.part;
@@ -64,7 +65,8 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.dkv = (float*)w;
 }
 static int pa_run(const GzslPackedAttn& d, PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) {
-    return d.dtype == GZSL_F32 ? pa_run_f32(a, p, backward, st) : pa_run_bf16(a, p, backward, st);
+    if (p.kind == 3) return pa_run_f32(a, p, backward, st);
+    return p.kind == 2 ? pa_run_x3(a, p, backward, st) : pa_run_bf16(a, p, backward, st);
 }
 
 extern "C" long long gzsl_packed_attn_work_bytes(const GzslPackedAttn* d, int backward) {

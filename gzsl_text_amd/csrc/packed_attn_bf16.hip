@@ -1,6 +1,9 @@
-// bf16 instantiation of the packed label attention.
+// bf16 tensors.
 #include "packed_attn_kernels.h"
 
 int pa_run_bf16(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) {
-    return p.waves == 8 && !backward ? pa_go<bf16, 8>(a, p, false, st) : pa_go<bf16, 4>(a, p, backward, st);
+    typedef PaGeo<PaBF, 7, 13> A;
+    typedef PaGeo<PaBF, 13, 13> B;
+    if (backward) return p.kind ? pa_go_bwd<PaBF, B, 8>(a, p, st) : pa_go_bwd<PaBF, A, 8>(a, p, st);
+    return p.kind ? pa_go_fwd<PaBF, B, 8, 4>(a, st) : pa_go_fwd<PaBF, A, 8, 4>(a, st);
 }

@@ -1,4 +1,7 @@
-// fp32 instantiation of the packed label attention.
+// fp32 tensors of a key width above 112: exact fp32 matrix instructions.
 #include "packed_attn_kernels.h"
 
-int pa_run_f32(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) { return pa_go<float, 4>(a, p, backward, st); }
+int pa_run_f32(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) {
+    typedef PaGeo<PaF32, 13, 13> G;
+    return backward ? pa_go_bwd<PaF32, G, 8>(a, p, st) : pa_go_fwd<PaF32, G, 4, 3>(a, st);
+}

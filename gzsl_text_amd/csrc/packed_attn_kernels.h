@@ -1,75 +1,119 @@
-// Kernels of the packed label attention, instantiated for fp32 in packed_attn_f32.hip and for bf16 in packed_attn_bf16.hip; the
-// mathematics, the fragments, the tile images and the cut of the work are in packed_attn.h.
+// Kernels of the packed label attention, instantiated by kind of product in packed_attn_{bf16,x3,f32}.hip; the mathematics, the
+// fragments, the tile images and the cut of the work are in packed_attn.h.
 #pragma once
 #include <type_traits>
 #include "packed_attn.h"
 
 // ------------------------------------------------------------------------------------------------------------- pre-pass
-// One 16-byte chunk of an image row from a row of W elements (nullptr: zeros).
-template <typename T>
-__device__ __forceinline__ u32x4 pa_chunk(const T* row, int e0, int W) {
-    constexpr int KF = 16 / sizeof(T);
-    if (row == nullptr || e0 >= W) return u32x4{0, 0, 0, 0};
-    const T* p = row + e0;
-    if (e0 + KF <= W) {
-        if (((uintptr_t)p & 15) == 0) return *reinterpret_cast<const u32x4*>(p);
-        if (((uintptr_t)p & 7) == 0) {
-            const u32x2 lo = reinterpret_cast<const u32x2*>(p)[0], hi = reinterpret_cast<const u32x2*>(p)[1];
-            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+// A tile's rows into LDS, zeros past nrows and past W (row stride P elements).
+template <typename T, int ROWS, int P>
+__device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld, int row0, int nrows, int W, int tid) {
+    if (((uintptr_t)src & 15) == 0 && ld % (16 / sizeof(T)) == 0 && W % (16 / sizeof(T)) == 0) {
+        constexpr int V = 16 / sizeof(T), C = P / V;
+        typedef T vec __attribute__((ext_vector_type(V)));
+        for (int c = tid; c < ROWS * C; c += 256) {
+            const int r = c / C, e = c % C * V;
+            vec v;
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = (T)0.f;
+            if (row0 + r < nrows && e < W) v = *reinterpret_cast<const vec*>(src + (long long)(row0 + r) * ld + e);
+            *reinterpret_cast<vec*>(&sh[r][e]) = v;
+        }
+    } else {
+        for (int c = tid; c < ROWS * P; c += 256) {
+            const int r = c / P, e = c % P;
+            sh[r][e] = row0 + r < nrows && e < W ? src[(long long)(row0 + r) * ld + e] : (T)0.f;
         }
     }
-    T v[KF];
-#pragma unroll
-    for (int j = 0; j < KF; ++j) v[j] = e0 + j < W ? p[j] : (T)0.f;
-    return __builtin_bit_cast(u32x4, v);
 }
-template <typename T, int ROWS>
-__device__ __forceinline__ void pa_image(char* img, int pitch, const T* src, long long ld, int row0, int nrows, int W, int tid, int nt) {
-    const int per = pitch / 16;
-    for (int c = tid; c < ROWS * per; c += nt) {
-        const int r = c / per, k = c - r * per;
-        const u32x4 v = pa_chunk<T>(row0 + r < nrows ? src + (long long)(row0 + r) * ld : nullptr, k * (16 / (int)sizeof(T)), W);
-        *reinterpret_cast<u32x4*>(img + r * pitch + 16 * k) = v;
+// Row (ROW) or column fragments of the staged tile: N of them (a plane), written 1 KB a wave.
+template <class K, class G, int N, int STEPS, bool ROW, int P>
+__device__ __forceinline__ void pa_emit(typename K::T (*sh)[P], char* img, int tid) {
+    typedef typename K::M M;
+    const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+    for (int i = tid >> 6; i < N; i += 4) {
+        typename K::T x[G::KF];
+#pragma unroll
+        for (int j = 0; j < G::KF; ++j) {
+            if (ROW) x[j] = sh[16 * (i / STEPS) + n][i % STEPS * G::KK + g * G::KF + j];
+            else x[j] = sh[16 * (j >> 2) + 4 * g + (j & 3)][16 * i + n];
+        }
+        char* at = img + i * 1024 + lane * 16;
+        if constexpr (K::PL == 1) {
+            M v[G::KF];
+#pragma unroll
+            for (int j = 0; j < G::KF; ++j) v[j] = x[j];
+            *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, v);
+        } else {
+            bf16x8 p[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                bf16 h, m, l;
+                pa_split(x[j], h, m, l);
+                p[0][j] = h, p[1][j] = m, p[2][j] = l;
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(at + q * N * 1024) = p[q];
+        }
     }
 }
-// Blocks [0, B nT): key and value images of a token tile; then nQ blocks of query images.
-template <typename T, class G>
+// Blocks [0, B nT): a token tile (keys, values); then nQ blocks of queries.
+template <class K, class G, bool BWD>
 __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
-    const int id = blockIdx.x, nTok = a.B * a.nT;
+    typedef typename K::T T;
+    constexpr int PE = G::SE * G::KK, PF = G::SF * G::KK;
+    __shared__ __attribute__((aligned(16))) T se[G::ROWS][PE + 16 / sizeof(T)], sf[G::ROWS][PF + 16 / sizeof(T)];
+    const int id = blockIdx.x, nTok = a.B * a.nT, tid = threadIdx.x;
     if (id < nTok) {
         const int b = id / a.nT, t = id % a.nT;
         const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
         if (t * G::ROWS >= sp.len) return;
-        char* img = a.KV + (long long)id * G::KV;
-        pa_image<T, G::ROWS>(img, G::PE, (const T*)a.keys + sp.start * a.ldk, a.ldk, t * G::ROWS, sp.len, a.E, threadIdx.x, 256);
-        pa_image<T, G::ROWS>(img + G::EB, G::PF, (const T*)a.values + sp.start * a.ldv, a.ldv, t * G::ROWS, sp.len, a.F, threadIdx.x, 256);
+        pa_stage<T, G::ROWS>(se, (const T*)a.keys + sp.start * a.ldk, a.ldk, t * G::ROWS, sp.len, a.E, tid);
+        pa_stage<T, G::ROWS>(sf, (const T*)a.values + sp.start * a.ldv, a.ldv, t * G::ROWS, sp.len, a.F, tid);
+        __syncthreads();
+        char* img = a.TK + (long long)id * (BWD ? G::TOK : G::FWD) * 1024;
+        pa_emit<K, G, G::RE, G::SE, true>(se, img, tid);
+        img += G::PL * G::RE * 1024;
+        if (!BWD) {
+            pa_emit<K, G, G::NF, 1, false>(sf, img, tid);
+        } else {
+            pa_emit<K, G, G::RF, G::SF, true>(sf, img, tid);
+            if (!G::TR) pa_emit<K, G, G::NE, 1, false>(se, img + G::PL * G::RF * 1024, tid);
+        }
     } else {
         const int q = id - nTok;
-        pa_image<T, G::ROWS>(a.Q + (long long)q * G::QB, G::PE, (const T*)a.queries, a.ldq, q * G::ROWS, a.L, a.E, threadIdx.x, 256);
+        pa_stage<T, G::ROWS>(se, (const T*)a.queries, a.ldq, q * G::ROWS, a.L, a.E, tid);
+        __syncthreads();
+        char* img = a.Q + (long long)q * (BWD ? G::QRY : G::PL * G::RE) * 1024;
+        pa_emit<K, G, G::RE, G::SE, true>(se, img, tid);
+        if (BWD && !G::TR) pa_emit<K, G, G::NE, 1, false>(se, img + G::RE * 1024, tid);
     }
 }
-// Backward: dO images of (note, label tile); behind the rows, for each label, off and scale of its weights
+// Backward: dO images of (note, label tile); behind the fragments, for each label, off and scale of its weights
 // P = exp2(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; scale 0 past the
-// last label) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  `TPR` threads a row.
-template <typename T, class G>
+// last label) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.
+template <class K, class G>
 __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
-    constexpr int TPR = 256 / G::ROWS;
+    typedef typename K::T T;
+    constexpr int TPR = 256 / G::ROWS, PF = G::SF * G::KK;
+    __shared__ __attribute__((aligned(16))) T sf[G::ROWS][PF + 16 / sizeof(T)];
     const int q = blockIdx.x % a.nQ, b = blockIdx.x / a.nQ, tid = threadIdx.x;
-    char* img = a.DO + ((long long)b * a.nQ + q) * G::OB;
-    const T* dO = (const T*)a.dO + (long long)b * a.L * a.F;
-    pa_image<T, G::ROWS>(img, G::PF, dO, a.F, q * G::ROWS, a.L, a.F, tid, 256);
+    char* img = a.DO + ((long long)b * a.nQ + q) * G::OUT * 1024;
+    pa_stage<T, G::ROWS>(sf, (const T*)a.dO + (long long)b * a.L * a.F, a.F, q * G::ROWS, a.L, a.F, tid);
+    __syncthreads();
     const int r = tid / TPR, l = q * G::ROWS + r;
     const long long row = (long long)b * a.L + l;
     float s = 0.f;
     if (l < a.L) {
-        const T *x = dO + (long long)l * a.F, *y = (const T*)a.cO + row * a.F;
+        const T* y = (const T*)a.cO + row * a.F;
         const bf16* low = sizeof(T) == 2 && a.crest ? reinterpret_cast<const bf16*>(a.crest + 2LL * a.B * a.L) + row * a.F : nullptr;
-        for (int f = tid % TPR; f < a.F; f += TPR) s = fmaf((float)x[f], (float)y[f] + (low ? (float)low[f] : 0.f), s);
+#pragma unroll 4
+        for (int f = tid % TPR; f < a.F; f += TPR) s = fmaf((float)sf[r][f], (float)y[f] + (low ? (float)low[f] : 0.f), s);
     }
 #pragma unroll
     for (int o = 1; o < TPR; o <<= 1) s += __shfl_xor(s, o);
     if (tid % TPR == 0) {
-        float* aux = reinterpret_cast<float*>(img + G::FB);
+        float* aux = reinterpret_cast<float*>(img + (G::OUT - 1) * 1024);
         float off = 0.f, scale = 0.f;
         if (l < a.L) {
             if (a.crest) off = a.crest[2 * row], scale = a.crest[2 * row + 1];
@@ -79,6 +123,8 @@ __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
         aux[G::ROWS + r] = scale;
         aux[2 * G::ROWS + r] = s;
     }
+    pa_emit<K, G, G::RF, G::SF, true>(sf, img, tid);
+    if (!G::TR) pa_emit<K, G, G::NF, 1, false>(sf, img + G::PL * G::RF * 1024, tid);
 }
 
 // Four consecutive values of an output row, and what rounding them dropped.
@@ -114,10 +160,11 @@ __device__ __forceinline__ void pa_out(const f32x4& v, T* row, bf16* low, int c,
 
 // -------------------------------------------------------------------------------------------------------------- forward
 // Workgroup = WAVES x 16 labels of one note (or of one chunk of it); labels on the lane axis.
-template <typename T, class G, int WAVES, bool CAP, bool DROP>
-__global__ __launch_bounds__(WAVES * 64, (sizeof(T) == 2 && G::NE == 7) ? 4 : (sizeof(T) == 2 ? 3 : 2)) void pa_fwd_kernel(PaArgs a) {
-    typedef typename PaTy<T>::frag frag;
-    constexpr int U = G::U;
+template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
+__global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
+    typedef typename K::T T;
+    typedef typename K::frag frag;
+    constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int lt = blockIdx.x % a.nLT;
@@ -126,14 +173,15 @@ __global__ __launch_bounds__(WAVES * 64, (sizeof(T) == 2 && G::NE == 7) ? 4 : (s
     const int b = un.b, len = un.sp.len;
     const int t0 = un.c * (un.chunk / G::ROWS), t1 = (int)min((long long)(len + G::ROWS - 1) / G::ROWS, (long long)t0 + un.chunk / G::ROWS);
     const int l0 = (lt * WAVES + wave) * 16;
+    const bool idle = l0 >= a.L;  // (wave-uniform: copies and barriers only)
     const PaCap cap = pa_cap(a.cap);
 
     frag qf[G::SE];
     {
-        const int l = min(l0 + n, a.nQ * G::ROWS - 1);
-        const char* row = a.Q + (long long)(l / G::ROWS) * G::QB + (l % G::ROWS) * G::PE + 16 * g;
+        const int c = min(l0, a.nQ * G::ROWS - 16);
+        const char* img = a.Q + (long long)(c / G::ROWS) * G::PL * G::RE * 1024;
 #pragma unroll
-        for (int s = 0; s < G::SE; ++s) qf[s] = *reinterpret_cast<const frag*>(row + 64 * s);
+        for (int s = 0; s < G::SE; ++s) qf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
     }
     const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + (uint32_t)(l0 + n));
     f32x4 acc[G::NF];
@@ -143,66 +191,69 @@ __global__ __launch_bounds__(WAVES * 64, (sizeof(T) == 2 && G::NE == 7) ? 4 : (s
     // nothing is ever rescaled.  Otherwise a tile whose maximum exceeds the running one by more than 2^12 moves it.
     const bool fixed = CAP && a.cap <= 30.f;
     float m = fixed ? 0.f : -INFINITY, sum = 0.f;
-    const char* kv = a.KV + (long long)b * a.nT * G::KV;
-    if (t0 < t1) pa_dma<WAVES>(kv + (long long)t0 * G::KV, sm, G::KV, wave, lane);
+    const char* tk = a.TK + (long long)b * a.nT * G::FWD * 1024;
+    if (t0 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)t0 * G::FWD * 1024, sm, wave, lane);
     pa_arrive();
     auto step = [&](int t, auto last) {  // last: the tile may end behind the note
-        const char* K = sm + ((t - t0) & 1) * G::KV;
-        const char* V = K + G::EB;
-        if (t + 1 < t1) pa_dma<WAVES>(kv + (long long)(t + 1) * G::KV, sm + ((t - t0 + 1) & 1) * G::KV, G::KV, wave, lane);
-        f32x4 s[U];
+        const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
+        const char* VC = KR + G::PL * G::RE * 1024;
+        if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)(t + 1) * G::FWD * 1024, sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
+        if (!idle) {
+            f32x4 s[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < U; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            frag ring[D];
+            auto ldk = [&](int i) { return pa_frag<K, G::RE>(KR, i % U * G::SE + i / U, lane); };
+            auto ldv = [&](int j) { return pa_frag<K, G::NF>(VC, j, lane); };
+            pa_fill_ring<G::RE>(ring, ldk);
+            pa_run_ring<G::RE>(ring, ldk, [&](int i, const frag& f) { s[i % U] = pa_mma(f, qf[i / U], s[i % U]); });
+            pa_fill_ring<G::NF>(ring, ldv);  // under way during the softmax
+            float y[U][4], th[U][4];
+            pa_scores<K, CAP, U, false>(s, cap, y, th);
+            if constexpr (decltype(last)::value) {
+                const int left = len - t * G::ROWS;
 #pragma unroll
-            for (int k = 0; k < G::SE; ++k) s[u] = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s[u]);
-        }
-        float y[U][4], th[U][4];
-        pa_scores<T, CAP, U, false>(s, cap, y, th);
-        if constexpr (decltype(last)::value) {
-            const int left = len - t * G::ROWS;
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * u + 4 * g + r >= left) y[u][r] = -INFINITY;
-        }
-        if (!fixed) {
-            float mt = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
-            if (__any(mt > m + 12.f)) {  // m is the same in the four lanes of a column
-                mt = fmaxf(mt, __shfl_xor(mt, 16));
-                mt = fmaxf(mt, __shfl_xor(mt, 32));
-                const float mn = fmaxf(m, mt), alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-                for (int j = 0; j < G::NF; ++j) acc[j] *= alpha;
-                sum *= alpha;
-                m = mn;
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * u + 4 * g + r >= left) y[u][r] = -INFINITY;
             }
-            const float mi = m == -INFINITY ? 0.f : m;  // (no finite score yet: every weight is 2^-inf = 0)
+            if (!fixed) {
+                float mt = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[u][r] -= mi;
-        }
-        frag pf;
-        {
-            float p[U][4];
+                    for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
+                if (__any(mt > m + 12.f)) {  // m is the same in the four lanes of a column
+                    mt = fmaxf(mt, __shfl_xor(mt, 16));
+                    mt = fmaxf(mt, __shfl_xor(mt, 32));
+                    const float mn = fmaxf(m, mt), alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[u][r] = __builtin_amdgcn_exp2f(y[u][r]);
-                    sum += p[u][r];
-                    if (DROP) p[u][r] = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
+                    for (int j = 0; j < G::NF; ++j) acc[j] *= alpha;
+                    sum *= alpha;
+                    m = mn;
                 }
-            pa_pack(p, pf);
-        }
+                const float mi = m == -INFINITY ? 0.f : m;  // (no finite score yet: every weight is 2^-inf = 0)
 #pragma unroll
-        for (int j = 0; j < G::NF; ++j) acc[j] = pa_mma(pa_col<T>(V, G::PF, 0, 16 * j, n, g), pf, acc[j]);
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[u][r] -= mi;
+            }
+            frag pf;
+            {
+                float p[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[u][r] = __builtin_amdgcn_exp2f(y[u][r]);
+                        sum += p[u][r];
+                        if (DROP) p[u][r] = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
+                    }
+                pa_pack(p, pf);
+            }
+            pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) { acc[j] = pa_mma(f, pf, acc[j]); });
+        }
         pa_arrive();
     };
     for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
@@ -310,105 +361,127 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
     if (CAP) ds *= fmaf(-th, th, 1.f);
 }
 
-// dK / dV: workgroup = 64 tokens of one note (16 a wave, tokens on the lane axis), sweeping its share of the labels.
-template <typename T, class G, bool CAP, bool DROP>
-__global__ __launch_bounds__(256, 2) void pa_bwd_kv_kernel(PaArgs a) {
-    typedef typename PaTy<T>::frag frag;
+// dK / dV: workgroup = 128 tokens of one note (16 a wave, tokens on the lane axis), sweeping its share of the labels.  PaX3 takes dV
+// and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a wave at two
+// waves a SIMD, and the scores a second time are a fifth of the products.
+template <class K, class G, int PART, bool CAP, bool DROP>
+__global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
+    typedef typename K::T T;
+    typedef typename K::frag frag;
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    constexpr int BUF = G::QB + G::OB, WAVES = PA_TILE / 16, U = G::U;
+    constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U, D = G::PL == 3 ? 2 : 4;
+    constexpr bool DV = PART & 1, DK = PART & 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const PaTileUnit un = pa_tile_unit(a, blockIdx.x);
     if (un.b < 0) return;
     const int b = un.b, len = un.sp.len;
     const int per = (a.nQ + un.shares - 1) / un.shares, q0 = un.share * per, q1 = min(a.nQ, q0 + per);
-    const int tok = (un.tile * WAVES + wave) * 16 + n;
+    const int tok0 = (un.tile * WAVES + wave) * 16, tok = tok0 + n;
+    const bool idle = tok0 >= len;  // (wave-uniform: copies and barriers only)
     const PaCap cap = pa_cap(a.cap);
-    frag kf[G::SE], vf[G::SF];
+    frag kf[G::SE], vf[DK ? G::SF : 1];
     {
-        const int t = min(tok, (len - 1) / G::ROWS * G::ROWS + G::ROWS - 1);  // inside the note's last tile image
-        const char* img = a.KV + ((long long)b * a.nT + t / G::ROWS) * G::KV + 16 * g;
+        const int c = min(tok0, (len - 1) / 16 * 16);
+        const char* img = a.TK + ((long long)b * a.nT + c / G::ROWS) * G::TOK * 1024;
 #pragma unroll
-        for (int s = 0; s < G::SE; ++s) kf[s] = *reinterpret_cast<const frag*>(img + (t % G::ROWS) * G::PE + 64 * s);
+        for (int s = 0; s < G::SE; ++s) kf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
+        if (DK)
 #pragma unroll
-        for (int s = 0; s < G::SF; ++s) vf[s] = *reinterpret_cast<const frag*>(img + G::EB + (t % G::ROWS) * G::PF + 64 * s);
+            for (int s = 0; s < G::SF; ++s) vf[s] = pa_frag<K, G::RF>(img + G::PL * G::RE * 1024, (c % G::ROWS / 16) * G::SF + s, lane);
     }
-    f32x4 dv[G::NF], dk[G::NE];
+    f32x4 dv[DV ? G::NF : 1], dk[DK ? G::NE : 1];
 #pragma unroll
-    for (int j = 0; j < G::NF; ++j) dv[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < (DV ? G::NF : 1); ++j) dv[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < G::NE; ++j) dk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const char* dO = a.DO + (long long)b * a.nQ * G::OB;
+    for (int j = 0; j < (DK ? G::NE : 1); ++j) dk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const char* dO = a.DO + (long long)b * a.nQ * G::OUT * 1024;
     auto fetch = [&](int q, char* buf) {
-        pa_dma<WAVES>(a.Q + (long long)q * G::QB, buf, G::QB, wave, lane);
-        pa_dma<WAVES>(dO + (long long)q * G::OB, buf + G::QB, G::OB, wave, lane);
+        pa_dma<WAVES, G::QRY>(a.Q + (long long)q * G::QRY * 1024, buf, wave, lane);
+        pa_dma<WAVES, G::OUT>(dO + (long long)q * G::OUT * 1024, buf + G::QRY * 1024, wave, lane);
     };
     if (q0 < q1) fetch(q0, sm);
     pa_arrive();
     for (int q = q0; q < q1; ++q) {
-        const char* Q = sm + ((q - q0) & 1) * BUF;
-        const char* D = Q + G::QB;
-        const float* aux = reinterpret_cast<const float*>(D + G::FB);
+        const char* QR = sm + ((q - q0) & 1) * BUF;
+        const char* DR = QR + G::QRY * 1024;
+        const float* aux = reinterpret_cast<const float*>(DR + (G::OUT - 1) * 1024);
         if (q + 1 < q1) fetch(q + 1, sm + ((q - q0 + 1) & 1) * BUF);
-        float p[U][4], ds[U][4], y[U][4], th[U][4];
-        f32x4 s[U], dp[U];
+        if (!idle) {
+            f32x4 s[U], dp[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < U; ++u) s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            frag ring[D];
+            // rows of the queries, then rows of dO
+            constexpr int NS = G::RE + (DK ? G::RF : 0);
+            auto ldr = [&](int i) {
+                return i < G::RE ? pa_frag<K, G::RE>(QR, i % U * G::SE + i / U, lane) : pa_frag<K, G::RF>(DR, (i - G::RE) % U * G::SF + (i - G::RE) / U, lane);
+            };
+            pa_fill_ring<NS>(ring, ldr);
+            pa_run_ring<NS>(ring, ldr, [&](int i, const frag& f) {
+                if (i < G::RE) s[i % U] = pa_mma(f, kf[i / U], s[i % U]);
+                else dp[(i - G::RE) % U] = pa_mma(f, vf[DK ? (i - G::RE) / U : 0], dp[(i - G::RE) % U]);
+            });
+            auto ldv = [&](int j) {
+                if constexpr (G::TR) return pa_col_tr<G::SF>(DR, j, n, g);
+                else return pa_frag<K, G::NF>(DR + G::RF * 1024, j, lane);
+            };
+            auto ldk = [&](int j) {
+                if constexpr (G::TR) return pa_col_tr<G::SE>(QR, j, n, g);
+                else return pa_frag<K, G::NE>(QR + G::RE * 1024, j, lane);
+            };
+            constexpr int NC = (DV ? G::NF : 0) + (DK ? G::NE : 0);
+            auto ldc = [&](int j) { return DV && j < G::NF ? ldv(j) : ldk(j - (DV ? G::NF : 0)); };
+            pa_fill_ring<NC>(ring, ldc);
+            float p[U][4], ds[U][4], y[U][4], th[U][4];
+            pa_scores<K, CAP, U, DK>(s, cap, y, th);
 #pragma unroll
-            for (int k = 0; k < G::SF; ++k) {
-                if (k < G::SE) s[u] = pa_mma(pa_row<T>(Q, G::PE, 16 * u, k, n, g), kf[k], s[u]);
-                dp[u] = pa_mma(pa_row<T>(D, G::PF, 16 * u, k, n, g), vf[k], dp[u]);
-            }
-        }
-        pa_scores<T, CAP, U, true>(s, cap, y, th);
+            for (int u = 0; u < U; ++u) {
+                const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
+                            delta = *reinterpret_cast<const f32x4*>(aux + 2 * G::ROWS + 16 * u + 4 * g);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
-                        delta = *reinterpret_cast<const f32x4*>(aux + 2 * G::ROWS + 16 * u + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float keep = 1.f;
-                if (DROP) {
-                    const uint32_t l = (uint32_t)(q * G::ROWS + 16 * u + 4 * g + r);
-                    const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
-                    keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
+                for (int r = 0; r < 4; ++r) {
+                    float keep = 1.f;
+                    if (DROP) {
+                        const uint32_t l = (uint32_t)(q * G::ROWS + 16 * u + 4 * g + r);
+                        const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
+                        keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
+                    }
+                    pa_grad<CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
                 }
-                pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
             }
-        }
-        frag pf, sf;
-        pa_pack(p, pf);
-        pa_pack(ds, sf);
-#pragma unroll
-        for (int j = 0; j < G::NF; ++j) dv[j] = pa_mma(pa_col<T>(D, G::PF, 0, 16 * j, n, g), pf, dv[j]);
-        if constexpr (sizeof(T) == 2) {
-            frag sl;
-            pa_pack_low(ds, sl);
-#pragma unroll
-            for (int j = 0; j < G::NE; ++j) {
-                const frag f = pa_col<T>(Q, G::PE, 0, 16 * j, n, g);
-                dk[j] = pa_mma(f, sf, pa_mma(f, sl, dk[j]));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < G::NE; ++j) dk[j] = pa_mma(pa_col<T>(Q, G::PE, 0, 16 * j, n, g), sf, dk[j]);
+            frag pf, sf;
+            bf16x8 sl;
+            if (DV) pa_pack(p, pf);
+            if (DK) pa_pack(ds, sf);
+            if constexpr (DK && sizeof(T) == 2) pa_pack_low(ds, sl);
+            pa_run_ring<NC>(ring, ldc, [&](int j, const frag& f) {
+                if (DV && j < G::NF) {
+                    dv[DV ? j : 0] = pa_mma(f, pf, dv[DV ? j : 0]);
+                } else {
+                    const int e = DK ? j - (DV ? G::NF : 0) : 0;
+                    if constexpr (sizeof(T) == 2) dk[e] = pa_mma(f, sl, dk[e]);
+                    dk[e] = pa_mma(f, sf, dk[e]);
+                }
+            });
         }
         pa_arrive();
     }
     if (tok >= len) return;
     const long long row = un.sp.start + tok;
-    if (un.shares > 1) {
-        float* out = a.dkv + ((long long)un.unit * PA_TILE + wave * 16 + n) * (a.E + a.F);
+    const bool slab = un.shares > 1;
+    float* part = a.dkv + ((long long)un.unit * PA_TILE + wave * 16 + n) * (a.E + a.F);
+    if (DK)
 #pragma unroll
-        for (int j = 0; j < G::NE; ++j) pa_out<float>(dk[j], out, nullptr, 16 * j + 4 * g, a.E);
+        for (int j = 0; j < G::NE; ++j) {
+            if (slab) pa_out<float>(dk[j], part, nullptr, 16 * j + 4 * g, a.E);
+            else pa_out<T>(dk[j], (T*)a.dK + row * a.E, nullptr, 16 * j + 4 * g, a.E);
+        }
+    if (DV)
 #pragma unroll
-        for (int j = 0; j < G::NF; ++j) pa_out<float>(dv[j], out + a.E, nullptr, 16 * j + 4 * g, a.F);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < G::NE; ++j) pa_out<T>(dk[j], (T*)a.dK + row * a.E, nullptr, 16 * j + 4 * g, a.E);
-#pragma unroll
-    for (int j = 0; j < G::NF; ++j) pa_out<T>(dv[j], (T*)a.dV + row * a.F, nullptr, 16 * j + 4 * g, a.F);
+        for (int j = 0; j < G::NF; ++j) {
+            if (slab) pa_out<float>(dv[j], part + a.E, nullptr, 16 * j + 4 * g, a.F);
+            else pa_out<T>(dv[j], (T*)a.dV + row * a.F, nullptr, 16 * j + 4 * g, a.F);
+        }
 }
 // dK / dV from the label shares, in order, and zeros in the rows of no note: 16 rows a workgroup, counted from a note's first
 // (blockIdx.y = B: the rows in front of the first note), a wave to a row.
@@ -458,10 +531,11 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
 }
 
 // dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.
-template <typename T, class G, int WAVES, bool CAP, bool DROP>
+template <class K, class G, int WAVES, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
-    typedef typename PaTy<T>::frag frag;
-    constexpr int U = G::U;
+    typedef typename K::T T;
+    typedef typename K::frag frag;
+    constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int lt = blockIdx.x % a.nLT;
@@ -470,72 +544,77 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     const int b = un.b, len = un.sp.len;
     const int t0 = un.c * (un.chunk / G::ROWS), t1 = (int)min((long long)(len + G::ROWS - 1) / G::ROWS, (long long)t0 + un.chunk / G::ROWS);
     const int l0 = (lt * WAVES + wave) * 16;
+    const bool idle = l0 >= a.L;
     const PaCap cap = pa_cap(a.cap);
     frag qf[G::SE], df[G::SF];
     float off, scale, delta;
     {
-        const int l = min(l0 + n, a.nQ * G::ROWS - 1);
-        const char* qr = a.Q + (long long)(l / G::ROWS) * G::QB + (l % G::ROWS) * G::PE + 16 * g;
-        const char* dimg = a.DO + ((long long)b * a.nQ + l / G::ROWS) * G::OB;
+        const int c = min(l0, a.nQ * G::ROWS - 16), u = c % G::ROWS / 16;
+        const char* qi = a.Q + (long long)(c / G::ROWS) * G::QRY * 1024;
+        const char* di = a.DO + ((long long)b * a.nQ + c / G::ROWS) * G::OUT * 1024;
 #pragma unroll
-        for (int s = 0; s < G::SE; ++s) qf[s] = *reinterpret_cast<const frag*>(qr + 64 * s);
+        for (int s = 0; s < G::SE; ++s) qf[s] = pa_frag<K, G::RE>(qi, u * G::SE + s, lane);
 #pragma unroll
-        for (int s = 0; s < G::SF; ++s) df[s] = *reinterpret_cast<const frag*>(dimg + (l % G::ROWS) * G::PF + 16 * g + 64 * s);
-        const float* aux = reinterpret_cast<const float*>(dimg + G::FB);
-        off = aux[l % G::ROWS], scale = aux[G::ROWS + l % G::ROWS], delta = aux[2 * G::ROWS + l % G::ROWS];
+        for (int s = 0; s < G::SF; ++s) df[s] = pa_frag<K, G::RF>(di, u * G::SF + s, lane);
+        const float* aux = reinterpret_cast<const float*>(di + (G::OUT - 1) * 1024) + 16 * u + n;
+        off = aux[0], scale = aux[G::ROWS], delta = aux[2 * G::ROWS];
     }
     const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + (uint32_t)(l0 + n));
     f32x4 dq[G::NE];
 #pragma unroll
     for (int j = 0; j < G::NE; ++j) dq[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const char* kv = a.KV + (long long)b * a.nT * G::KV;
-    if (t0 < t1) pa_dma<WAVES>(kv + (long long)t0 * G::KV, sm, G::KV, wave, lane);
+    const char* tk = a.TK + (long long)b * a.nT * G::TOK * 1024;
+    if (t0 < t1) pa_dma<WAVES, G::TOK>(tk + (long long)t0 * G::TOK * 1024, sm, wave, lane);
     pa_arrive();
     auto step = [&](int t, auto last) {  // last: the tile may end behind the note
-        const char* K = sm + ((t - t0) & 1) * G::KV;
-        const char* V = K + G::EB;
-        if (t + 1 < t1) pa_dma<WAVES>(kv + (long long)(t + 1) * G::KV, sm + ((t - t0 + 1) & 1) * G::KV, G::KV, wave, lane);
-        float ds[U][4], y[U][4], th[U][4];
-        f32x4 s[U], dp[U];
+        const char* KR = sm + ((t - t0) & 1) * G::TOK * 1024;
+        const char* VR = KR + G::PL * G::RE * 1024;
+        if (t + 1 < t1) pa_dma<WAVES, G::TOK>(tk + (long long)(t + 1) * G::TOK * 1024, sm + ((t - t0 + 1) & 1) * G::TOK * 1024, wave, lane);
+        if (!idle) {
+            f32x4 s[U], dp[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < G::SF; ++k) {
-                if (k < G::SE) s[u] = pa_mma(pa_row<T>(K, G::PE, 16 * u, k, n, g), qf[k], s[u]);
-                dp[u] = pa_mma(pa_row<T>(V, G::PF, 16 * u, k, n, g), df[k], dp[u]);
-            }
-        }
-        pa_scores<T, CAP, U, true>(s, cap, y, th);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float keep = 1.f, p;
-                if (DROP) keep = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? a.scale : 0.f;
-                pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
-            }
-        if constexpr (decltype(last)::value) {  // (a key of zeros has the score 0, which may be far above the note's own)
-            const int left = len - t * G::ROWS;
+            for (int u = 0; u < U; ++u) s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            frag ring[D];
+            constexpr int NS = G::RE + G::RF;
+            auto ldr = [&](int i) {
+                return i < G::RE ? pa_frag<K, G::RE>(KR, i % U * G::SE + i / U, lane) : pa_frag<K, G::RF>(VR, (i - G::RE) % U * G::SF + (i - G::RE) / U, lane);
+            };
+            pa_fill_ring<NS>(ring, ldr);
+            pa_run_ring<NS>(ring, ldr, [&](int i, const frag& f) {
+                if (i < G::RE) s[i % U] = pa_mma(f, qf[i / U], s[i % U]);
+                else dp[(i - G::RE) % U] = pa_mma(f, df[(i - G::RE) / U], dp[(i - G::RE) % U]);
+            });
+            auto ldc = [&](int j) {
+                if constexpr (G::TR) return pa_col_tr<G::SE>(KR, j, n, g);
+                else return pa_frag<K, G::NE>(VR + G::RF * 1024, j, lane);
+            };
+            pa_fill_ring<G::NE>(ring, ldc);
+            float ds[U][4], y[U][4], th[U][4];
+            pa_scores<K, CAP, U, true>(s, cap, y, th);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * u + 4 * g + r >= left) ds[u][r] = 0.f;
-        }
-        frag sf;
-        pa_pack(ds, sf);
-        if constexpr (sizeof(T) == 2) {
-            frag sl;
-            pa_pack_low(ds, sl);
+                for (int r = 0; r < 4; ++r) {
+                    float keep = 1.f, p;
+                    if (DROP) keep = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? a.scale : 0.f;
+                    pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
+                }
+            if constexpr (decltype(last)::value) {  // (a key of zeros has the score 0, which may be far above the note's own)
+                const int left = len - t * G::ROWS;
 #pragma unroll
-            for (int j = 0; j < G::NE; ++j) {
-                const frag f = pa_col<T>(K, G::PE, 0, 16 * j, n, g);
-                dq[j] = pa_mma(f, sf, pa_mma(f, sl, dq[j]));
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * u + 4 * g + r >= left) ds[u][r] = 0.f;
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < G::NE; ++j) dq[j] = pa_mma(pa_col<T>(K, G::PE, 0, 16 * j, n, g), sf, dq[j]);
+            frag sf;
+            bf16x8 sl;
+            pa_pack(ds, sf);
+            if constexpr (sizeof(T) == 2) pa_pack_low(ds, sl);
+            pa_run_ring<G::NE>(ring, ldc, [&](int j, const frag& f) {
+                if constexpr (sizeof(T) == 2) dq[j] = pa_mma(f, sl, dq[j]);
+                dq[j] = pa_mma(f, sf, dq[j]);
+            });
         }
         pa_arrive();
     };
@@ -561,10 +640,11 @@ __global__ __launch_bounds__(256) void pa_q_join_kernel(PaArgs a) {
 }
 
 // --------------------------------------------------------------------------------------------------------------- launch
-template <typename T, class G, int W, bool CAP, bool DROP>
+template <class K, class G, int W, int OCC, bool CAP, bool DROP>
 static int pa_fwd(PaArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((pa_pack_kernel<T, G>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((pa_fwd_kernel<T, G, W, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::KV, st, a);
+    typedef typename K::T T;
+    hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     if (a.extra > 0) {
         if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 4>), dim3(a.B * a.L), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 1>), dim3(a.B * cdiv(a.L, 4)), dim3(256), 0, st, a);
@@ -572,27 +652,39 @@ static int pa_fwd(PaArgs& a, hipStream_t st) {
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <typename T, class G, int W, bool CAP, bool DROP>
+template <class K, class G, int W, bool CAP, bool DROP>
 static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
-    hipLaunchKernelGGL((pa_pack_kernel<T, G>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((pa_pack_do_kernel<T, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
-    if (p.units > 0) hipLaunchKernelGGL((pa_bwd_kv_kernel<T, G, CAP, DROP>), dim3((unsigned)p.units), dim3(256), 2 * (G::QB + G::OB), st, a);
+    typedef typename K::T T;
+    constexpr int lds = 2 * (G::QRY + G::OUT) * 1024;
+    static_assert(lds <= 160 * 1024 && 2 * G::TOK <= 160 && 2 * G::FWD <= 160, "two buffers in LDS");
+    hipLaunchKernelGGL((pa_pack_kernel<K, G, true>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pa_pack_do_kernel<K, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
+    if (p.units > 0) {
+        if constexpr (G::PL == 3) {
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 1, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 2, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
+        } else {
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 3, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
+        }
+    }
     hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, PA_JOIN_ROWS) : 1, a.B + 1), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((pa_bwd_q_kernel<T, G, W, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::KV, st, a);
+    hipLaunchKernelGGL((pa_bwd_q_kernel<K, G, W, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::TOK * 1024, st, a);
     const long long n = (long long)a.L * a.E;
     hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS>), dim3((unsigned)(n < 256 * 4096 ? cdiv((long)n, 256) : 4096)), dim3(256), 0, st, a);
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <typename T, class G, int W, bool CAP>
-static int pa_go2(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) {
-    if (backward) return a.thresh ? pa_bwd<T, G, W, CAP, true>(a, p, st) : pa_bwd<T, G, W, CAP, false>(a, p, st);
-    return a.thresh ? pa_fwd<T, G, W, CAP, true>(a, st) : pa_fwd<T, G, W, CAP, false>(a, st);
+template <class K, class G, int W, int OCC, bool CAP>
+static int pa_fwd_drop(PaArgs& a, hipStream_t st) {
+    return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true>(a, st) : pa_fwd<K, G, W, OCC, CAP, false>(a, st);
 }
-template <typename T, int W>
-static int pa_go(PaArgs& a, const PaPlan& p, bool backward, hipStream_t st) {
-    typedef PaGeo<T, 7, 13> A;
-    typedef PaGeo<T, 13, 13> B;
-    if (a.cap > 0.f) return p.wide ? pa_go2<T, B, W, true>(a, p, backward, st) : pa_go2<T, A, W, true>(a, p, backward, st);
-    return p.wide ? pa_go2<T, B, W, false>(a, p, backward, st) : pa_go2<T, A, W, false>(a, p, backward, st);
+// W waves, OCC waves a SIMD asked of the compiler
+template <class K, class G, int W, int OCC>
+static int pa_go_fwd(PaArgs& a, hipStream_t st) {
+    return a.cap > 0.f ? pa_fwd_drop<K, G, W, OCC, true>(a, st) : pa_fwd_drop<K, G, W, OCC, false>(a, st);
+}
+template <class K, class G, int W>
+static int pa_go_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
+    if (a.cap > 0.f) return a.thresh ? pa_bwd<K, G, W, true, true>(a, p, st) : pa_bwd<K, G, W, true, false>(a, p, st);
+    return a.thresh ? pa_bwd<K, G, W, false, true>(a, p, st) : pa_bwd<K, G, W, false, false>(a, p, st);
 }
