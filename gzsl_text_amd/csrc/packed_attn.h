@@ -218,16 +218,22 @@ __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, f
     }
 }
 
-// Copies KB KB of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  The caller waits with
-// pa_arrive() before anyone reads.
+// Copies KB KB of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  `src` and `wave` are scalars.
+// The caller waits with pa_arrive() before anyone reads.  (Buffer loads: after the global form the compiler takes every LDS read for
+// one that may return out of order and waits for all of them each time.)
 template <int WAVES, int KB>
 __device__ __forceinline__ void pa_dma(const char* src, char* dst, int wave, int lane) {
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), 0, KB * 1024, 0x00020000);
 #pragma unroll
     for (int i = 0; i < (KB + WAVES - 1) / WAVES; ++i) {
         const int o = (wave + i * WAVES) * 1024;
         if (KB % WAVES == 0 || i < KB / WAVES || o < KB * 1024)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + o + 16 * lane), (GZ_LDS void*)(dst + o), 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (GZ_LDS void*)(dst + o), 16, 16 * lane, o, 0, 0);
     }
+}
+__device__ __forceinline__ int pa_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long pa_scalar(long long x) {
+    return (long long)(uint32_t)pa_scalar((int)x) | (long long)pa_scalar((int)(x >> 32)) << 32;
 }
 // this wave's copies have landed and every wave is past its reads of the other buffer
 __device__ __forceinline__ void pa_arrive() {
@@ -245,6 +251,7 @@ struct PaArgs {
     float scale;
     int nLT, extra;                   // label workgroups of a note; token chunks beyond one a note (0: notes are not cut)
     int shares, slots;                // dK / dV: label shares of a token tile at most, slabs that the workspace has room for
+    float slab;                       // time of a slab's write and read by the whole chip, in times of a tile on one compute unit
     // workspace
     char *TK, *Q, *DO;  // images: token tiles [B][nT], queries [nQ], dO [B][nQ]
     float *part, *ml;  // forward, notes cut: unnormalised O [chunk][L][F] and (max, sum) [chunk][L][2]
@@ -284,6 +291,7 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
         if (per < 256) per = 256;  // a share that pays for its own start and its part in the join
         chunk = (int)min(per / ROWS * ROWS + ROWS, (long long)0x7FFFFFC0);
     }
+    chunk = pa_scalar(chunk);
     u.chunk = chunk;
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -309,20 +317,24 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
         const unsigned long long hit = want_b >= 0 ? __ballot(note == want_b) : __ballot(base + incl > ci);
         if (u.b < 0 && hit) {
             const int src = __ffsll((long long)hit) - 1;
-            u.b = __shfl(note, src);
-            u.nch = __shfl(nch, src);
-            const int first = base + __shfl(incl, src) - u.nch;
+            u.b = pa_scalar(__shfl(note, src));
+            u.nch = pa_scalar(__shfl(nch, src));
+            const int first = base + pa_scalar(__shfl(incl, src)) - u.nch;
             u.c = ci - first;
             if (want_b >= 0) u.c = 0, u.ci = first;
         }
-        base += __shfl(incl, 63);
+        base += pa_scalar(__shfl(incl, 63));
     }
     u.all = base;
-    if (u.b >= 0) u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+    if (u.b >= 0) {
+        u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+        u.sp = {pa_scalar(u.sp.start), pa_scalar(u.sp.len)};
+    }
     return u;
 }
-// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  The parts are as many as fill the chip's 256 compute
-// units best, a slab written and read again counted as 2 % a part.
+// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  With s parts the chip's 256 compute units take
+// ceil(n s / 256) rounds of 1 / s of a tile's time, and n s slabs are written and read again, each a.slab of a round: the s that is
+// least.
 struct PaTileUnit {
     int b, tile, share, shares, unit, tiles;
     NoteSpan sp;
@@ -336,13 +348,13 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
     for (int b0 = 0; b0 < a.B; b0 += 64) n += tiles_of(b0 + lane);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    n = pa_scalar(n);
     u.tiles = n;
     u.shares = 1;
-    float best = -1.f;
+    float best = 1e30f;
     for (int s = 1; s <= a.shares && (s == 1 || (long long)n * s <= a.slots); ++s) {
-        const int all = n * s, rounds = (all + 255) / 256;
-        const float fill = rounds > 0 ? (float)all / (256.f * rounds) - 0.02f * s : 0.f;
-        if (fill > best) best = fill, u.shares = s;
+        const float t = (float)((n * s + 255) / 256) / s + (s > 1 ? a.slab * n * s : 0.f);
+        if (t < best) best = t, u.shares = s;
     }
     u.unit = unit;
     const int t = unit / u.shares;
@@ -358,18 +370,22 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
         }
         const unsigned long long hit = want_b >= 0 ? __ballot(b0 + lane == want_b) : __ballot(base + incl > t);
         if (u.b < 0 && hit) {
-            const int src = __ffsll((long long)hit) - 1, first = base + __shfl(incl, src) - __shfl(nt, src);
+            const int src = __ffsll((long long)hit) - 1, first = base + pa_scalar(__shfl(incl, src) - __shfl(nt, src));
             u.b = b0 + src;
             u.tile = want_b >= 0 ? first : t - first;  // want_b: the note's first tile among all
         }
-        base += __shfl(incl, 63);
+        base += pa_scalar(__shfl(incl, 63));
     }
-    if (u.b >= 0) u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+    if (u.b >= 0) {
+        u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+        u.sp = {pa_scalar(u.sp.start), pa_scalar(u.sp.len)};
+    }
     return u;
 }
 
 struct PaPlan {
     int nT, nQ, kind, waves, extra, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
+    float slab;
     long long units;  // workgroups of the dK / dV sweep
     long long kv, q, dO, part, ml, dq, dkv, bytes;
 };

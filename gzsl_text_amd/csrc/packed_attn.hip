@@ -22,11 +22,12 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     else if (p.kind == 1) pa_sizes<PaGeo<PaBF, 13, 13>>(p, *d, backward);
     else if (p.kind == 2) pa_sizes<PaGeo<PaX3, 7, 13>>(p, *d, backward);
     else pa_sizes<PaGeo<PaF32, 13, 13>>(p, *d, backward);
-    p.waves = p.kind == 3 && !backward ? 4 : 8;
+    // 128 labels a workgroup (64: PaF32's forward, and bf16 where 128 leave fewer workgroups than the chip has places, two a compute
+    // unit); notes are cut where the (note, label) workgroups alone would leave compute units without one.
+    p.waves = (p.kind == 3 && !backward) || (p.kind < 2 && (long long)d->B * cdiv(d->L, 128) < 512) ? 4 : 8;
     p.nLT = cdiv(d->L, 16 * p.waves);
-    // notes are cut where (note, label) workgroups alone do not fill the chip's places (one or two workgroups a compute unit)
-    const long long wgs = (long long)d->B * p.nLT, places = p.kind == 2 ? 256 : 512;
-    p.extra = wgs > 0 && wgs < places && d->max_len > 256 ? cdiv(places, p.nLT) : 0;
+    const long long wgs = (long long)d->B * p.nLT;
+    p.extra = wgs > 0 && wgs < 256 && d->max_len > 256 ? cdiv(p.waves == 4 ? 512 : 256, p.nLT) : 0;
     if (p.extra > d->B * (d->max_len / 256 + 1)) p.extra = d->B * (d->max_len / 256 + 1);
     const long long chunks = d->B + p.extra;
     if ((long long)d->B * p.nT + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
@@ -40,6 +41,9 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
         long long tiles = (long long)d->B * cdiv(d->max_len, PA_TILE);  // at most
         if (tiles > d->rows / PA_TILE + d->B) tiles = d->rows / PA_TILE + d->B;
         p.shares = p.nQ / 4 < 1 ? 1 : (p.nQ / 4 > 16 ? 16 : p.nQ / 4);  // (four label tiles a share at least)
+        // a slab moves (E + F) 8 bytes a token at 4 TB/s; a tile's scores take L / (scores a ns of the chip / 256) a token on one unit
+        const float rate = p.kind < 2 ? 300.f : (p.kind == 2 ? 113.f : 80.f);
+        p.slab = (d->E + d->F) * 8 / 4000.f * rate / 256.f / (float)(d->L > 0 ? d->L : 1);
         // the number of shares is chosen on the device, at most 1024 units of more than one share
         p.units = p.shares > 1 ? (tiles * p.shares < 1024 ? tiles * p.shares : (tiles > 1024 ? tiles : 1024)) : tiles;
         if (p.units > 0x3FFFFFFF) return GZSL_ETOOBIG;
@@ -54,7 +58,7 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.rows = d.rows, a.ldk = d.ldk, a.ldv = d.ldv, a.ldq = d.ldq;
     a.B = d.B, a.max_len = d.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
-    a.nLT = p.nLT, a.extra = p.extra, a.shares = p.shares, a.slots = p.slots;
+    a.nLT = p.nLT, a.extra = p.extra, a.shares = p.shares, a.slots = p.slots, a.slab = p.slab;
     char* w = (char*)work;
     a.TK = w, w += p.kv;
     a.Q = w, w += p.q;

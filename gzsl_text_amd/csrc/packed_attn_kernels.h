@@ -166,7 +166,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     typedef typename K::frag frag;
     constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
     const int lt = blockIdx.x % a.nLT;
     const PaUnit un = pa_unit<G::ROWS>(a, blockIdx.x / a.nLT);
     if (un.ci >= un.all) return;
@@ -286,9 +286,9 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
 // Joins the chunks of a (note, label), in order.  G waves share a row's chunks (few rows over many chunks) and meet in LDS; a row
 // is 64 lanes over the widths.
 template <typename T, int ROWS, int G>
-__global__ __launch_bounds__(256) void pa_join_kernel(PaArgs a) {
-    __shared__ float so[4][256], ss[4], sM[4];
-    constexpr int R = 4 / G;  // rows of a workgroup
+__global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a) {
+    __shared__ float so[G][256], ss[G], sM[G];
+    constexpr int R = G == 1 ? 4 : 1;  // rows of a workgroup
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, part = w % G, nb = (a.L + R - 1) / R;
     const int l = blockIdx.x % nb * R + w / G;
     const PaUnit un = pa_unit<ROWS>(a, 0, blockIdx.x / nb);
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U, D = G::PL == 3 ? 2 : 4;
     constexpr bool DV = PART & 1, DK = PART & 2;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
     const PaTileUnit un = pa_tile_unit(a, blockIdx.x);
     if (un.b < 0) return;
     const int b = un.b, len = un.sp.len;
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     typedef typename K::frag frag;
     constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
     const int lt = blockIdx.x % a.nLT;
     const PaUnit un = pa_unit<G::ROWS>(a, blockIdx.x / a.nLT);
     if (un.ci >= un.all) return;
@@ -646,7 +646,7 @@ static int pa_fwd(PaArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     if (a.extra > 0) {
-        if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 4>), dim3(a.B * a.L), dim3(256), 0, st, a);
+        if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 16>), dim3(a.B * a.L), dim3(1024), 0, st, a);
         else hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 1>), dim3(a.B * cdiv(a.L, 4)), dim3(256), 0, st, a);
     }
     GZSL_CHECK_LAUNCH();
