@@ -249,7 +249,7 @@ struct PaArgs {
     float cap;
     uint32_t l_offset, L_total, seed, thresh;
     float scale;
-    int nLT, extra;                   // label workgroups of a note; token chunks beyond one a note (0: notes are not cut)
+    int nLT, extra, least;            // label workgroups of a note; token chunks beyond one a note (0: notes are not cut), their tokens at least
     int shares, slots;                // dK / dV: label shares of a token tile at most, slabs that the workspace has room for
     float slab;                       // time of a slab's write and read by the whole chip, in times of a tile on one compute unit
     // workspace
@@ -288,7 +288,7 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
         long long per = (n + a.extra - 1) / a.extra;
-        if (per < 256) per = 256;  // a share that pays for its own start and its part in the join
+        if (per < a.least) per = a.least;
         chunk = (int)min(per / ROWS * ROWS + ROWS, (long long)0x7FFFFFC0);
     }
     chunk = pa_scalar(chunk);
@@ -384,7 +384,7 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
 }
 
 struct PaPlan {
-    int nT, nQ, kind, waves, extra, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
+    int nT, nQ, kind, waves, extra, least, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
     float slab;
     long long units;  // workgroups of the dK / dV sweep
     long long kv, q, dO, part, ml, dq, dkv, bytes;

@@ -24,11 +24,13 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     else pa_sizes<PaGeo<PaF32, 13, 13>>(p, *d, backward);
     // 128 labels a workgroup (64: PaF32's forward, and bf16 where 128 leave fewer workgroups than the chip has places, two a compute
     // unit); notes are cut where the (note, label) workgroups alone would leave compute units without one.
-    p.waves = (p.kind == 3 && !backward) || (p.kind < 2 && (long long)d->B * cdiv(d->L, 128) < 512) ? 4 : 8;
+    const bool fits = !backward && d->L <= 128;  // one workgroup a note: it works from the rows themselves
+    p.waves = !fits && ((p.kind == 3 && !backward) || (p.kind < 2 && (long long)d->B * cdiv(d->L, 128) < 512)) ? 4 : 8;
     p.nLT = cdiv(d->L, 16 * p.waves);
     const long long wgs = (long long)d->B * p.nLT;
-    p.extra = wgs > 0 && wgs < 256 && d->max_len > 256 ? cdiv(p.waves == 4 ? 512 : 256, p.nLT) : 0;
-    if (p.extra > d->B * (d->max_len / 256 + 1)) p.extra = d->B * (d->max_len / 256 + 1);
+    p.least = fits ? 128 : 256;  // tokens of a chunk that pay for its own start and its part in the join
+    p.extra = wgs > 0 && wgs < 256 && d->max_len > p.least ? cdiv(p.waves == 4 ? 512 : 256, p.nLT) : 0;
+    if (p.extra > d->B * (d->max_len / p.least + 1)) p.extra = d->B * (d->max_len / p.least + 1);
     const long long chunks = d->B + p.extra;
     if ((long long)d->B * p.nT + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
         return GZSL_ETOOBIG;
@@ -58,7 +60,7 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.rows = d.rows, a.ldk = d.ldk, a.ldv = d.ldv, a.ldq = d.ldq;
     a.B = d.B, a.max_len = d.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
-    a.nLT = p.nLT, a.extra = p.extra, a.shares = p.shares, a.slots = p.slots, a.slab = p.slab;
+    a.nLT = p.nLT, a.extra = p.extra, a.least = p.least, a.shares = p.shares, a.slots = p.slots, a.slab = p.slab;
     char* w = (char*)work;
     a.TK = w, w += p.kv;
     a.Q = w, w += p.q;

@@ -4,6 +4,31 @@
 #include <type_traits>
 #include "packed_attn.h"
 
+// The KF elements x of one lane -> its 16 bytes of a fragment (of each plane).
+template <class K, class G>
+__device__ __forceinline__ typename K::frag pa_cut(const typename K::T (&x)[G::KF]) {
+    if constexpr (K::PL == 1) {
+        return __builtin_bit_cast(typename K::frag, x);
+    } else {
+        PaPieces f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            bf16 h, m, l;
+            pa_split(x[j], h, m, l);
+            f.p[0][j] = h, f.p[1][j] = m, f.p[2][j] = l;
+        }
+        return f;
+    }
+}
+template <class K, int COUNT>
+__device__ __forceinline__ void pa_put(char* img, int i, const typename K::frag& f, int lane) {
+    if constexpr (K::PL == 1) {
+        *reinterpret_cast<typename K::frag*>(img + i * 1024 + lane * 16) = f;
+    } else {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(img + (p * COUNT + i) * 1024 + lane * 16) = f.p[p];
+    }
+}
 // ------------------------------------------------------------------------------------------------------------- pre-pass
 // A tile's rows into LDS, zeros past nrows and past W (row stride P elements).
 template <typename T, int ROWS, int P>
@@ -29,32 +54,28 @@ __device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld,
 // Row (ROW) or column fragments of the staged tile: N of them (a plane), written 1 KB a wave.
 template <class K, class G, int N, int STEPS, bool ROW, int P>
 __device__ __forceinline__ void pa_emit(typename K::T (*sh)[P], char* img, int tid) {
-    typedef typename K::M M;
+    typedef typename K::T T;
     const int lane = tid & 63, n = lane & 15, g = lane >> 4;
-    for (int i = tid >> 6; i < N; i += 4) {
-        typename K::T x[G::KF];
 #pragma unroll
-        for (int j = 0; j < G::KF; ++j) {
-            if (ROW) x[j] = sh[16 * (i / STEPS) + n][i % STEPS * G::KK + g * G::KF + j];
-            else x[j] = sh[16 * (j >> 2) + 4 * g + (j & 3)][16 * i + n];
-        }
-        char* at = img + i * 1024 + lane * 16;
-        if constexpr (K::PL == 1) {
-            M v[G::KF];
+    for (int q0 = 0; q0 < N; q0 += 4) {
+        const int i = q0 + (tid >> 6);
+        if (i >= N) break;
+        T x[G::KF];
+        if (ROW) {
+            constexpr int V = 16 / (int)sizeof(T);
+            typedef T vec __attribute__((ext_vector_type(V)));
+            const T* row = &sh[16 * (i / STEPS) + n][i % STEPS * G::KK + g * G::KF];
 #pragma unroll
-            for (int j = 0; j < G::KF; ++j) v[j] = x[j];
-            *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, v);
-        } else {
-            bf16x8 p[3];
+            for (int j = 0; j < G::KF; j += V) {
+                const vec v = *reinterpret_cast<const vec*>(row + j);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                bf16 h, m, l;
-                pa_split(x[j], h, m, l);
-                p[0][j] = h, p[1][j] = m, p[2][j] = l;
+                for (int k = 0; k < V; ++k) x[j + k] = v[k];
             }
+        } else {
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(at + q * N * 1024) = p[q];
+            for (int j = 0; j < G::KF; ++j) x[j] = sh[16 * (j >> 2) + 4 * g + (j & 3)][16 * i + n];
         }
+        pa_put<K, N>(img, i, pa_cut<K, G>(x), lane);
     }
 }
 // Blocks [0, B nT): a token tile (keys, values); then nQ blocks of queries.
@@ -159,14 +180,120 @@ __device__ __forceinline__ void pa_out(const f32x4& v, T* row, bf16* low, int c,
 }
 
 // -------------------------------------------------------------------------------------------------------------- forward
-// Workgroup = WAVES x 16 labels of one note (or of one chunk of it); labels on the lane axis.
-template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
-__global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
-    typedef typename K::T T;
+// One wave's 16 labels (on the lane axis) against one token tile.
+template <class K, class G>
+struct PaFwdState {
+    typename K::frag qf[G::SE];
+    f32x4 acc[G::NF];
+    float m, sum;
+    uint32_t key;
+    bool fixed;
+};
+template <class K, class G>
+__device__ __forceinline__ void pa_fwd_begin(PaFwdState<K, G>& w, const PaArgs& a, bool cap, int b, int l) {
+#pragma unroll
+    for (int j = 0; j < G::NF; ++j) w.acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w.key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + (uint32_t)l);
+    // Scores capped at 30 lie within 2^+-44: their exponentials and sums are plain fp32 numbers without a maximum taken off, and
+    // nothing is ever rescaled.  Otherwise a tile whose maximum exceeds the running one by more than 2^12 moves it.
+    w.fixed = cap && a.cap <= 30.f;
+    w.m = w.fixed ? 0.f : -INFINITY, w.sum = 0.f;
+}
+// KR: row fragments of the keys, VC: column fragments of the values; t0: the tile's first token, LAST: it may end behind the note (left
+// tokens are the note's).
+template <class K, class G, bool CAP, bool DROP, bool LAST>
+__device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left, int lane) {
     typedef typename K::frag frag;
     constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
+    const int g = lane >> 4;
+    f32x4 s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    frag ring[D];
+    auto ldk = [&](int i) { return pa_frag<K, G::RE>(KR, i % U * G::SE + i / U, lane); };
+    auto ldv = [&](int j) { return pa_frag<K, G::NF>(VC, j, lane); };
+    pa_fill_ring<G::RE>(ring, ldk);
+    pa_run_ring<G::RE>(ring, ldk, [&](int i, const frag& f) { s[i % U] = pa_mma(f, w.qf[i / U], s[i % U]); });
+    pa_fill_ring<G::NF>(ring, ldv);  // under way during the softmax
+    float y[U][4], th[U][4];
+    pa_scores<K, CAP, U, false>(s, cap, y, th);
+    if (LAST) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (16 * u + 4 * g + r >= left) y[u][r] = -INFINITY;
+    }
+    if (!w.fixed) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
+        if (__any(mt > w.m + 12.f)) {  // m is the same in the four lanes of a column
+            mt = fmaxf(mt, __shfl_xor(mt, 16));
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float mn = fmaxf(w.m, mt), alpha = mn == w.m ? 1.f : __builtin_amdgcn_exp2f(w.m - mn);
+#pragma unroll
+            for (int j = 0; j < G::NF; ++j) w.acc[j] *= alpha;
+            w.sum *= alpha;
+            w.m = mn;
+        }
+        const float mi = w.m == -INFINITY ? 0.f : w.m;  // (no finite score yet: every weight is 2^-inf = 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[u][r] -= mi;
+    }
+    frag pf;
+    {
+        float p[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[u][r] = __builtin_amdgcn_exp2f(y[u][r]);
+                w.sum += p[u][r];
+                if (DROP) p[u][r] = gz_u32(w.key, (uint32_t)(t0 + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
+            }
+        pa_pack(p, pf);
+    }
+    pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) { w.acc[j] = pa_mma(f, pf, w.acc[j]); });
+}
+// Output rows, or a chunk's part of them.
+template <class K, class G>
+__device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a, const PaUnit& un, int l, int lane) {
+    typedef typename K::T T;
+    const int g = lane >> 4;
+    float sum = w.sum;
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (l >= a.L) return;
+    const long long row = (long long)un.b * a.L + l;
+    if (un.nch > 1) {
+        const long long pr = (long long)un.ci * a.L + l;
+        if (g == 0) a.ml[2 * pr] = w.m, a.ml[2 * pr + 1] = sum;
+#pragma unroll
+        for (int j = 0; j < G::NF; ++j) pa_out<float>(w.acc[j], a.part + pr * a.F, nullptr, 16 * j + 4 * g, a.F);
+        return;
+    }
+    const bool some = un.sp.len > 0;
+    const float inv = some ? 1.f / sum : 0.f;
+    if (g == 0) {
+        a.LSE[row] = some ? (w.m + __builtin_amdgcn_logf(sum)) * PA_LN2 : -INFINITY;
+        if (a.rest) a.rest[2 * row] = w.m, a.rest[2 * row + 1] = inv;
+    }
+    T* out = (T*)a.O + row * a.F;
+    bf16* low = sizeof(T) == 2 && a.rest ? reinterpret_cast<bf16*>(a.rest + 2LL * a.B * a.L) + row * a.F : nullptr;
+#pragma unroll
+    for (int j = 0; j < G::NF; ++j) pa_out<T>(w.acc[j] * inv, out, low, 16 * j + 4 * g, a.F);
+}
+
+// Workgroup = WAVES x 16 labels of one note (or of one chunk of it), token tiles from the pre-pass's images.
+template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
+__global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15;
     const int lt = blockIdx.x % a.nLT;
     const PaUnit un = pa_unit<G::ROWS>(a, blockIdx.x / a.nLT);
     if (un.ci >= un.all) return;
@@ -175,113 +302,125 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     const int l0 = (lt * WAVES + wave) * 16;
     const bool idle = l0 >= a.L;  // (wave-uniform: copies and barriers only)
     const PaCap cap = pa_cap(a.cap);
-
-    frag qf[G::SE];
+    PaFwdState<K, G> w;
+    pa_fwd_begin(w, a, CAP, b, l0 + n);
     {
         const int c = min(l0, a.nQ * G::ROWS - 16);
         const char* img = a.Q + (long long)(c / G::ROWS) * G::PL * G::RE * 1024;
 #pragma unroll
-        for (int s = 0; s < G::SE; ++s) qf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
+        for (int s = 0; s < G::SE; ++s) w.qf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
     }
-    const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + (uint32_t)(l0 + n));
-    f32x4 acc[G::NF];
-#pragma unroll
-    for (int j = 0; j < G::NF; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // Scores capped at 30 lie within 2^+-44: their exponentials and sums are plain fp32 numbers without a maximum taken off, and
-    // nothing is ever rescaled.  Otherwise a tile whose maximum exceeds the running one by more than 2^12 moves it.
-    const bool fixed = CAP && a.cap <= 30.f;
-    float m = fixed ? 0.f : -INFINITY, sum = 0.f;
     const char* tk = a.TK + (long long)b * a.nT * G::FWD * 1024;
     if (t0 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)t0 * G::FWD * 1024, sm, wave, lane);
     pa_arrive();
-    auto step = [&](int t, auto last) {  // last: the tile may end behind the note
+    auto step = [&](int t, auto last) {
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
-        const char* VC = KR + G::PL * G::RE * 1024;
         if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)(t + 1) * G::FWD * 1024, sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
-        if (!idle) {
-            f32x4 s[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            frag ring[D];
-            auto ldk = [&](int i) { return pa_frag<K, G::RE>(KR, i % U * G::SE + i / U, lane); };
-            auto ldv = [&](int j) { return pa_frag<K, G::NF>(VC, j, lane); };
-            pa_fill_ring<G::RE>(ring, ldk);
-            pa_run_ring<G::RE>(ring, ldk, [&](int i, const frag& f) { s[i % U] = pa_mma(f, qf[i / U], s[i % U]); });
-            pa_fill_ring<G::NF>(ring, ldv);  // under way during the softmax
-            float y[U][4], th[U][4];
-            pa_scores<K, CAP, U, false>(s, cap, y, th);
-            if constexpr (decltype(last)::value) {
-                const int left = len - t * G::ROWS;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (16 * u + 4 * g + r >= left) y[u][r] = -INFINITY;
-            }
-            if (!fixed) {
-                float mt = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
-                if (__any(mt > m + 12.f)) {  // m is the same in the four lanes of a column
-                    mt = fmaxf(mt, __shfl_xor(mt, 16));
-                    mt = fmaxf(mt, __shfl_xor(mt, 32));
-                    const float mn = fmaxf(m, mt), alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-                    for (int j = 0; j < G::NF; ++j) acc[j] *= alpha;
-                    sum *= alpha;
-                    m = mn;
-                }
-                const float mi = m == -INFINITY ? 0.f : m;  // (no finite score yet: every weight is 2^-inf = 0)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) y[u][r] -= mi;
-            }
-            frag pf;
-            {
-                float p[U][4];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[u][r] = __builtin_amdgcn_exp2f(y[u][r]);
-                        sum += p[u][r];
-                        if (DROP) p[u][r] = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
-                    }
-                pa_pack(p, pf);
-            }
-            pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) { acc[j] = pa_mma(f, pf, acc[j]); });
-        }
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         pa_arrive();
     };
     for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
     if (t0 < t1) step(t1 - 1, std::true_type{});
-    const int l = l0 + n;
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (l >= a.L) return;
-    const long long row = (long long)b * a.L + l;
-    if (un.nch > 1) {
-        const long long pr = (long long)un.ci * a.L + l;
-        if (g == 0) a.ml[2 * pr] = m, a.ml[2 * pr + 1] = sum;
+    pa_fwd_end(w, a, un, l0 + n, lane);
+}
+
+// KF consecutive elements of a row from e0 (clamped address, no branch around a load).  wide: 16-byte loads are allowed.
+template <class G, typename T>
+__device__ __forceinline__ void pa_row_load(const T* row, int e0, int W, bool wide, T (&x)[G::KF]) {
+    constexpr int V = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(V)));
+    if (wide) {
 #pragma unroll
-        for (int j = 0; j < G::NF; ++j)
+        for (int j = 0; j < G::KF; j += V) {
+            const vec v = *reinterpret_cast<const vec*>(row + min(e0 + j, W - V));
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (16 * j + 4 * g + r < a.F) a.part[pr * a.F + 16 * j + 4 * g + r] = acc[j][r];
-        return;
+            for (int k = 0; k < V; ++k) x[j + k] = v[k];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < G::KF; ++j) x[j] = row[min(e0 + j, W - 1)];
     }
-    const float inv = len > 0 ? 1.f / sum : 0.f;
-    if (g == 0) {
-        a.LSE[row] = len > 0 ? (m + __builtin_amdgcn_logf(sum)) * PA_LN2 : -INFINITY;
-        if (a.rest) a.rest[2 * row] = m, a.rest[2 * row + 1] = inv;
-    }
-    T* out = (T*)a.O + row * a.F;
-    bf16* low = sizeof(T) == 2 && a.rest ? reinterpret_cast<bf16*>(a.rest + 2LL * a.B * a.L) + row * a.F : nullptr;
+}
+
+// The same for at most WAVES x 16 labels (one label workgroup a note or chunk): every token tile is then read by one workgroup
+// alone, which cuts its fragments itself: each wave loads the elements of its share of the next tile's fragments while it works on the
+// current one.  No images and one launch less.
+template <class K, class G, int WAVES, bool CAP, bool DROP>
+__global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) {
+    typedef typename K::T T;
+    constexpr int V = 16 / (int)sizeof(T), NR = (G::RE + WAVES - 1) / WAVES, NC = (G::NF + WAVES - 1) / WAVES;  // fragments of a wave
+    extern __shared__ __attribute__((aligned(16))) char sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
+    const PaUnit un = pa_unit<G::ROWS>(a, blockIdx.x);
+    if (un.ci >= un.all) return;
+    const int b = un.b, len = un.sp.len;
+    const int t0 = un.c * (un.chunk / G::ROWS), t1 = (int)min((long long)(len + G::ROWS - 1) / G::ROWS, (long long)t0 + un.chunk / G::ROWS);
+    const int l0 = wave * 16;
+    const bool idle = l0 >= a.L;
+    const PaCap cap = pa_cap(a.cap);
+    const T *kp = (const T*)a.keys + un.sp.start * a.ldk, *vp = (const T*)a.values + un.sp.start * a.ldv;
+    const bool kwide = a.E % V == 0 && a.ldk % V == 0 && ((uintptr_t)kp & 15) == 0;
+    T xk[NR][G::KF], xv[NC][G::KF];
+    auto load = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < G::NF; ++j) pa_out<T>(acc[j] * inv, out, low, 16 * j + 4 * g, a.F);
+        for (int q = 0; q < NR; ++q) {
+            const int i = min(wave + q * WAVES, G::RE - 1), row = min(t * G::ROWS + 16 * (i / G::SE) + n, len - 1);
+            pa_row_load<G>(kp + row * a.ldk, i % G::SE * G::KK + g * G::KF, a.E, kwide, xk[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const int c = min(16 * min(wave + q * WAVES, G::NF - 1) + n, a.F - 1);
+#pragma unroll
+            for (int j = 0; j < G::KF; ++j) xv[q][j] = vp[min(t * G::ROWS + 16 * (j >> 2) + 4 * g + (j & 3), len - 1) * a.ldv + c];
+        }
+    };
+    // zeros past the note's end and past E / F
+    auto store = [&](int t, char* buf) {
+#pragma unroll
+        for (int q = 0; q < NR; ++q) {
+            const int i = wave + q * WAVES, e0 = i % G::SE * G::KK + g * G::KF;
+            if (i >= G::RE) break;
+            const bool in = t * G::ROWS + 16 * (i / G::SE) + n < len;
+#pragma unroll
+            for (int j = 0; j < G::KF; ++j) xk[q][j] = in && e0 + j < a.E ? xk[q][j] : (T)0.f;
+            pa_put<K, G::RE>(buf, i, pa_cut<K, G>(xk[q]), lane);
+        }
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+            const int i = wave + q * WAVES;
+            if (i >= G::NF) break;
+#pragma unroll
+            for (int j = 0; j < G::KF; ++j) xv[q][j] = t * G::ROWS + 16 * (j >> 2) + 4 * g + (j & 3) < len && 16 * i + n < a.F ? xv[q][j] : (T)0.f;
+            pa_put<K, G::NF>(buf + G::PL * G::RE * 1024, i, pa_cut<K, G>(xv[q]), lane);
+        }
+    };
+    if (t0 < t1) load(t0);
+    PaFwdState<K, G> w;
+    pa_fwd_begin(w, a, CAP, b, l0 + n);
+    {
+        const T* row = (const T*)a.queries + (long long)min(l0 + n, a.L - 1) * a.ldq;
+        const bool qwide = a.E % V == 0 && a.ldq % V == 0 && ((uintptr_t)a.queries & 15) == 0;
+#pragma unroll
+        for (int s = 0; s < G::SE; ++s) {
+            const int e0 = s * G::KK + g * G::KF;
+            T x[G::KF];
+            pa_row_load<G>(row, e0, a.E, qwide, x);
+#pragma unroll
+            for (int j = 0; j < G::KF; ++j) x[j] = l0 + n < a.L && e0 + j < a.E ? x[j] : (T)0.f;
+            w.qf[s] = pa_cut<K, G>(x);
+        }
+    }
+    if (t0 < t1) store(t0, sm);
+    if (t0 + 1 < t1) load(t0 + 1);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {  // (the masked form for every tile: one copy of the code, whose first run is part of a short call)
+        const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, true>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
+        if (t + 1 < t1) store(t + 1, sm + ((t - t0 + 1) & 1) * G::FWD * 1024);
+        if (t + 2 < t1) load(t + 2);
+        __syncthreads();
+    }
+    pa_fwd_end(w, a, un, l0 + n, lane);
 }
 // Joins the chunks of a (note, label), in order.  G waves share a row's chunks (few rows over many chunks) and meet in LDS; a row
 // is 64 lanes over the widths.
@@ -643,8 +782,13 @@ __global__ __launch_bounds__(256) void pa_q_join_kernel(PaArgs a) {
 template <class K, class G, int W, int OCC, bool CAP, bool DROP>
 static int pa_fwd(PaArgs& a, hipStream_t st) {
     typedef typename K::T T;
-    hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+    if constexpr (W == 8) if (a.nLT == 1) {
+        hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+    }
+    if (W != 8 || a.nLT > 1) {
+        hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+    }
     if (a.extra > 0) {
         if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 16>), dim3(a.B * a.L), dim3(1024), 0, st, a);
         else hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 1>), dim3(a.B * cdiv(a.L, 4)), dim3(256), 0, st, a);
