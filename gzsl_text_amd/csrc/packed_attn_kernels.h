@@ -422,68 +422,76 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) 
     }
     pa_fwd_end(w, a, un, l0 + n, lane);
 }
-// Joins the chunks of a (note, label), in order.  G waves share a row's chunks (few rows over many chunks) and meet in LDS; a row
-// is 64 lanes over the widths.
+// Joins the chunks of a (note, label), in order: a workgroup of 4 rows of one wave each, or (G > 1, few rows over many chunks) of one
+// row whose chunks G waves share and join in LDS.  A lane weighs one chunk; a row's F values lie over the lanes.
 template <typename T, int ROWS, int G>
 __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a) {
-    __shared__ float so[G][256], ss[G], sM[G];
-    constexpr int R = G == 1 ? 4 : 1;  // rows of a workgroup
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, part = w % G, nb = (a.L + R - 1) / R;
+    __shared__ float so[G == 1 ? 4 : G][256], ss[G == 1 ? 4 : G], sM[G];
+    constexpr int R = G == 1 ? 4 : 1;
+    const int lane = threadIdx.x & 63, w = pa_scalar((int)threadIdx.x >> 6), part = w % G, nb = (a.L + R - 1) / R;
     const int l = blockIdx.x % nb * R + w / G;
     const PaUnit un = pa_unit<ROWS>(a, 0, blockIdx.x / nb);
     if (un.nch == 1) return;
-    const bool on = l < a.L;
+    const bool on = l < a.L, vec = a.F % 4 == 0;
     const int per = (un.nch + G - 1) / G, c0 = on ? part * per : 0, c1 = on ? min(un.nch, c0 + per) : 0;
+    const float* ml = a.ml + 2 * ((long long)un.ci * a.L + l);
+    const float* pr = a.part + ((long long)un.ci * a.L + l) * a.F;
     float M = -INFINITY;
-    for (int c = c0 + lane; c < c1; c += 64) {
-        const float* ml = a.ml + 2 * ((long long)(un.ci + c) * a.L + l);
-        if (ml[1] != 0.f) M = fmaxf(M, ml[0]);  // (no finite score in this chunk: sum 0)
-    }
+    for (int c = c0 + lane; c < c1; c += 64)
+        if (ml[2LL * c * a.L + 1] != 0.f) M = fmaxf(M, ml[2LL * c * a.L]);  // (no finite score in this chunk: sum 0)
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
     if (G > 1) {
-        if (lane == 0) sM[w] = M;
+        if (lane == 0) sM[part] = M;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < G; ++k) M = fmaxf(M, sM[w - part + k]);
+        for (int k = 0; k < G; ++k) M = fmaxf(M, sM[k]);
     }
-    float sum = 0.f, o4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int c = c0; c < c1; ++c) {
-        const long long pr = (long long)(un.ci + c) * a.L + l;
-        const float s = a.ml[2 * pr + 1], f = s != 0.f ? __builtin_amdgcn_exp2f(a.ml[2 * pr] - M) : 0.f;
+    float sum = 0.f;
+    f32x4 o4 = f32x4{0.f, 0.f, 0.f, 0.f};  // values 4 lane .. + 3 (vec), else lane + 64 k
+    for (int b0 = c0; b0 < c1; b0 += 64) {
+        const int c = min(b0 + lane, c1 - 1);
+        const float s = b0 + lane < c1 ? ml[2LL * c * a.L + 1] : 0.f, f = s != 0.f ? __builtin_amdgcn_exp2f(ml[2LL * c * a.L] - M) : 0.f;
         sum = fmaf(f, s, sum);
+        const int n = min(64, c1 - b0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float fi = __shfl(f, i);
+            const float* x = pr + (long long)(b0 + i) * a.L * a.F;
+            f32x4 v;
+            if (vec) {
+                v = *reinterpret_cast<const f32x4*>(x + min(4 * lane, a.F - 4));
+            } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float x = lane + 64 * k < a.F ? a.part[pr * a.F + lane + 64 * k] : 0.f;
-            o4[k] = f != 0.f ? fmaf(f, x, o4[k]) : o4[k];
+                for (int k = 0; k < 4; ++k) v[k] = x[min(lane + 64 * k, a.F - 1)];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o4[k] = fi != 0.f ? fmaf(fi, v[k], o4[k]) : o4[k];
         }
     }
-    if (G > 1) {
+    sum = wave_sum(sum);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) so[w][lane + 64 * k] = o4[k];
-        if (lane == 0) ss[w] = sum;
-        __syncthreads();
-        if (part > 0) return;
-        for (int q = 1; q < G; ++q) {
-            sum += ss[w + q];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o4[k] += so[w + q][lane + 64 * k];
-        }
-    }
-    if (!on) return;
+    for (int k = 0; k < 4; ++k) so[w][vec ? 4 * lane + k : lane + 64 * k] = o4[k];
+    if (lane == 0) ss[w] = sum;
+    __syncthreads();
+    // one thread a value from here on
     const long long row = (long long)un.b * a.L + l;
+    bf16* low = sizeof(T) == 2 && a.rest ? reinterpret_cast<bf16*>(a.rest + 2LL * a.B * a.L) + row * a.F : nullptr;
+    const int f0 = G == 1 ? lane : threadIdx.x, step = G == 1 ? 64 : 64 * G, w0 = G == 1 ? w : 0;
+    if (!on) return;
+    sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < G; ++q) sum += ss[w0 + q];
     const float inv = 1.f / sum;
-    if (lane == 0) {
+    if (f0 == 0) {
         a.LSE[row] = (M + __builtin_amdgcn_logf(sum)) * PA_LN2;
         if (a.rest) a.rest[2 * row] = M, a.rest[2 * row + 1] = inv;
     }
-    bf16* low = sizeof(T) == 2 && a.rest ? reinterpret_cast<bf16*>(a.rest + 2LL * a.B * a.L) + row * a.F : nullptr;
+    for (int f = f0; f < a.F; f += step) {
+        float o = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int f = lane + 64 * k;
-        if (f >= a.F) continue;
-        const float o = o4[k] * inv;
+        for (int q = 0; q < G; ++q) o += so[w0 + q][f];
+        o *= inv;
         const T r = (T)o;
         ((T*)a.O)[row * a.F + f] = r;
         if (low) low[f] = (bf16)(o - (float)r);
