@@ -6,7 +6,8 @@
 // Both directions are the recurrence x <- A x + B, whose steps join: (A1, B1) then (A2, B2) = (A2 A1, A2 B1 + B2).  The time axis is
 // cut into chunks, one workgroup each (a thread owns V channels and S consecutive steps of a tile, all in registers):
 //   1. gs_chunk_kernel reduces every chunk to its (A, B)         reads g and c (g and dh)
-//   2. gs_apply_kernel joins the pairs of the chunks before its own into the state it starts from, then runs through its tiles:
+//   2. gs_join_kernel, where there are many chunks, joins the pairs to the state in front of each
+//   3. gs_apply_kernel takes that state (or joins the pairs of the chunks before its own itself), then runs through its tiles:
 //      each thread's steps to a pair, a scan of the pairs over the tile's threads in LDS, the steps again from the state in front.
 // Memory-bound: 3 (6) tensors forward (backward), of which the first pass reads two once more (from the 256 MB last-level cache
 // where they fit).  The pairs meet in a fixed order, so results repeat bit for bit; tokens in front of a step never see it.
@@ -14,6 +15,8 @@
 #include "../../include/gzsl_hip.h"
 
 #define GS_THREADS 256
+#define GS_JTHREADS 512
+#define GS_JGROUPS 4
 #define GS_LOG2E 1.4426950408889634f
 
 struct GsArgs {
@@ -29,6 +32,7 @@ struct GsArgs {
     void *dg, *dc;
     float* dh0;
     float* pair;                             // [B][nch][2][H]
+    int joined;
     int ncg, nblk, TS, tiles, chunk, nch;    // channel groups of a workgroup, workgroups over the channels, threads over time, tiles of a chunk
 };
 
@@ -174,6 +178,49 @@ __global__ __launch_bounds__(GS_THREADS) void gs_chunk_kernel(GsArgs a) {
     }
 }
 
+// The state in front of each chunk of a note, in place of its pair's A.  A workgroup takes GS_JGROUPS vectors of channels, its threads
+// share out the chunks; latency-bound (512 chunks x 256 channels: 7 us; 256 or 1024 threads 9).
+template <int V>
+__global__ __launch_bounds__(GS_JTHREADS) void gs_join_kernel(GsArgs a, const float* init) {
+    extern __shared__ float sh[];
+    const int tid = threadIdx.x, cg = tid % GS_JGROUPS, j = tid / GS_JGROUPS, TS = GS_JTHREADS / GS_JGROUPS, b = blockIdx.x;
+    int ch = (blockIdx.y * GS_JGROUPS + cg) * V;
+    const bool on = ch < a.H;
+    if (!on) ch = 0;
+    const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
+    const int n = (int)(((long long)sp.len + a.chunk - 1) / a.chunk);  // chunks of this note; the last one's pair is not there and not needed
+    const int per = (n + TS - 1) / TS, q0 = min(n, j * per), q1 = min(n, q0 + per);
+    float* pr = a.pair + (long long)b * a.nch * 2 * a.H + ch;
+    float A[V], B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll 8
+    for (int q = q0; q < min(q1, n - 1); ++q) {
+        float ka[V], kb[V];
+        gs_load<float, V>(pr + (long long)q * 2 * a.H, ka);
+        gs_load<float, V>(pr + (long long)q * 2 * a.H + a.H, kb);
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = fmaf(ka[v], B[v], kb[v]), A[v] *= ka[v];
+    }
+    float Ae[V], Be[V], At[V], Bt[V], x[V];
+    gs_scan<V>(A, B, Ae, Be, At, Bt, sh, tid, j, TS, GS_JGROUPS, GS_JTHREADS);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = fmaf(Ae[v], init ? init[(long long)b * a.H + ch + v] : 0.f, Be[v]);
+    if (!on) return;
+#pragma unroll 8
+    for (int q = q0; q < q1; ++q) {
+        float ka[V], kb[V];
+        if (q < n - 1) {
+            gs_load<float, V>(pr + (long long)q * 2 * a.H, ka);
+            gs_load<float, V>(pr + (long long)q * 2 * a.H + a.H, kb);
+        }
+        gs_store<float, V>(pr + (long long)q * 2 * a.H, x);
+        if (q < n - 1)
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = fmaf(ka[v], x[v], kb[v]);
+    }
+}
+
 template <typename T, int V, int S, bool BWD>
 __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
     extern __shared__ float sh[];
@@ -207,14 +254,16 @@ __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
 #pragma unroll
     for (int v = 0; v < V; ++v) x[v] = init ? init[at + v] : 0.f;
     float Ae[V], Be[V], At[V], Bt[V];
-    if (p.k > 0) {
+    if (p.k > 0 && a.joined) {
+        gs_load<float, V>(a.pair + ((long long)p.b * a.nch + p.k) * 2 * a.H + p.ch, x);
+    } else if (p.k > 0) {
         // the pairs of the chunks in front, shared out over the threads along time
         const int per = (p.k + a.TS - 1) / a.TS, q0 = p.j * per, q1 = min(p.k, q0 + per);
         const float* pr = a.pair + (long long)p.b * a.nch * 2 * a.H + p.ch;
         float A[V], B[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int q = q0; q < q1; ++q) {
             float ka[V], kb[V];
             gs_load<float, V>(pr + (long long)q * 2 * a.H, ka);
@@ -327,7 +376,7 @@ __global__ __launch_bounds__(256) void gs_step_kernel(const T* g, const T* c, fl
 static int gs_check(const GzslGatedScan* d) {
     if (!d || d->B < 0 || d->rows < 0 || d->max_len < 0 || d->H < 1 || d->ldg < d->H || d->ldc < d->H) return GZSL_EINVAL;
     if (d->dtype != GZSL_F32 && d->dtype != GZSL_BF16) return GZSL_EINVAL;
-    if (d->B > 65534 || d->max_len > 0x7FF00000) return GZSL_ETOOBIG;  // (positions of a last, partial tile stay below 2^31)
+    if (d->B > 65534 || d->H > 65536 || d->max_len > 0x7FF00000) return GZSL_ETOOBIG;  // (positions of a last, partial tile stay below 2^31)
     if (d->B > 0 && !d->spans) return GZSL_EINVAL;
     if (d->rows > 0 && (!d->gates || !d->cands)) return GZSL_EINVAL;
     return 0;
@@ -354,14 +403,15 @@ static int gs_shape(GsArgs& a, int V) {
     a.nblk = (groups + a.ncg - 1) / a.ncg;
     a.TS = GS_THREADS / a.ncg;
     const long long tile = (long long)a.TS * gs_steps(V), all = (a.max_len + tile - 1) / tile, wgs = all * a.B * a.nblk;
-    // a chunk is one tile until that makes over 1024 workgroups (four to a compute unit) or over 256 chunks to look back at
+    // a chunk is one tile until that makes over 1024 workgroups, four to a compute unit (81600 x 256 bf16: first pass and third 22 + 38 us
+    // with half as many, 19 + 26 so, 18 + 28 with twice as many)
     long long m = wgs / 1024;
-    if (m < (all + 255) / 256) m = (all + 255) / 256;
+    if (m > all) m = all;
     if (m < 1) m = 1;
     a.tiles = (int)m, a.chunk = (int)(m * tile);
-    a.nch = (int)((a.max_len + a.chunk - 1) / a.chunk);
+    a.nch = (int)(((long long)a.max_len + a.chunk - 1) / a.chunk);
     if (a.nch < 1) a.nch = 1;
-    return (long long)a.nch * a.B > 0x7FFFFFFF || a.nblk > 65535 ? GZSL_ETOOBIG : 0;
+    return (long long)a.nch * a.B > 0x7FFFFFFF ? GZSL_ETOOBIG : 0;
 }
 
 template <typename T, int V, bool BWD>
@@ -373,6 +423,14 @@ static int gs_go(GsArgs& a, void* work, long long work_bytes, hipStream_t st) {
     const dim3 grid(a.nch * a.B, a.nblk), block(a.ncg * a.TS);
     const size_t lds = sizeof(float) * 2 * V * block.x;
     if (a.nch > 1) hipLaunchKernelGGL((gs_chunk_kernel<T, V, S, BWD>), grid, block, lds, st, a);
+    // Up to 64 chunks every workgroup joins the pairs in front of its own by itself (18388 x 200 fp32 in 40 chunks: a kernel for it would
+    // take 6 us and save 1 to 3); of more, each would read more pairs than rows (512 chunks of 128 steps: 52 us against 26 + 7).
+    a.joined = a.nch > 64;
+    if (a.joined) {
+        constexpr int JV = V >= 4 ? 4 : 1;
+        const float* init = BWD ? a.dlast : a.h0;
+        hipLaunchKernelGGL((gs_join_kernel<JV>), dim3(a.B, (a.H + JV * GS_JGROUPS - 1) / (JV * GS_JGROUPS)), dim3(GS_JTHREADS), sizeof(float) * 2 * JV * GS_JTHREADS, st, a, init);
+    }
     hipLaunchKernelGGL((gs_apply_kernel<T, V, S, BWD>), grid, block, lds, st, a);
     GZSL_CHECK_LAUNCH();
     return 0;

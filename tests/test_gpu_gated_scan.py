@@ -60,6 +60,17 @@ def test_forward_and_backward_against_64_bits(ops, lens, H, dtype, reverse):
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('lens,H,reverse', [([9000, 0, 2700, 1], 200, False), ([9001], 256, True), ([27001, 400], 5, False)])
+def test_notes_of_many_chunks(ops, lens, H, dtype, reverse):
+    g, c, spans, max_len, h0, dh, dl, sl = make(lens, H, dtype, seed=H, tail=3)
+    h, last = ops.gated_scan_fwd(g, c, spans, max_len, h0, reverse)
+    got = (h, last, *ops.gated_scan_bwd(dh, dl, h, g, c, spans, max_len, h0, reverse))
+    ref = scan_ref(g, c, sl, h0, reverse, dh, dl)
+    for name, x in zip(NAMES, got):
+        within(x, ref[name], name)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
 @pytest.mark.parametrize('garbage', [float('nan'), float('inf')])
 def test_padded_batch_leaves_its_padding_out(ops, dtype, garbage):
     g, c, spans, max_len, h0, dh, dl, sl = make([37, 0, 70, 1], 20, dtype, seed=3, pitch=75, tail=9, garbage=garbage)
