@@ -24,8 +24,9 @@
 // A pre-pass writes the operands as tile images made of such fragments (a tile: the rows of one k step of the second product, 32,
 // or 16 of PaF32), zero-filled past the note's end, past the last label and past E / F.  The sweeps copy images by LDS-DMA and read
 // them 16 bytes a lane at one address plus constants, free of bank conflicts without padding; odd widths, row pitches, alignment
-// and whatever lies between the notes (NaN included) end in the pre-pass.  PaX3's backward, for lack of LDS, takes its column
-// fragments out of the row fragments with ds_read_b64_tr_b16.
+// and whatever lies between the notes (NaN included) end in the pre-pass.  The backward
+// takes the column fragments of bf16 pieces out of the row fragments with ds_read_b64_tr_b16, PaX3 all of them for lack of LDS, PaBF
+// those of the keys (dQ 87 -> 78 us at 17404 tokens x 1999 labels of 200; of the labels' tiles it was no gain).
 #pragma once
 #include "packed.h"
 #include "rng.h"
@@ -63,11 +64,11 @@ struct PaGeo {
     static constexpr int NE = NE_, NF = NF_, PL = K::PL, SZ = sizeof(typename K::M), KF = 16 / SZ, KK = 4 * KF, ROWS = KK, U = ROWS / 16;
     static constexpr int SE = (NE * 16 + KK - 1) / KK, SF = (NF * 16 + KK - 1) / KK;  // k steps over e / f
     static constexpr int RE = U * SE, RF = U * SF;                                    // row fragments of a tile (one plane)
-    static constexpr bool TR = PL == 3;                                               // backward: columns by transposed reads
+    static constexpr bool TRT = SZ == 2, TRL = PL == 3;                               // backward, columns of token and label tiles: by transposed reads
     static constexpr int FWD = PL * (RE + NF);                                        // token tile, forward: keys by rows, values by columns
-    static constexpr int TOK = PL * (RE + RF) + (TR ? 0 : NE);                        // token tile, backward: keys, values by rows, keys by columns
-    static constexpr int QRY = PL * RE + (TR ? 0 : NE);                               // label tile: queries by rows (and columns)
-    static constexpr int OUT = PL * RF + (TR ? 0 : NF) + 1;                           // label tile: dO by rows (and columns), then off, scale, delta
+    static constexpr int TOK = PL * (RE + RF) + (TRT ? 0 : NE);                        // token tile, backward: keys, values by rows, keys by columns
+    static constexpr int QRY = PL * RE + (TRL ? 0 : NE);                               // label tile: queries by rows (and columns)
+    static constexpr int OUT = PL * RF + (TRL ? 0 : NF) + 1;                           // label tile: dO by rows (and columns), then off, scale, delta
 };
 
 __device__ __forceinline__ f32x4 pa_mma(f32x4 a, f32x4 b, f32x4 c) {
@@ -99,18 +100,18 @@ __device__ __forceinline__ typename K::frag pa_frag(const char* img, int i, int 
 }
 // Column fragment j out of the row fragments (SK k steps, U = 2) of a tile.  Row r, columns 16 j + 4 q .. + 3 lie in k step j / 2, lane
 // (16 (2 (j & 1) + q / 2) + r), bytes 8 (q & 1); the transposed read gives lane n of a 16-lane group column n of its 4 x 16 block.
-template <int SK>
-__device__ __forceinline__ PaPieces pa_col_tr(const char* img, int j, int n, int g) {
+template <class K, int SK>
+__device__ __forceinline__ typename K::frag pa_col_tr(const char* img, int j, int n, int g) {
     const int r = 4 * g + (n >> 2), q = n & 3;
     const char* at = img + (j >> 1) * 1024 + ((2 * (j & 1) + (q >> 1)) * 16 + r) * 16 + 8 * (q & 1);
-    PaPieces f;
+    bf16x8 f[K::PL];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
+    for (int p = 0; p < K::PL; ++p) {
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(at + p * 2 * SK * 1024));
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GZ_LDS s16x4*)(at + (p * 2 + 1) * SK * 1024));
-        f.p[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        f[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    return f;
+    return __builtin_bit_cast(typename K::frag, f);
 }
 // accumulator registers of the tile's score tiles -> operand fragment
 __device__ __forceinline__ void pa_pack(const float (&p)[1][4], f32x4& out) { out = f32x4{p[0][0], p[0][1], p[0][2], p[0][3]}; }
@@ -157,65 +158,58 @@ __device__ __forceinline__ void pa_fill_ring(F (&ring)[D], LD&& ld) {
 }
 
 struct PaCap {
-    float inv, k1, c2;  // 1 / cap, 2 log2(e) / cap, cap log2(e)
+    float inv, k1, c2, kt;  // 1 / cap, 2 log2(e) / cap, cap log2(e), 1 / (cap log2(e))
 };
 __device__ __forceinline__ PaCap pa_cap(float cap) {
-    return {cap > 0.f ? 1.f / cap : 0.f, cap > 0.f ? 2.f * PA_LOG2E / cap : 0.f, cap * PA_LOG2E};
+    const float inv = cap > 0.f ? 1.f / cap : 0.f;
+    return {inv, 2.f * PA_LOG2E * inv, cap * PA_LOG2E, PA_LN2 * inv};
 }
-// tanh u = 1 - 2 / (1 + e^{2u}): exact limits at +-inf, absolute error of a few 2^-24.  fp32 tensors take the odd series below
-// |u| = 0.35 (the next term is below 2^-26 of the value there), where the difference would lose relative accuracy that the
-// products of the gradient still have.  `far` (the same in the whole wave): some lane needs the exponential.
-__device__ __forceinline__ float pa_sech(float x, const PaCap& c) {  // 1 / (1 + e^{2 x / cap})
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1));
-}
-__device__ __forceinline__ float pa_series(float u) {
-    const float w = u * u;
-    return u * fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+__device__ __forceinline__ float pa_far(float x, const PaCap& c) {  // cap log2(e) tanh(x / cap) = cap log2(e) (1 - 2 / (1 + e^{2 x / cap}))
+    return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1)), -2.f * c.c2, c.c2);
 }
 #define PA_NEAR 0.35f
-// Scores x of a tile -> y in units of log 2 (and th = tanh(x / cap) for the gradient).
+// Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself
+// (pa_over takes it as it is).  bf16 tensors take the closed form: exact limits at +-inf, absolute error of a few 2^-24.  fp32 tensors
+// take the odd series below |x / cap| = 0.35 (the next term is below 2^-26 of the value), for the relative accuracy that the products
+// of the gradient still have, and the closed form only where a wave's tile holds a larger one.  (For bf16 the series is the longer way:
+// 148 us against 138 for 19309 tokens x 9000 labels.)
 template <class K, bool CAP, int U, bool TH>
 __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, float (&y)[U][4], float (&th)[U][4]) {
-    if (!CAP) {
+    constexpr bool SERIES = CAP && sizeof(typename K::T) == 4;
+    float most = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[u][r] = x[u][r] * PA_LOG2E;
-    } else if (sizeof(typename K::T) == 2) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float q = pa_sech(x[u][r], c);
-                y[u][r] = fmaf(q, -2.f * c.c2, c.c2);
-                if (TH) th[u][r] = fmaf(q, -2.f, 1.f);
+        for (int r = 0; r < 4; ++r) {
+            if (!CAP) {
+                y[u][r] = x[u][r];
+            } else if (!SERIES) {
+                y[u][r] = pa_far(x[u][r], c);
+            } else {
+                const float v = x[u][r] * c.inv, w = v * v;
+                most = fmaxf(most, fabsf(v));  // (a NaN passes it by and stays one in the series)
+                float t = fmaf(w, -1382.f / 155925.f * PA_LOG2E, 62.f / 2835.f * PA_LOG2E);
+                t = fmaf(w, fmaf(w, fmaf(w, fmaf(w, t, -17.f / 315.f * PA_LOG2E), 2.f / 15.f * PA_LOG2E), -1.f / 3.f * PA_LOG2E), PA_LOG2E);
+                y[u][r] = x[u][r] * t;
             }
-    } else {
-        bool near = true;
-        float t[U][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float v = x[u][r] * c.inv;
-                near = near && fabsf(v) < PA_NEAR;  // (false for a NaN)
-                t[u][r] = pa_series(v);
-            }
-        if (!__all(near)) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (!(fabsf(x[u][r] * c.inv) < PA_NEAR)) t[u][r] = fmaf(pa_sech(x[u][r], c), -2.f, 1.f);
         }
+    if (SERIES && __any(most >= PA_NEAR)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                y[u][r] = t[u][r] * c.c2;
-                if (TH) th[u][r] = t[u][r];
-            }
+            for (int r = 0; r < 4; ++r)
+                if (fabsf(x[u][r] * c.inv) >= PA_NEAR) y[u][r] = pa_far(x[u][r], c);
     }
+    if (CAP && TH)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) th[u][r] = y[u][r] * c.kt;
+}
+// 2^(y - off)
+template <bool CAP>
+__device__ __forceinline__ float pa_over(float y, float off) {
+    return __builtin_amdgcn_exp2f(CAP ? y - off : fmaf(y, PA_LOG2E, -off));
 }
 
 // Copies KB KB of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  `src` and `wave` are scalars.
@@ -235,9 +229,10 @@ __device__ __forceinline__ int pa_scalar(int x) { return __builtin_amdgcn_readfi
 __device__ __forceinline__ long long pa_scalar(long long x) {
     return (long long)(uint32_t)pa_scalar((int)x) | (long long)pa_scalar((int)(x >> 32)) << 32;
 }
-// this wave's copies have landed and every wave is past its reads of the other buffer
+// this wave's copies have landed, all but the newest LEFT of them, and every wave is past its reads of the other buffers
+template <int LEFT = 0>
 __device__ __forceinline__ void pa_arrive() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
     __syncthreads();
 }
 
@@ -280,11 +275,11 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
     u.ci = ci;
     u.b = -1;
     int chunk = 0x7FFFFFC0;
-    auto length = [&](int b) { return b < a.B ? note_span(a.spans, b, a.rows, a.max_len).len : 0; };
-    int len = length(lane);
+    auto span = [&](int b) { return b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0}; };
+    NoteSpan sp = span(lane);
     if (a.extra > 0) {
-        long long n = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) n += b0 ? length(b0 + lane) : len;
+        long long n = sp.len;
+        for (int b0 = 64; b0 < a.B; b0 += 64) n += span(b0 + lane).len;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
         long long per = (n + a.extra - 1) / a.extra;
@@ -295,8 +290,8 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
     u.chunk = chunk;
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        int note = b0 + lane;
-        if (b0) len = length(note);
+        if (b0) sp = span(b0 + lane);
+        int note = b0 + lane, len = sp.len;
         if (a.B <= 64) {  // order by length, longest first (ties: lower note first)
             int rank = 0;
             for (int j = 0; j < a.B; ++j) {
@@ -307,7 +302,7 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
             note = __builtin_amdgcn_ds_permute(rank << 2, note);
             len = __builtin_amdgcn_ds_permute(rank << 2, len);
         }
-        const int nch = note < a.B ? max(1, (len + chunk - 1) / chunk) : 0;
+        const int nch = note < a.B ? max(1, (int)(((uint32_t)len + (uint32_t)chunk - 1) / (uint32_t)chunk)) : 0;
         int incl = nch;  // chunks up to and with this lane
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -322,14 +317,11 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
             const int first = base + pa_scalar(__shfl(incl, src)) - u.nch;
             u.c = ci - first;
             if (want_b >= 0) u.c = 0, u.ci = first;
+            u.sp = {pa_scalar(__shfl(sp.start, u.b - b0)), pa_scalar(__shfl(len, src))};
         }
         base += pa_scalar(__shfl(incl, 63));
     }
     u.all = base;
-    if (u.b >= 0) {
-        u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
-        u.sp = {pa_scalar(u.sp.start), pa_scalar(u.sp.len)};
-    }
     return u;
 }
 // dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  With s parts the chip's 256 compute units take
@@ -343,9 +335,11 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
     const int lane = threadIdx.x & 63;
     PaTileUnit u;
     u.b = -1;
-    auto tiles_of = [&](int b) { return b < a.B ? (note_span(a.spans, b, a.rows, a.max_len).len + PA_TILE - 1) / PA_TILE : 0; };
-    int n = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) n += tiles_of(b0 + lane);
+    auto span = [&](int b) { return b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0}; };
+    NoteSpan sp = span(lane);
+    auto tiles = [](int len) { return (int)(((uint32_t)len + PA_TILE - 1) / PA_TILE); };
+    int n = tiles(sp.len);
+    for (int b0 = 64; b0 < a.B; b0 += 64) n += tiles(span(b0 + lane).len);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     n = pa_scalar(n);
@@ -361,7 +355,8 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
     u.share = unit % u.shares;
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int nt = tiles_of(b0 + lane);
+        if (b0) sp = span(b0 + lane);
+        const int nt = tiles(sp.len);
         int incl = nt;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -373,12 +368,9 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
             const int src = __ffsll((long long)hit) - 1, first = base + pa_scalar(__shfl(incl, src) - __shfl(nt, src));
             u.b = b0 + src;
             u.tile = want_b >= 0 ? first : t - first;  // want_b: the note's first tile among all
+            u.sp = {pa_scalar(__shfl(sp.start, src)), pa_scalar(__shfl(sp.len, src))};
         }
         base += pa_scalar(__shfl(incl, 63));
-    }
-    if (u.b >= 0) {
-        u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
-        u.sp = {pa_scalar(u.sp.start), pa_scalar(u.sp.len)};
     }
     return u;
 }

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
             pa_emit<K, G, G::NF, 1, false>(sf, img, tid);
         } else {
             pa_emit<K, G, G::RF, G::SF, true>(sf, img, tid);
-            if (!G::TR) pa_emit<K, G, G::NE, 1, false>(se, img + G::PL * G::RF * 1024, tid);
+            if (!G::TRT) pa_emit<K, G, G::NE, 1, false>(se, img + G::PL * G::RF * 1024, tid);
         }
     } else {
         const int q = id - nTok;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
         __syncthreads();
         char* img = a.Q + (long long)q * (BWD ? G::QRY : G::PL * G::RE) * 1024;
         pa_emit<K, G, G::RE, G::SE, true>(se, img, tid);
-        if (BWD && !G::TR) pa_emit<K, G, G::NE, 1, false>(se, img + G::RE * 1024, tid);
+        if (BWD && !G::TRL) pa_emit<K, G, G::NE, 1, false>(se, img + G::RE * 1024, tid);
     }
 }
 // Backward: dO images of (note, label tile); behind the fragments, for each label, off and scale of its weights
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
         aux[2 * G::ROWS + r] = s;
     }
     pa_emit<K, G, G::RF, G::SF, true>(sf, img, tid);
-    if (!G::TR) pa_emit<K, G, G::NF, 1, false>(sf, img + G::PL * G::RF * 1024, tid);
+    if (!G::TRL) pa_emit<K, G, G::NF, 1, false>(sf, img + G::PL * G::RF * 1024, tid);
 }
 
 // Four consecutive values of an output row, and what rounding them dropped.
@@ -230,6 +230,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
+        if (!CAP) mt *= PA_LOG2E;
         if (__any(mt > w.m + 12.f)) {  // m is the same in the four lanes of a column
             mt = fmaxf(mt, __shfl_xor(mt, 16));
             mt = fmaxf(mt, __shfl_xor(mt, 32));
@@ -243,7 +244,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[u][r] -= mi;
+            for (int r = 0; r < 4; ++r) y[u][r] = CAP ? y[u][r] - mi : fmaf(y[u][r], PA_LOG2E, -mi);
     }
     frag pf;
     {
@@ -500,12 +501,12 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
 
 // ------------------------------------------------------------------------------------------------------------- backward
 // P and dS of a tile: weights w = exp2(y - off) * scale, dropout factor keep.
-template <bool CAP>
+template <bool CAP, bool TH>
 __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, float scale, float delta, float keep, float& p, float& ds) {
-    const float w = __builtin_amdgcn_exp2f(y - off) * scale;
+    const float w = __builtin_amdgcn_exp2f(CAP ? y - off : fmaf(y, PA_LOG2E, -off)) * scale;
     p = w * keep;
     ds = w * fmaf(dp, keep, -delta);
-    if (CAP) ds *= fmaf(-th, th, 1.f);
+    if (TH) ds *= fmaf(-th, th, 1.f);
 }
 
 // dK / dV: workgroup = 128 tokens of one note (16 a wave, tokens on the lane axis), sweeping its share of the labels.  PaX3 takes dV
@@ -569,11 +570,11 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
                 else dp[(i - G::RE) % U] = pa_mma(f, vf[DK ? (i - G::RE) / U : 0], dp[(i - G::RE) % U]);
             });
             auto ldv = [&](int j) {
-                if constexpr (G::TR) return pa_col_tr<G::SF>(DR, j, n, g);
+                if constexpr (G::TRL) return pa_col_tr<K, G::SF>(DR, j, n, g);
                 else return pa_frag<K, G::NF>(DR + G::RF * 1024, j, lane);
             };
             auto ldk = [&](int j) {
-                if constexpr (G::TR) return pa_col_tr<G::SE>(QR, j, n, g);
+                if constexpr (G::TRL) return pa_col_tr<K, G::SE>(QR, j, n, g);
                 else return pa_frag<K, G::NE>(QR + G::RE * 1024, j, lane);
             };
             constexpr int NC = (DV ? G::NF : 0) + (DK ? G::NE : 0);
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
                         const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
                         keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
                     }
-                    pa_grad<CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
+                    pa_grad<CAP, CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
                 }
             }
             frag pf, sf;
@@ -677,14 +678,15 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     }
 }
 
-// dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.
-template <class K, class G, int WAVES, bool CAP, bool DROP>
-__global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
+// dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.  H = 2: twice the
+// waves, which take turns at the token tiles and add up in LDS (few labels: half the way through the longest note).
+template <class K, class G, int WAVES, int H, bool CAP, bool DROP>
+__global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     typedef typename K::T T;
     typedef typename K::frag frag;
     constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6) % WAVES, h = pa_scalar(tid >> 6) / WAVES, n = lane & 15, g = lane >> 4;
     const int lt = blockIdx.x % a.nLT;
     const PaUnit un = pa_unit<G::ROWS>(a, blockIdx.x / a.nLT);
     if (un.ci >= un.all) return;
@@ -711,13 +713,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
 #pragma unroll
     for (int j = 0; j < G::NE; ++j) dq[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const char* tk = a.TK + (long long)b * a.nT * G::TOK * 1024;
-    if (t0 < t1) pa_dma<WAVES, G::TOK>(tk + (long long)t0 * G::TOK * 1024, sm, wave, lane);
+    auto fetch = [&](int t, int k) {
+        if (t < t1) pa_dma<WAVES, G::TOK>(tk + (long long)t * G::TOK * 1024, sm + (2 * h + (k & 1)) * G::TOK * 1024, wave, lane);
+    };
+    fetch(t0 + h, 0);
     pa_arrive();
-    auto step = [&](int t, auto last) {  // last: the tile may end behind the note
-        const char* KR = sm + ((t - t0) & 1) * G::TOK * 1024;
+    const int steps = (t1 - t0 + H - 1) / H;
+    auto step = [&](int k, auto last) {  // last: the tile may end behind the note, or there is none for this half
+        const char* KR = sm + (2 * h + (k & 1)) * G::TOK * 1024;
         const char* VR = KR + G::PL * G::RE * 1024;
-        if (t + 1 < t1) pa_dma<WAVES, G::TOK>(tk + (long long)(t + 1) * G::TOK * 1024, sm + ((t - t0 + 1) & 1) * G::TOK * 1024, wave, lane);
-        if (!idle) {
+        const int t = t0 + k * H + h;
+        fetch(t + H, k + 1);
+        if (!idle && (!decltype(last)::value || t < t1)) {
             f32x4 s[U], dp[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -732,7 +739,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
                 else dp[(i - G::RE) % U] = pa_mma(f, df[(i - G::RE) / U], dp[(i - G::RE) % U]);
             });
             auto ldc = [&](int j) {
-                if constexpr (G::TR) return pa_col_tr<G::SE>(KR, j, n, g);
+                if constexpr (G::TRT) return pa_col_tr<K, G::SE>(KR, j, n, g);
                 else return pa_frag<K, G::NE>(VR + G::RF * 1024, j, lane);
             };
             pa_fill_ring<G::NE>(ring, ldc);
@@ -744,7 +751,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
                 for (int r = 0; r < 4; ++r) {
                     float keep = 1.f, p;
                     if (DROP) keep = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? a.scale : 0.f;
-                    pa_grad<CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
+                    pa_grad<CAP, CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
                 }
             if constexpr (decltype(last)::value) {  // (a key of zeros has the score 0, which may be far above the note's own)
                 const int left = len - t * G::ROWS;
@@ -765,8 +772,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
         }
         pa_arrive();
     };
-    for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
-    if (t0 < t1) step(t1 - 1, std::true_type{});
+    for (int k = 0; k < steps - 1; ++k) step(k, std::false_type{});
+    if (steps > 0) step(steps - 1, std::true_type{});
+    if constexpr (H == 2) {
+        f32x4* sum = reinterpret_cast<f32x4*>(sm) + wave * G::NE * 64 + lane;
+        static_assert(WAVES * G::NE <= 4 * G::TOK, "fits the buffers");
+        if (h == 1)
+#pragma unroll
+            for (int j = 0; j < G::NE; ++j) sum[64 * j] = dq[j];
+        __syncthreads();
+        if (h == 1) return;
+#pragma unroll
+        for (int j = 0; j < G::NE; ++j) dq[j] += sum[64 * j];
+    }
     const int l = l0 + n;
     if (l >= a.L) return;
     float* out = a.dq + ((long long)un.ci * a.L + l) * a.E;
@@ -804,11 +822,11 @@ static int pa_fwd(PaArgs& a, hipStream_t st) {
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <class K, class G, int W, bool CAP, bool DROP>
+template <class K, class G, int W, int H, bool CAP, bool DROP>
 static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     typedef typename K::T T;
     constexpr int lds = 2 * (G::QRY + G::OUT) * 1024;
-    static_assert(lds <= 160 * 1024 && 2 * G::TOK <= 160 && 2 * G::FWD <= 160, "two buffers in LDS");
+    static_assert(lds <= 160 * 1024 && 2 * H * G::TOK <= 160 && 2 * G::FWD <= 160, "two buffers in LDS");
     hipLaunchKernelGGL((pa_pack_kernel<K, G, true>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_pack_do_kernel<K, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
     if (p.units > 0) {
@@ -820,7 +838,7 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
         }
     }
     hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, PA_JOIN_ROWS) : 1, a.B + 1), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((pa_bwd_q_kernel<K, G, W, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::TOK * 1024, st, a);
+    hipLaunchKernelGGL((pa_bwd_q_kernel<K, G, W, H, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * H * 64), 2 * H * G::TOK * 1024, st, a);
     const long long n = (long long)a.L * a.E;
     hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS>), dim3((unsigned)(n < 256 * 4096 ? cdiv((long)n, 256) : 4096)), dim3(256), 0, st, a);
     GZSL_CHECK_LAUNCH();
@@ -835,8 +853,8 @@ template <class K, class G, int W, int OCC>
 static int pa_go_fwd(PaArgs& a, hipStream_t st) {
     return a.cap > 0.f ? pa_fwd_drop<K, G, W, OCC, true>(a, st) : pa_fwd_drop<K, G, W, OCC, false>(a, st);
 }
-template <class K, class G, int W>
+template <class K, class G, int W, int H>
 static int pa_go_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
-    if (a.cap > 0.f) return a.thresh ? pa_bwd<K, G, W, true, true>(a, p, st) : pa_bwd<K, G, W, true, false>(a, p, st);
-    return a.thresh ? pa_bwd<K, G, W, false, true>(a, p, st) : pa_bwd<K, G, W, false, false>(a, p, st);
+    if (a.cap > 0.f) return a.thresh ? pa_bwd<K, G, W, H, true, true>(a, p, st) : pa_bwd<K, G, W, H, true, false>(a, p, st);
+    return a.thresh ? pa_bwd<K, G, W, H, false, true>(a, p, st) : pa_bwd<K, G, W, H, false, false>(a, p, st);
 }
