@@ -384,7 +384,7 @@ static int gs_check(const GzslGatedScan* d) {
 static GsArgs gs_args(const GzslGatedScan& d) {
     GsArgs a{};
     a.g = d.gates, a.c = d.cands, a.spans = d.spans, a.h0 = d.h0, a.rows = d.rows, a.ldg = d.ldg, a.ldc = d.ldc;
-    a.B = d.B, a.max_len = d.max_len, a.H = d.H, a.reverse = d.reverse;
+    a.B = d.B, a.max_len = d.max_len < d.rows ? d.max_len : (int)d.rows, a.H = d.H, a.reverse = d.reverse;
     return a;
 }
 

@@ -376,7 +376,7 @@ __device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, in
 }
 
 struct PaPlan {
-    int nT, nQ, kind, waves, extra, least, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
+    int max_len, nT, nQ, kind, waves, extra, least, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
     float slab;
     long long units;  // workgroups of the dK / dV sweep
     long long kv, q, dO, part, ml, dq, dkv, bytes;

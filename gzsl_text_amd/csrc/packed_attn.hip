@@ -5,7 +5,7 @@ static inline long long up256(long long n) { return (n + 255) / 256 * 256; }
 
 template <class G>
 static void pa_sizes(PaPlan& p, const GzslPackedAttn& d, int backward) {
-    p.nT = (int)(((long long)d.max_len + G::ROWS - 1) / G::ROWS), p.nQ = (int)(((long long)d.L + G::ROWS - 1) / G::ROWS);
+    p.nT = (int)(((long long)p.max_len + G::ROWS - 1) / G::ROWS), p.nQ = (int)(((long long)d.L + G::ROWS - 1) / G::ROWS);
     p.kv = 1024LL * d.B * p.nT * (backward ? G::TOK : G::FWD);
     p.q = 1024LL * p.nQ * (backward ? G::QRY : G::PL * G::RE);
     p.dO = backward ? 1024LL * d.B * p.nQ * G::OUT : 0;
@@ -13,10 +13,11 @@ static void pa_sizes(PaPlan& p, const GzslPackedAttn& d, int backward) {
 static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     if (!d || d->B < 0 || d->rows < 0 || d->max_len < 0 || d->L < 0 || d->E < 1 || d->F < 1 || d->E > 208 || d->F > 208) return GZSL_EINVAL;
     if (d->dtype != GZSL_F32 && d->dtype != GZSL_BF16) return GZSL_EINVAL;
-    if (!(d->cap >= 0.f) || d->cap > 1e30f) return GZSL_EINVAL;
+    if (d->cap != 0.f && !(d->cap >= 1e-30f && d->cap <= 1e30f)) return GZSL_EINVAL;
     if (d->ldk < d->E || d->ldv < d->F || d->ldq < d->E) return GZSL_EINVAL;
     if (d->B > 65534 || d->max_len > 0x7FFF0000 || d->L > 0x7FFF0000) return GZSL_ETOOBIG;
     p = PaPlan{};
+    p.max_len = d->max_len < d->rows ? d->max_len : (int)d->rows;  // (no note is longer than the rows there are)
     p.kind = (d->dtype == GZSL_F32 ? 2 : 0) + (d->E > 112);
     if (p.kind == 0) pa_sizes<PaGeo<PaBF, 7, 13>>(p, *d, backward);
     else if (p.kind == 1) pa_sizes<PaGeo<PaBF, 13, 13>>(p, *d, backward);
@@ -31,8 +32,8 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     p.nLT = cdiv(d->L, 16 * p.waves);
     const long long wgs = (long long)d->B * p.nLT;
     p.least = fits ? 128 : 256;  // tokens of a chunk that pay for its own start and its part in the join
-    p.extra = wgs > 0 && wgs < 256 && d->max_len > p.least ? cdiv(p.waves == 4 && !backward ? 512 : 256, p.nLT) : 0;
-    if (p.extra > d->B * (d->max_len / p.least + 1)) p.extra = d->B * (d->max_len / p.least + 1);
+    p.extra = wgs > 0 && wgs < 256 && p.max_len > p.least ? cdiv(p.waves == 4 && !backward ? 512 : 256, p.nLT) : 0;
+    if (p.extra > (long long)d->B * (p.max_len / p.least + 1)) p.extra = d->B * (p.max_len / p.least + 1);
     const long long chunks = d->B + p.extra;
     if ((long long)d->B * p.nT + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
         return GZSL_ETOOBIG;
@@ -42,7 +43,7 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     }
     if (backward) {
         p.dq = up256(4 * chunks * d->L * d->E);
-        long long tiles = (long long)d->B * cdiv(d->max_len, PA_TILE);  // at most
+        long long tiles = (long long)d->B * cdiv(p.max_len, PA_TILE);  // at most
         if (tiles > d->rows / PA_TILE + d->B) tiles = d->rows / PA_TILE + d->B;
         p.shares = p.nQ / 4 < 1 ? 1 : (p.nQ / 4 > 16 ? 16 : p.nQ / 4);  // (four label tiles a share at least)
         // a slab moves (E + F) 8 bytes a token at 4 TB/s; a tile's scores take L / (scores a ns of the chip / 256) a token on one unit
@@ -60,7 +61,7 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
 static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* work) {
     a.keys = d.keys, a.values = d.values, a.queries = d.queries, a.spans = d.spans;
     a.rows = d.rows, a.ldk = d.ldk, a.ldv = d.ldv, a.ldq = d.ldq;
-    a.B = d.B, a.max_len = d.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
+    a.B = d.B, a.max_len = p.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
     a.nLT = p.nLT, a.extra = p.extra, a.least = p.least, a.shares = p.shares, a.slots = p.slots, a.slab = p.slab;
     char* w = (char*)work;

@@ -205,6 +205,9 @@ void touched(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// The gradients come from kernels that autograd does not see through: a graph of them would miss every term.
+void check_once(const char* what) { TORCH_CHECK(!at::GradMode::is_enabled(), "gzsl: ", what, " is differentiable once (backward with create_graph)"); }
+
 struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttention> {
     static GzslPackedAttn describe(const Tensor& k, const Tensor& v, const Tensor& q, const Tensor& spans, int64_t max_len, double cap, double p,
                                    int64_t seed, int64_t l_offset, int64_t L_total) {
@@ -226,7 +229,7 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         TORCH_CHECK(k.size(1) == q.size(1), "gzsl: keys / queries disagree on the embedding width");
         TORCH_CHECK(k.device() == v.device() && k.device() == q.device(), "gzsl: tensors on one device");
         TORCH_CHECK(k.size(1) <= 208 && v.size(1) <= 208 && k.size(1) > 0 && v.size(1) > 0, "gzsl: widths from 1 to 208");
-        TORCH_CHECK(cap >= 0.0 && cap <= 1e30, "gzsl: cap must be 0 (none) or positive");
+        TORCH_CHECK(cap == 0.0 || (cap >= 1e-30 && cap <= 1e30), "gzsl: cap must be 0 (none) or from 1e-30 to 1e30");
         TORCH_CHECK(p_drop >= 0.0 && p_drop < 1.0, "gzsl: drop probability in [0, 1)");
         check_spans(spans, max_len, k);
         if (L_total <= 0) L_total = q.size(0);
@@ -251,6 +254,7 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         return {O, lse};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_once("packed_label_attention");
         const auto saved = ctx->get_saved_variables();
         const Tensor &k = saved[0], &v = saved[1], &q = saved[2], &spans = saved[3], &O = saved[4], &lse = saved[5], &rest = saved[6];
         const c10::DeviceGuard guard(k.device());
@@ -314,6 +318,7 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
         return {h, last};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_once("gated_scan");
         const auto saved = ctx->get_saved_variables();
         const Tensor &g = saved[0], &c = saved[1], &spans = saved[2], &h = saved[3], &h0 = saved[4];
         const c10::DeviceGuard guard(g.device());
@@ -362,7 +367,7 @@ void gated_scan_step_(const Tensor& gates, const Tensor& cands, const Tensor& st
 }
 
 // ---- gradient clipping (gzsl_clip_grad_norm, gzsl_adamw_clip_step)
-// Addresses of contiguous tensors on one device; a tensor given twice would be updated twice at once.
+// Addresses of contiguous tensors on one device.
 std::vector<void*> pointers(at::TensorList ts, const c10::Device& dev, const char* name, bool f32_only) {
     std::vector<void*> out;
     out.reserve(ts.size());
@@ -374,9 +379,24 @@ std::vector<void*> pointers(at::TensorList ts, const c10::Device& dev, const cha
     }
     return out;
 }
-void check_distinct(std::vector<void*> all) {
-    std::sort(all.begin(), all.end());
-    for (size_t i = 1; i < all.size(); ++i) TORCH_CHECK(!all[i] || all[i] != all[i - 1], "gzsl: the same tensor appears twice in the list");
+// Written tensors may share memory with nothing else of the call: it would be updated twice at once, or read in between.
+struct Extent {
+    const char *at, *end;
+    bool written;
+};
+void extents(std::vector<Extent>& all, at::TensorList ts, bool written) {
+    all.reserve(all.size() + ts.size());
+    for (const Tensor& t : ts)
+        if (t.numel() > 0) all.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + t.nbytes(), written});
+}
+void check_apart(std::vector<Extent>& all) {
+    std::sort(all.begin(), all.end(), [](const Extent& a, const Extent& b) { return a.at < b.at; });
+    const char *end = nullptr, *written = nullptr;  // of the extents so far: furthest end, and that of a written one
+    for (const Extent& e : all) {
+        TORCH_CHECK(e.at >= (e.written ? end : written), "gzsl: the same tensor appears twice in the list, or two of them overlap");
+        end = std::max(end, e.end);
+        if (e.written) written = std::max(written, e.end);
+    }
 }
 c10::Device device_of(at::TensorList ts) { return ts.empty() ? c10::Device(c10::kCUDA, c10::hip::current_device()) : ts[0].device(); }
 
@@ -384,7 +404,9 @@ Tensor clip_grad_norm_(at::TensorList grads, double max_norm) {
     TORCH_CHECK(max_norm > 0.0, "gzsl: max_norm must be positive");
     const c10::Device dev = device_of(grads);
     const auto g = pointers(grads, dev, "grads", false);
-    check_distinct(g);
+    std::vector<Extent> held;
+    extents(held, grads, true);
+    check_apart(held);
     std::vector<long long> n;
     std::vector<int> t;
     for (const Tensor& x : grads) n.push_back(x.numel()), t.push_back(x.scalar_type() == at::kFloat ? GZSL_F32 : GZSL_BF16);
@@ -404,10 +426,9 @@ Tensor adamw_clip_step_(at::TensorList params, at::TensorList grads, at::TensorL
     TORCH_CHECK(params.size() == grads.size() && params.size() == m.size() && params.size() == v.size(), "gzsl: params, grads and moments do not fit");
     const c10::Device dev = device_of(params);
     const auto p = pointers(params, dev, "params", true), g = pointers(grads, dev, "grads", true), mm = pointers(m, dev, "m", true), vv = pointers(v, dev, "v", true);
-    std::vector<void*> written(p);
-    written.insert(written.end(), mm.begin(), mm.end());
-    written.insert(written.end(), vv.begin(), vv.end());
-    check_distinct(written);
+    std::vector<Extent> held;
+    extents(held, params, true), extents(held, m, true), extents(held, v, true), extents(held, grads, false);
+    check_apart(held);
     std::vector<long long> n;
     for (size_t i = 0; i < params.size(); ++i) {
         TORCH_CHECK(grads[i].sizes() == params[i].sizes() && m[i].sizes() == params[i].sizes() && v[i].sizes() == params[i].sizes(),

@@ -611,13 +611,22 @@ class HipOps:
     # ------------------------------------------------------------------------------------ gradient clipping
     @staticmethod
     def _pointers(ts):
-        """Host array of the tensors' addresses; a tensor given twice would be updated twice at once."""
+        """Host array of the tensors' addresses."""
         import ctypes
-        a = [ptr(t) for t in ts]
-        held = [x for x in a if x]
-        if len(set(held)) != len(held):
-            raise RuntimeError('the same tensor appears twice in the list')
-        return (ctypes.c_void_p * max(len(a), 1))(*a)
+        return (ctypes.c_void_p * max(len(ts), 1))(*[ptr(t) for t in ts])
+
+    @staticmethod
+    def _apart(written, read=()):
+        """Written tensors may share memory with nothing else of the call: it would be updated twice at once, or read in between."""
+        held = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w) for ts, w in ((written, True), (read, False))
+                      for t in ts if t.numel())
+        end = written_end = 0
+        for a, b, w in held:
+            if a < (end if w else written_end):
+                raise RuntimeError('the same tensor appears twice in the list, or two of them overlap')
+            end = max(end, b)
+            if w:
+                written_end = max(written_end, b)
 
     @staticmethod
     def _sizes(ts):
@@ -636,6 +645,7 @@ class HipOps:
         dev = grads[0].device if grads else torch.device('cuda', torch.cuda.current_device())
         sizes, n = self._sizes(grads), len(grads)
         types = (ctypes.c_int * max(n, 1))(*[self._dtype(t) for t in grads])
+        self._apart(grads)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         work = torch.empty(max(hip.load().gzsl_clip_work_bytes(sizes, n), 16), dtype=torch.uint8, device=dev)
         call('gzsl_clip_grad_norm', self._pointers(grads), sizes, types, n, float(max_norm), ptr(norm), ptr(work), work.numel())
@@ -655,7 +665,7 @@ class HipOps:
             _check_f32(*x)
         dev = lists[0][0].device if n else torch.device('cuda', torch.cuda.current_device())
         sizes = self._sizes(lists[0])
-        self._pointers(lists[0] + lists[2] + lists[3])  # (no tensor may be written twice, across the lists either)
+        self._apart(lists[0] + lists[2] + lists[3], lists[1])
         norm = torch.empty((), dtype=torch.float32, device=dev)
         work = torch.empty(max(hip.load().gzsl_clip_work_bytes(sizes, n), 16), dtype=torch.uint8, device=dev)
         call('gzsl_adamw_clip_step', *[self._pointers(x) for x in lists], sizes, n, float(max_norm), lr, beta1, beta2, eps, wd,

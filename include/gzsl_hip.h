@@ -269,7 +269,8 @@ int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long 
 /* ---- packed notes -----------------------------------------------------------------------------------------------
  * Notes of unequal length in one [rows, width] tensor: note b owns rows spans[2b] .. spans[2b] + spans[2b+1] - 1 (int64, on
  * the device, ascending and disjoint; a padded [B,T,width] batch is spans (b*T, length)).  `max_len` is at least the longest
- * count.  The kernels clamp every span to [0, rows) and max_len.  Tensors are fp32 or bf16 (`dtype`), their rows `ld*`
+ * count.  The kernels clamp every span to [0, rows) and max_len: a table that is neither ascending nor disjoint gives wrong numbers, never an
+ * access out of range.  Tensors are fp32 or bf16 (`dtype`), their rows `ld*`
  * elements apart with consecutive elements inside a row; sums, softmax statistics and states are fp32 for both. */
 #define GZSL_F32 0
 #define GZSL_BF16 1
@@ -277,7 +278,7 @@ int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long 
  * padding):  x = <q_l, k_t>, y = cap*tanh(x/cap) (cap = 0: y = x), softmax of y over the note's own tokens, dropout on the
  * weights (the masks of gzsl_label_attn_fwd, keyed on (b*L_total + l_offset + l, token index in the note)), pooling of the
  * values.  O [B,L,F] of the tensors' type, LSE [B,L] fp32 (natural units); a note of no tokens gives O = 0, LSE = -inf.
- * E, F <= 208.  `work`: 16-byte aligned device scratch of gzsl_packed_attn_work_bytes(d, backward) bytes (-1: bad arguments),
+ * E, F <= 208; cap 0 or from 1e-30 to 1e30.  `work`: 16-byte aligned device scratch of gzsl_packed_attn_work_bytes(d, backward) bytes (-1: bad arguments),
  * its contents undefined before and after. */
 typedef struct GzslPackedAttn {
     const void* keys;    /* [rows, E] */

@@ -295,6 +295,20 @@ def test_many_notes(ops):
             within(x, ref[name], name)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('E,cap', [(24, 0.0), (24, 30.0), (200, 0.0), (200, 3.0)])
+def test_more_workgroups_than_the_chip_has_places(ops, dtype, E, cap):
+    """66 notes x 1100 labels: label workgroups of full width in both directions, at both key widths."""
+    gen = torch.Generator().manual_seed(6)
+    lens = [int(x) for x in torch.randint(0, 50, (65,), generator=gen)] + [133]
+    k, v, q, do, spans, max_len, sl = make(lens, E, 40, 1100, dtype, seed=9, tail=2)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
+    got = (O, lse, *ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, cap))
+    ref = attn_ref(k, v, q, sl, cap, do)
+    for name, x in zip(('O', 'lse', 'dK', 'dV', 'dQ'), got):
+        within(x, ref[name], name)
+
+
 def test_a_wrong_table_is_clamped_to_the_rows(ops):
     """Counts and starts outside of the rows give other numbers, never an access out of range (the kernels clamp them)."""
     k, v, q, do, _, _, _ = make([40], 16, 16, 5, torch.float32, seed=2)

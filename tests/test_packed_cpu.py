@@ -159,3 +159,32 @@ def test_adamw_refuses_a_bad_max_grad_norm():
     for bad in (0.0, -1.0, float('nan')):
         with pytest.raises(ValueError):
             AdamW([torch.nn.Parameter(torch.zeros(3))], max_grad_norm=bad)
+
+
+@lib_built
+@pytest.mark.parametrize('cap', [1e-31, 2e30])
+def test_attention_refuses_a_cap_without_a_reciprocal(cap):
+    assert hip.load().gzsl_packed_attn_work_bytes(attn(cap=cap), 0) == -1
+
+
+@lib_built
+def test_max_len_beyond_the_rows_takes_no_more_workspace():
+    lib = hip.load()
+    for backward in (0, 1):
+        assert lib.gzsl_packed_attn_work_bytes(attn(max_len=2 ** 30), backward) == lib.gzsl_packed_attn_work_bytes(attn(max_len=10), backward) > 0
+    d = dict(gates=4096, cands=4096, spans=4096, h0=None, rows=10 ** 5, ldg=8, ldc=8, B=1, max_len=10 ** 5, H=8, reverse=0, dtype=hip.F32)
+    need = lib.gzsl_gated_scan_work_bytes(hip.GzslGatedScan(**d), 0)
+    assert need > 0 and lib.gzsl_gated_scan_work_bytes(hip.GzslGatedScan(**dict(d, max_len=2 ** 30)), 0) == need
+    # chunk sizes stay below 2^31 at the largest batch, and a width of more channels than the grid has room for is refused
+    assert lib.gzsl_gated_scan_work_bytes(hip.GzslGatedScan(**dict(d, B=65534, rows=2 ** 31, max_len=2 ** 30)), 0) >= 0
+    assert lib.gzsl_gated_scan_work_bytes(hip.GzslGatedScan(**dict(d, H=65537, ldg=65537, ldc=65537)), 0) == -1
+
+
+def test_overlapping_tensors_are_found():
+    from gzsl_text_amd.ops_hip import HipOps
+    x = torch.zeros(10)
+    HipOps._apart([x[:5], x[5:], x[:0]], [torch.ones(3)])
+    HipOps._apart([torch.ones(2)], [x, x])  # read twice: nothing is written there
+    for written, read in (([x, x], ()), ([x[:6], x[5:]], ()), ([x[2:4]], [x]), ([x], [x[9:]]), ([x[:1], x], [x])):
+        with pytest.raises(RuntimeError, match='overlap'):
+            HipOps._apart(written, read)
