@@ -437,6 +437,21 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
     const int per = (un.nch + G - 1) / G, c0 = on ? part * per : 0, c1 = on ? min(un.nch, c0 + per) : 0;
     const float* ml = a.ml + 2 * ((long long)un.ci * a.L + l);
     const float* pr = a.part + ((long long)un.ci * a.L + l) * a.F;
+    constexpr int D = 4;  // parts of a row on their way, the first of them while the weights are worked out
+    f32x4 v[D];           // values 4 lane .. + 3 (vec), else lane + 64 k
+    auto load = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            const float* x = pr + (long long)min(c + i, c1 - 1) * a.L * a.F;
+            if (vec) {
+                v[i] = *reinterpret_cast<const f32x4*>(x + min(4 * lane, a.F - 4));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[i][k] = x[min(lane + 64 * k, a.F - 1)];
+            }
+        }
+    };
+    if (c0 < c1) load(c0);
     float M = -INFINITY;
     for (int c = c0 + lane; c < c1; c += 64)
         if (ml[2LL * c * a.L + 1] != 0.f) M = fmaxf(M, ml[2LL * c * a.L]);  // (no finite score in this chunk: sum 0)
@@ -448,27 +463,23 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
 #pragma unroll
         for (int k = 0; k < G; ++k) M = fmaxf(M, sM[k]);
     }
-    float sum = 0.f;
-    f32x4 o4 = f32x4{0.f, 0.f, 0.f, 0.f};  // values 4 lane .. + 3 (vec), else lane + 64 k
-    for (int b0 = c0; b0 < c1; b0 += 64) {
-        const int c = min(b0 + lane, c1 - 1);
-        const float s = b0 + lane < c1 ? ml[2LL * c * a.L + 1] : 0.f, f = s != 0.f ? __builtin_amdgcn_exp2f(ml[2LL * c * a.L] - M) : 0.f;
-        sum = fmaf(f, s, sum);
-        const int n = min(64, c1 - b0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float fi = __shfl(f, i);
-            const float* x = pr + (long long)(b0 + i) * a.L * a.F;
-            f32x4 v;
-            if (vec) {
-                v = *reinterpret_cast<const f32x4*>(x + min(4 * lane, a.F - 4));
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = x[min(lane + 64 * k, a.F - 1)];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o4[k] = fi != 0.f ? fmaf(fi, v[k], o4[k]) : o4[k];
+    float sum = 0.f, f = 0.f;
+    f32x4 o4 = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b0 = c0; b0 < c1; b0 += D) {
+        if ((b0 - c0) % 64 == 0) {
+            const int c = min(b0 + lane, c1 - 1);
+            const float s = b0 + lane < c1 ? ml[2LL * c * a.L + 1] : 0.f;
+            f = s != 0.f ? __builtin_amdgcn_exp2f(ml[2LL * c * a.L] - M) : 0.f;
+            sum = fmaf(f, s, sum);
         }
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            const float fi = __shfl(f, (b0 - c0) % 64 + i);
+            if (b0 + i < c1 && fi != 0.f)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o4[k] = fmaf(fi, v[i][k], o4[k]);
+        }
+        if (b0 + D < c1) load(b0 + D);
     }
     sum = wave_sum(sum);
 #pragma unroll
