@@ -245,12 +245,10 @@ struct PaArgs {
     uint32_t l_offset, L_total, seed, thresh;
     float scale;
     int nLT, extra, least;            // label workgroups of a note; token chunks beyond one a note (0: notes are not cut), their tokens at least
-    int shares, slots;                // dK / dV: label shares of a token tile at most, slabs that the workspace has room for
-    float slab;                       // time of a slab's write and read by the whole chip, in times of a tile on one compute unit
     // workspace
     char *TK, *Q, *DO;  // images: token tiles [B][nT], queries [nQ], dO [B][nQ]
     float *part, *ml;  // forward, notes cut: unnormalised O [chunk][L][F] and (max, sum) [chunk][L][2]
-    float *dq, *dkv;   // backward: [chunk][L][E]; [unit][PA_TILE][E + F]
+    float *dq, *dkv;   // backward: [chunk][L][E]; [slab][PA_TILE][E + F]
     // results and the backward's inputs
     void* O;
     float *LSE, *rest;  // rest: (max in log 2, 1 / sum) [B][L][2], then for bf16 what the rounding of O dropped, [B][L][F]
@@ -324,61 +322,68 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
     u.all = base;
     return u;
 }
-// dK / dV: units of PA_TILE tokens x one of `shares` parts of the labels.  With s parts the chip's 256 compute units take
-// ceil(n s / 256) rounds of 1 / s of a tile's time, and n s slabs are written and read again, each a.slab of a round: the s that is
-// least.
-struct PaTileUnit {
-    int b, tile, share, shares, unit, tiles;
+// dK / dV: the steps of the sweep, token tile by token tile (PA_TILE tokens x the label tiles), in PA_UNITS equal runs, one for each
+// compute unit (less where a run would be under four steps): every compute unit works for the same time, and only the tiles at a run's
+// two ends are shared and go through slabs (2 u for one that the run begins inside of, 2 u + 1 for the one that it ends in).  With
+// equal parts of a tile instead, as many as a cost rule found best, 17404 tokens x 1999 labels of 200 bf16 took 99 us, so 88; x 9000
+// labels, with their slabs' join, 415 and 380.
+#define PA_UNITS 256
+struct PaTile {
+    int b, tile;  // note, token tile in it
     NoteSpan sp;
 };
-__device__ __forceinline__ PaTileUnit pa_tile_unit(const PaArgs& a, int unit, int want_b = -1) {
+__device__ __forceinline__ int pa_tiles(int len) { return (int)(((uint32_t)len + PA_TILE - 1) / PA_TILE); }
+// Token tiles of all notes, and of those in front of note b.
+__device__ __forceinline__ int pa_all_tiles(const PaArgs& a, int b, int& before) {
     const int lane = threadIdx.x & 63;
-    PaTileUnit u;
-    u.b = -1;
-    auto span = [&](int b) { return b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0}; };
-    NoteSpan sp = span(lane);
-    auto tiles = [](int len) { return (int)(((uint32_t)len + PA_TILE - 1) / PA_TILE); };
-    int n = tiles(sp.len);
-    for (int b0 = 64; b0 < a.B; b0 += 64) n += tiles(span(b0 + lane).len);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-    n = pa_scalar(n);
-    u.tiles = n;
-    u.shares = 1;
-    float best = 1e30f;
-    for (int s = 1; s <= a.shares && (s == 1 || (long long)n * s <= a.slots); ++s) {
-        const float t = (float)((n * s + 255) / 256) / s + (s > 1 ? a.slab * n * s : 0.f);
-        if (t < best) best = t, u.shares = s;
-    }
-    u.unit = unit;
-    const int t = unit / u.shares;
-    u.share = unit % u.shares;
-    int base = 0;
+    int n = 0, m = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        if (b0) sp = span(b0 + lane);
-        const int nt = tiles(sp.len);
+        const int t = b0 + lane < a.B ? pa_tiles(note_span(a.spans, b0 + lane, a.rows, a.max_len).len) : 0;
+        n += t;
+        m += b0 + lane < b ? t : 0;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o), m += __shfl_xor(m, o);
+    before = pa_scalar(m);
+    return pa_scalar(n);
+}
+// Token tile i of all.
+__device__ __forceinline__ PaTile pa_tile(const PaArgs& a, int i) {
+    const int lane = threadIdx.x & 63;
+    PaTile u;
+    u.b = -1;
+    int base = 0;
+    for (int b0 = 0; b0 < a.B && u.b < 0; b0 += 64) {
+        const NoteSpan sp = b0 + lane < a.B ? note_span(a.spans, b0 + lane, a.rows, a.max_len) : NoteSpan{0, 0};
+        const int nt = pa_tiles(sp.len);
         int incl = nt;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int x = __shfl_up(incl, o);
             if (lane >= o) incl += x;
         }
-        const unsigned long long hit = want_b >= 0 ? __ballot(b0 + lane == want_b) : __ballot(base + incl > t);
-        if (u.b < 0 && hit) {
-            const int src = __ffsll((long long)hit) - 1, first = base + pa_scalar(__shfl(incl, src) - __shfl(nt, src));
+        const unsigned long long hit = __ballot(base + incl > i);
+        if (hit) {
+            const int src = __ffsll((long long)hit) - 1;
             u.b = b0 + src;
-            u.tile = want_b >= 0 ? first : t - first;  // want_b: the note's first tile among all
+            u.tile = i - base - pa_scalar(__shfl(incl, src) - __shfl(nt, src));
             u.sp = {pa_scalar(__shfl(sp.start, src)), pa_scalar(__shfl(sp.len, src))};
         }
         base += pa_scalar(__shfl(incl, 63));
     }
     return u;
 }
+struct PaRuns {
+    int steps, per, units;  // in all, of a run (the last may be shorter), runs
+    __device__ __forceinline__ PaRuns(int tiles, int nQ) {
+        steps = tiles * nQ;  // (the host has seen that it fits)
+        per = max(4, (steps - 1) / PA_UNITS + 1);
+        units = (steps + per - 1) / per;
+    }
+};
 
 struct PaPlan {
-    int max_len, nT, nQ, kind, waves, extra, least, shares, slots, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
-    float slab;
-    long long units;  // workgroups of the dK / dV sweep
+    int max_len, nT, nQ, kind, waves, extra, least, units, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
     long long kv, q, dO, part, ml, dq, dkv, bytes;
 };
 // packed_attn_bf16.hip, packed_attn_x3.hip, packed_attn_f32.hip

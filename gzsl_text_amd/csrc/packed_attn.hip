@@ -45,15 +45,10 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
         p.dq = up256(4 * chunks * d->L * d->E);
         long long tiles = (long long)d->B * cdiv(p.max_len, PA_TILE);  // at most
         if (tiles > d->rows / PA_TILE + d->B) tiles = d->rows / PA_TILE + d->B;
-        p.shares = p.nQ / 4 < 1 ? 1 : (p.nQ / 4 > 16 ? 16 : p.nQ / 4);  // (four label tiles a share at least)
-        // a slab moves (E + F) 8 bytes a token at 4 TB/s; a tile's scores take L / (scores a ns of the chip / 256) a token on one unit
-        const float rate = p.kind < 2 ? 300.f : (p.kind == 2 ? 113.f : 80.f);
-        p.slab = (d->E + d->F) * 8 / 4000.f * rate / 256.f / (float)(d->L > 0 ? d->L : 1);
-        // the number of shares is chosen on the device, at most 1024 units of more than one share
-        p.units = p.shares > 1 ? (tiles * p.shares < 1024 ? tiles * p.shares : (tiles > 1024 ? tiles : 1024)) : tiles;
-        if (p.units > 0x3FFFFFFF) return GZSL_ETOOBIG;
-        p.slots = p.shares > 1 ? (int)(p.units < 1024 ? p.units : 1024) : 0;
-        p.dkv = up256(4LL * p.slots * PA_TILE * (d->E + d->F));
+        const long long steps = tiles * p.nQ;  // at most: the runs are cut on the device
+        if (steps > 0x7FFFFF00) return GZSL_ETOOBIG;
+        p.units = (int)((steps + 3) / 4 < PA_UNITS ? (steps + 3) / 4 : PA_UNITS);
+        p.dkv = up256(8LL * p.units * PA_TILE * (d->E + d->F));
     }
     p.bytes = p.kv + p.q + p.dO + p.part + p.ml + p.dq + p.dkv;
     return 0;
@@ -63,7 +58,7 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.rows = d.rows, a.ldk = d.ldk, a.ldv = d.ldv, a.ldq = d.ldq;
     a.B = d.B, a.max_len = p.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
-    a.nLT = p.nLT, a.extra = p.extra, a.least = p.least, a.shares = p.shares, a.slots = p.slots, a.slab = p.slab;
+    a.nLT = p.nLT, a.extra = p.extra, a.least = p.least;
     char* w = (char*)work;
     a.TK = w, w += p.kv;
     a.Q = w, w += p.q;

@@ -520,7 +520,7 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
     if (TH) ds *= fmaf(-th, th, 1.f);
 }
 
-// dK / dV: workgroup = 128 tokens of one note (16 a wave, tokens on the lane axis), sweeping its share of the labels.  PaX3 takes dV
+// dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  PaX3 takes dV
 // and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a wave at two
 // waves a SIMD, and the scores a second time are a fifth of the products.
 template <class K, class G, int PART, bool CAP, bool DROP>
@@ -531,160 +531,169 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U, D = G::PL == 3 ? 2 : 4;
     constexpr bool DV = PART & 1, DK = PART & 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
-    const PaTileUnit un = pa_tile_unit(a, blockIdx.x);
-    if (un.b < 0) return;
-    const int b = un.b, len = un.sp.len;
-    const int per = (a.nQ + un.shares - 1) / un.shares, q0 = un.share * per, q1 = min(a.nQ, q0 + per);
-    const int tok0 = (un.tile * WAVES + wave) * 16, tok = tok0 + n;
-    const bool idle = tok0 >= len;  // (wave-uniform: copies and barriers only)
+    int before;
+    const PaRuns runs(pa_all_tiles(a, 0, before), a.nQ);
+    const int end = min(runs.steps, ((int)blockIdx.x + 1) * runs.per);
     const PaCap cap = pa_cap(a.cap);
-    frag kf[G::SE], vf[DK ? G::SF : 1];
-    {
-        const int c = min(tok0, (len - 1) / 16 * 16);
-        const char* img = a.TK + ((long long)b * a.nT + c / G::ROWS) * G::TOK * 1024;
+    for (int at = (int)blockIdx.x * runs.per; at < end;) {
+        const int tile = at / a.nQ, q0 = at % a.nQ, q1 = min(a.nQ, q0 + end - at);
+        at += q1 - q0;
+        const PaTile un = pa_tile(a, tile);
+        const int b = un.b, len = un.sp.len;
+        const int tok0 = (un.tile * WAVES + wave) * 16, tok = tok0 + n;
+        const bool idle = tok0 >= len;  // (wave-uniform: copies and barriers only)
+        frag kf[G::SE], vf[DK ? G::SF : 1];
+        {
+            const int c = min(tok0, (len - 1) / 16 * 16);
+            const char* img = a.TK + ((long long)b * a.nT + c / G::ROWS) * G::TOK * 1024;
 #pragma unroll
-        for (int s = 0; s < G::SE; ++s) kf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
-        if (DK)
+            for (int s = 0; s < G::SE; ++s) kf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
+            if (DK)
 #pragma unroll
-            for (int s = 0; s < G::SF; ++s) vf[s] = pa_frag<K, G::RF>(img + G::PL * G::RE * 1024, (c % G::ROWS / 16) * G::SF + s, lane);
-    }
-    f32x4 dv[DV ? G::NF : 1], dk[DK ? G::NE : 1];
-#pragma unroll
-    for (int j = 0; j < (DV ? G::NF : 1); ++j) dv[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < (DK ? G::NE : 1); ++j) dk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const char* dO = a.DO + (long long)b * a.nQ * G::OUT * 1024;
-    auto fetch = [&](int q, char* buf) {
-        pa_dma<WAVES, G::QRY>(a.Q + (long long)q * G::QRY * 1024, buf, wave, lane);
-        pa_dma<WAVES, G::OUT>(dO + (long long)q * G::OUT * 1024, buf + G::QRY * 1024, wave, lane);
-    };
-    if (q0 < q1) fetch(q0, sm);
-    pa_arrive();
-    for (int q = q0; q < q1; ++q) {
-        const char* QR = sm + ((q - q0) & 1) * BUF;
-        const char* DR = QR + G::QRY * 1024;
-        const float* aux = reinterpret_cast<const float*>(DR + (G::OUT - 1) * 1024);
-        if (q + 1 < q1) fetch(q + 1, sm + ((q - q0 + 1) & 1) * BUF);
-        if (!idle) {
-            f32x4 s[U], dp[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            frag ring[D];
-            // rows of the queries, then rows of dO
-            constexpr int NS = G::RE + (DK ? G::RF : 0);
-            auto ldr = [&](int i) {
-                return i < G::RE ? pa_frag<K, G::RE>(QR, i % U * G::SE + i / U, lane) : pa_frag<K, G::RF>(DR, (i - G::RE) % U * G::SF + (i - G::RE) / U, lane);
-            };
-            pa_fill_ring<NS>(ring, ldr);
-            pa_run_ring<NS>(ring, ldr, [&](int i, const frag& f) {
-                if (i < G::RE) s[i % U] = pa_mma(f, kf[i / U], s[i % U]);
-                else dp[(i - G::RE) % U] = pa_mma(f, vf[DK ? (i - G::RE) / U : 0], dp[(i - G::RE) % U]);
-            });
-            auto ldv = [&](int j) {
-                if constexpr (G::TRL) return pa_col_tr<K, G::SF>(DR, j, n, g);
-                else return pa_frag<K, G::NF>(DR + G::RF * 1024, j, lane);
-            };
-            auto ldk = [&](int j) {
-                if constexpr (G::TRL) return pa_col_tr<K, G::SE>(QR, j, n, g);
-                else return pa_frag<K, G::NE>(QR + G::RE * 1024, j, lane);
-            };
-            constexpr int NC = (DV ? G::NF : 0) + (DK ? G::NE : 0);
-            auto ldc = [&](int j) { return DV && j < G::NF ? ldv(j) : ldk(j - (DV ? G::NF : 0)); };
-            pa_fill_ring<NC>(ring, ldc);
-            float p[U][4], ds[U][4], y[U][4], th[U][4];
-            pa_scores<K, CAP, U, DK>(s, cap, y, th);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
-                            delta = *reinterpret_cast<const f32x4*>(aux + 2 * G::ROWS + 16 * u + 4 * g);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float keep = 1.f;
-                    if (DROP) {
-                        const uint32_t l = (uint32_t)(q * G::ROWS + 16 * u + 4 * g + r);
-                        const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
-                        keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
-                    }
-                    pa_grad<CAP, CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
-                }
-            }
-            frag pf, sf;
-            bf16x8 sl;
-            if (DV) pa_pack(p, pf);
-            if (DK) pa_pack(ds, sf);
-            if constexpr (DK && sizeof(T) == 2) pa_pack_low(ds, sl);
-            pa_run_ring<NC>(ring, ldc, [&](int j, const frag& f) {
-                if (DV && j < G::NF) {
-                    dv[DV ? j : 0] = pa_mma(f, pf, dv[DV ? j : 0]);
-                } else {
-                    const int e = DK ? j - (DV ? G::NF : 0) : 0;
-                    if constexpr (sizeof(T) == 2) dk[e] = pa_mma(f, sl, dk[e]);
-                    dk[e] = pa_mma(f, sf, dk[e]);
-                }
-            });
+                for (int s = 0; s < G::SF; ++s) vf[s] = pa_frag<K, G::RF>(img + G::PL * G::RE * 1024, (c % G::ROWS / 16) * G::SF + s, lane);
         }
+        f32x4 dv[DV ? G::NF : 1], dk[DK ? G::NE : 1];
+#pragma unroll
+        for (int j = 0; j < (DV ? G::NF : 1); ++j) dv[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < (DK ? G::NE : 1); ++j) dk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const char* dO = a.DO + (long long)b * a.nQ * G::OUT * 1024;
+        auto fetch = [&](int q, char* buf) {
+            pa_dma<WAVES, G::QRY>(a.Q + (long long)q * G::QRY * 1024, buf, wave, lane);
+            pa_dma<WAVES, G::OUT>(dO + (long long)q * G::OUT * 1024, buf + G::QRY * 1024, wave, lane);
+        };
+        fetch(q0, sm);
         pa_arrive();
+        for (int q = q0; q < q1; ++q) {
+            const char* QR = sm + ((q - q0) & 1) * BUF;
+            const char* DR = QR + G::QRY * 1024;
+            const float* aux = reinterpret_cast<const float*>(DR + (G::OUT - 1) * 1024);
+            if (q + 1 < q1) fetch(q + 1, sm + ((q - q0 + 1) & 1) * BUF);
+            if (!idle) {
+                f32x4 s[U], dp[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[u] = dp[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                frag ring[D];
+                // rows of the queries, then rows of dO
+                constexpr int NS = G::RE + (DK ? G::RF : 0);
+                auto ldr = [&](int i) {
+                    return i < G::RE ? pa_frag<K, G::RE>(QR, i % U * G::SE + i / U, lane) : pa_frag<K, G::RF>(DR, (i - G::RE) % U * G::SF + (i - G::RE) / U, lane);
+                };
+                pa_fill_ring<NS>(ring, ldr);
+                pa_run_ring<NS>(ring, ldr, [&](int i, const frag& f) {
+                    if (i < G::RE) s[i % U] = pa_mma(f, kf[i / U], s[i % U]);
+                    else dp[(i - G::RE) % U] = pa_mma(f, vf[DK ? (i - G::RE) / U : 0], dp[(i - G::RE) % U]);
+                });
+                auto ldv = [&](int j) {
+                    if constexpr (G::TRL) return pa_col_tr<K, G::SF>(DR, j, n, g);
+                    else return pa_frag<K, G::NF>(DR + G::RF * 1024, j, lane);
+                };
+                auto ldk = [&](int j) {
+                    if constexpr (G::TRL) return pa_col_tr<K, G::SE>(QR, j, n, g);
+                    else return pa_frag<K, G::NE>(QR + G::RE * 1024, j, lane);
+                };
+                constexpr int NC = (DV ? G::NF : 0) + (DK ? G::NE : 0);
+                auto ldc = [&](int j) { return DV && j < G::NF ? ldv(j) : ldk(j - (DV ? G::NF : 0)); };
+                pa_fill_ring<NC>(ring, ldc);
+                float p[U][4], ds[U][4], y[U][4], th[U][4];
+                pa_scores<K, CAP, U, DK>(s, cap, y, th);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
+                                delta = *reinterpret_cast<const f32x4*>(aux + 2 * G::ROWS + 16 * u + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float keep = 1.f;
+                        if (DROP) {
+                            const uint32_t l = (uint32_t)(q * G::ROWS + 16 * u + 4 * g + r);
+                            const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
+                            keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
+                        }
+                        pa_grad<CAP, CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
+                    }
+                }
+                frag pf, sf;
+                bf16x8 sl;
+                if (DV) pa_pack(p, pf);
+                if (DK) pa_pack(ds, sf);
+                if constexpr (DK && sizeof(T) == 2) pa_pack_low(ds, sl);
+                pa_run_ring<NC>(ring, ldc, [&](int j, const frag& f) {
+                    if (DV && j < G::NF) {
+                        dv[DV ? j : 0] = pa_mma(f, pf, dv[DV ? j : 0]);
+                    } else {
+                        const int e = DK ? j - (DV ? G::NF : 0) : 0;
+                        if constexpr (sizeof(T) == 2) dk[e] = pa_mma(f, sl, dk[e]);
+                        dk[e] = pa_mma(f, sf, dk[e]);
+                    }
+                });
+            }
+            pa_arrive();
+        }
+        if (tok < len) {
+            const long long row = un.sp.start + tok;
+            const bool slab = q1 - q0 < a.nQ;
+            int E = a.E, F = a.F;
+            asm volatile("" : "+s"(E), "+s"(F));  // (or the masks of all columns below are worked out in front of the loop, and spilled)
+            float* part = a.dkv + ((2LL * blockIdx.x + (q0 == 0)) * PA_TILE + wave * 16 + n) * (E + F);
+            if (DK)
+#pragma unroll
+                for (int j = 0; j < G::NE; ++j) {
+                    if (slab) pa_out<float>(dk[j], part, nullptr, 16 * j + 4 * g, E);
+                    else pa_out<T>(dk[j], (T*)a.dK + row * E, nullptr, 16 * j + 4 * g, E);
+                }
+            if (DV)
+#pragma unroll
+                for (int j = 0; j < G::NF; ++j) {
+                    if (slab) pa_out<float>(dv[j], part + E, nullptr, 16 * j + 4 * g, F);
+                    else pa_out<T>(dv[j], (T*)a.dV + row * F, nullptr, 16 * j + 4 * g, F);
+                }
+        }
     }
-    if (tok >= len) return;
-    const long long row = un.sp.start + tok;
-    const bool slab = un.shares > 1;
-    float* part = a.dkv + ((long long)un.unit * PA_TILE + wave * 16 + n) * (a.E + a.F);
-    if (DK)
-#pragma unroll
-        for (int j = 0; j < G::NE; ++j) {
-            if (slab) pa_out<float>(dk[j], part, nullptr, 16 * j + 4 * g, a.E);
-            else pa_out<T>(dk[j], (T*)a.dK + row * a.E, nullptr, 16 * j + 4 * g, a.E);
-        }
-    if (DV)
-#pragma unroll
-        for (int j = 0; j < G::NF; ++j) {
-            if (slab) pa_out<float>(dv[j], part + a.E, nullptr, 16 * j + 4 * g, a.F);
-            else pa_out<T>(dv[j], (T*)a.dV + row * a.F, nullptr, 16 * j + 4 * g, a.F);
-        }
 }
-// dK / dV from the label shares, in order, and zeros in the rows of no note: 16 rows a workgroup, counted from a note's first
+// dK / dV of the tiles that runs share, in order, and zeros in the rows of no note: 16 rows a workgroup, counted from a note's first
 // (blockIdx.y = B: the rows in front of the first note), a wave to a row.
 #define PA_JOIN_ROWS 16
 template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
-    const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = threadIdx.x >> 6, last = gridDim.x - 1;
-    long long start = 0, len = 0, end;  // rows [start + len, end) belong to no note
-    PaTileUnit un;
-    un.shares = 1;
-    if (b == a.B) {
-        end = note_span(a.spans, 0, a.rows, a.max_len).start;
-    } else {
-        un = pa_tile_unit(a, 0, b);
-        start = un.sp.start, len = un.sp.len;
-        end = b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows;
-    }
-    // (the last workgroup of a note takes all that is left behind it)
-    const long long stop = (int)blockIdx.x == last ? max(end - start, len) : (long long)(blockIdx.x + 1) * PA_JOIN_ROWS;
-    for (long long r = (long long)blockIdx.x * PA_JOIN_ROWS + w; r < stop; r += 4) {
-        const long long row = start + r;
-        if (r < len) {
-            if (un.shares == 1) continue;
-            const float* slab = a.dkv + ((un.tile + r / PA_TILE) * un.shares * PA_TILE + r % PA_TILE) * W;
-            if (((a.E | a.F) & 3) == 0) {
-                for (int c = 4 * lane; c < W; c += 256) {
-                    f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = pa_scalar((int)threadIdx.x >> 6);
+    const NoteSpan sp = b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0};
+    const long long end = b == a.B ? note_span(a.spans, 0, a.rows, a.max_len).start : (b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows);
+    int first;
+    const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
+    for (long long r0 = (long long)blockIdx.x * PA_JOIN_ROWS; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * PA_JOIN_ROWS) {
+        int u0 = 0, u1 = 0;  // the runs of this tile
+        if (r0 < sp.len) {
+            const int at = (first + (int)(r0 / PA_TILE)) * a.nQ;
+            u0 = at / runs.per, u1 = (at + a.nQ - 1) / runs.per;
+        }
+        for (long long r = r0 + w; r < r0 + PA_JOIN_ROWS; r += 4) {
+            const long long row = sp.start + r;
+            if (r < sp.len) {
+                if (u0 == u1) continue;
+                // parts: the first run's second slab, then the first slabs of those behind it
+                const float* slab = a.dkv + (2LL * u0 * PA_TILE + r % PA_TILE) * W;
+                const int n = u1 - u0;
+                if (((a.E | a.F) & 3) == 0) {
+                    for (int c = 4 * lane; c < W; c += 256) {
+                        f32x4 s = *reinterpret_cast<const f32x4*>(slab + (long long)PA_TILE * W + c);
 #pragma unroll 4
-                    for (int k = 0; k < un.shares; ++k) s += *reinterpret_cast<const f32x4*>(slab + (long long)k * PA_TILE * W + c);
-                    if (c < a.E) pa_out<T>(s, (T*)a.dK + row * a.E, nullptr, c, a.E);
-                    else pa_out<T>(s, (T*)a.dV + row * a.F, nullptr, c - a.E, a.F);
+                        for (int k = 1; k <= n; ++k) s += *reinterpret_cast<const f32x4*>(slab + 2LL * k * PA_TILE * W + c);
+                        if (c < a.E) pa_out<T>(s, (T*)a.dK + row * a.E, nullptr, c, a.E);
+                        else pa_out<T>(s, (T*)a.dV + row * a.F, nullptr, c - a.E, a.F);
+                    }
+                    continue;
                 }
-                continue;
-            }
-            for (int c = lane; c < W; c += 64) {
-                float s = 0.f;
+                for (int c = lane; c < W; c += 64) {
+                    float s = slab[(long long)PA_TILE * W + c];
 #pragma unroll 4
-                for (int k = 0; k < un.shares; ++k) s += slab[(long long)k * PA_TILE * W + c];
-                if (c < a.E) ((T*)a.dK)[row * a.E + c] = (T)s;
-                else ((T*)a.dV)[row * a.F + c - a.E] = (T)s;
+                    for (int k = 1; k <= n; ++k) s += slab[2LL * k * PA_TILE * W + c];
+                    if (c < a.E) ((T*)a.dK)[row * a.E + c] = (T)s;
+                    else ((T*)a.dV)[row * a.F + c - a.E] = (T)s;
+                }
+            } else if (row < end) {
+                for (int c = lane; c < a.E; c += 64) ((T*)a.dK)[row * a.E + c] = (T)0.f;
+                for (int c = lane; c < a.F; c += 64) ((T*)a.dV)[row * a.F + c] = (T)0.f;
             }
-        } else if (row < end) {
-            for (int c = lane; c < a.E; c += 64) ((T*)a.dK)[row * a.E + c] = (T)0.f;
-            for (int c = lane; c < a.F; c += 64) ((T*)a.dV)[row * a.F + c] = (T)0.f;
         }
     }
 }
@@ -842,10 +851,10 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     hipLaunchKernelGGL((pa_pack_do_kernel<K, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
     if (p.units > 0) {
         if constexpr (G::PL == 3) {
-            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 1, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
-            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 2, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 1, CAP, DROP>), dim3(p.units), dim3(PA_TILE * 4), lds, st, a);
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 2, CAP, DROP>), dim3(p.units), dim3(PA_TILE * 4), lds, st, a);
         } else {
-            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 3, CAP, DROP>), dim3((unsigned)p.units), dim3(PA_TILE * 4), lds, st, a);
+            hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 3, CAP, DROP>), dim3(p.units), dim3(PA_TILE * 4), lds, st, a);
         }
     }
     hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, PA_JOIN_ROWS) : 1, a.B + 1), dim3(256), 0, st, a);
