@@ -244,6 +244,7 @@ struct PaArgs {
     float cap;
     uint32_t l_offset, L_total, seed, thresh;
     float scale;
+    int join_rows;                    // rows of a workgroup of pa_kv_finish_kernel
     int nLT, extra, least;            // label workgroups of a note; token chunks beyond one a note (0: notes are not cut), their tokens at least
     // workspace
     char *TK, *Q, *DO;  // images: token tiles [B][nT], queries [nQ], dO [B][nQ]
@@ -323,11 +324,12 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
     return u;
 }
 // dK / dV: the steps of the sweep, token tile by token tile (PA_TILE tokens x the label tiles), in PA_UNITS equal runs, one for each
-// compute unit (less where a run would be under four steps): every compute unit works for the same time, and only the tiles at a run's
+// compute unit (less where a run would be under PA_RUN steps): every compute unit works for the same time, and only the tiles at a run's
 // two ends are shared and go through slabs (2 u for one that the run begins inside of, 2 u + 1 for the one that it ends in).  With
 // equal parts of a tile instead, as many as a cost rule found best, 17404 tokens x 1999 labels of 200 bf16 took 99 us, so 88; x 9000
 // labels, with their slabs' join, 415 and 380.
 #define PA_UNITS 256
+#define PA_RUN 2  // steps of a run, at least (of 4: 60 us against 35 of its two launches for 1000 tokens x 428 labels, fp32)
 struct PaTile {
     int b, tile;  // note, token tile in it
     NoteSpan sp;
@@ -377,7 +379,7 @@ struct PaRuns {
     int steps, per, units;  // in all, of a run (the last may be shorter), runs
     __device__ __forceinline__ PaRuns(int tiles, int nQ) {
         steps = tiles * nQ;  // (the host has seen that it fits)
-        per = max(4, (steps - 1) / PA_UNITS + 1);
+        per = max(PA_RUN, (steps - 1) / PA_UNITS + 1);
         units = (steps + per - 1) / per;
     }
 };

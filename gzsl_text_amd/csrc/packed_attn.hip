@@ -31,7 +31,10 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     p.waves = !fits && ((p.kind == 3 && !backward) || (p.kind < 2 && (long long)d->B * cdiv(d->L, 128) < 512)) ? 4 : 8;
     p.nLT = cdiv(d->L, 16 * p.waves);
     const long long wgs = (long long)d->B * p.nLT;
-    p.least = fits ? 128 : 256;  // tokens of a chunk that pay for its own start and its part in the join
+    // tokens of a chunk that pay for its own start and its part in the join (fp32: 1500 tokens x 32 labels of 200, 28 + 6 us at 128, 25 + 7 at
+    // 96, 20 + 6 at 64, but bf16 of 31, 21 + 8, 19 + 9, 19 + 9; dQ of 1000 tokens x 428 labels 38 us at 256, 25 at 128, 18 at 64; the
+    // forward 27 us at 256, 18 at 128, 15 at 64, but 319 x 5380 25 us at 128 and 29 at 64)
+    p.least = backward ? 64 : (fits ? 96 : 128);
     p.extra = wgs > 0 && wgs < 256 && p.max_len > p.least ? cdiv(p.waves == 4 && !backward ? 512 : 256, p.nLT) : 0;
     if (p.extra > (long long)d->B * (p.max_len / p.least + 1)) p.extra = d->B * (p.max_len / p.least + 1);
     const long long chunks = d->B + p.extra;
@@ -47,7 +50,7 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
         if (tiles > d->rows / PA_TILE + d->B) tiles = d->rows / PA_TILE + d->B;
         const long long steps = tiles * p.nQ;  // at most: the runs are cut on the device
         if (steps > 0x7FFFFF00) return GZSL_ETOOBIG;
-        p.units = (int)((steps + 3) / 4 < PA_UNITS ? (steps + 3) / 4 : PA_UNITS);
+        p.units = (int)((steps + PA_RUN - 1) / PA_RUN < PA_UNITS ? (steps + PA_RUN - 1) / PA_RUN : PA_UNITS);
         p.dkv = up256(8LL * p.units * PA_TILE * (d->E + d->F));
     }
     p.bytes = p.kv + p.q + p.dO + p.part + p.ml + p.dq + p.dkv;
@@ -59,6 +62,9 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.B = d.B, a.max_len = p.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
     a.nLT = p.nLT, a.extra = p.extra, a.least = p.least;
+    // few rows: one a wave, for the time of one row's parts to come in (1000 tokens x 428 labels: 31 us with four a wave, 12 so); many: four,
+    // to share out what a workgroup has to find out first (17404 x 1999: 21 us with one a wave, 19 so)
+    a.join_rows = (long long)p.max_len * d.B <= 16384 ? 4 : 16;
     char* w = (char*)work;
     a.TK = w, w += p.kv;
     a.Q = w, w += p.q;

@@ -30,24 +30,42 @@ __device__ __forceinline__ void pa_put(char* img, int i, const typename K::frag&
     }
 }
 // ------------------------------------------------------------------------------------------------------------- pre-pass
-// A tile's rows into LDS, zeros past nrows and past W (row stride P elements).
+// A tile's rows into LDS, zeros past nrows (at least 1) and past W (row stride P elements).  Addresses are clamped, not branched around,
+// and loaded in batches: a batch is on its way together.
 template <typename T, int ROWS, int P>
 __device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld, int row0, int nrows, int W, int tid) {
     if (((uintptr_t)src & 15) == 0 && ld % (16 / sizeof(T)) == 0 && W % (16 / sizeof(T)) == 0) {
-        constexpr int V = 16 / sizeof(T), C = P / V;
+        constexpr int V = 16 / sizeof(T), C = P / V, N = (ROWS * C + 255) / 256;
         typedef T vec __attribute__((ext_vector_type(V)));
-        for (int c = tid; c < ROWS * C; c += 256) {
-            const int r = c / C, e = c % C * V;
-            vec v;
+        vec v[N];
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = (T)0.f;
-            if (row0 + r < nrows && e < W) v = *reinterpret_cast<const vec*>(src + (long long)(row0 + r) * ld + e);
-            *reinterpret_cast<vec*>(&sh[r][e]) = v;
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 256 * i;
+            v[i] = *reinterpret_cast<const vec*>(src + (long long)min(row0 + c / C, nrows - 1) * ld + min(c % C * V, W - V));
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 256 * i, r = c / C, e = c % C * V;
+            if (!(row0 + r < nrows && e < W))
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] = (T)0.f;
+            if (c < ROWS * C) *reinterpret_cast<vec*>(&sh[r][e]) = v[i];
         }
     } else {
-        for (int c = tid; c < ROWS * P; c += 256) {
-            const int r = c / P, e = c % P;
-            sh[r][e] = row0 + r < nrows && e < W ? src[(long long)(row0 + r) * ld + e] : (T)0.f;
+        constexpr int N = (ROWS * P + 255) / 256, D = 8;
+#pragma unroll 1
+        for (int i0 = 0; i0 < N; i0 += D) {
+            T v[D];
+#pragma unroll
+            for (int i = 0; i < D; ++i) {
+                const int c = tid + 256 * (i0 + i);
+                v[i] = src[(long long)min(row0 + c / P, nrows - 1) * ld + min(c % P, W - 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < D; ++i) {
+                const int c = tid + 256 * (i0 + i), r = c / P, e = c % P;
+                if (c < ROWS * P) sh[r][e] = row0 + r < nrows && e < W ? v[i] : (T)0.f;
+            }
         }
     }
 }
@@ -128,8 +146,27 @@ __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
     if (l < a.L) {
         const T* y = (const T*)a.cO + row * a.F;
         const bf16* low = sizeof(T) == 2 && a.crest ? reinterpret_cast<const bf16*>(a.crest + 2LL * a.B * a.L) + row * a.F : nullptr;
+        constexpr int V = 16 / (int)sizeof(T), N = (208 / V + TPR - 1) / TPR;  // (F <= 208)
+        typedef T vec __attribute__((ext_vector_type(V)));
+        if (a.F % V == 0 && (((uintptr_t)y | (uintptr_t)low) & 15) == 0) {
+            vec v[N], w[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int f = min((tid % TPR + i * TPR) * V, a.F - V);
+                v[i] = *reinterpret_cast<const vec*>(y + f);
+                if (sizeof(T) == 2) w[i] = low ? *reinterpret_cast<const vec*>(low + f) : v[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int f = (tid % TPR + i * TPR) * V;
+                if (f < a.F)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) s = fmaf((float)sf[r][f + k], (float)v[i][k] + (low ? (float)w[i][k] : 0.f), s);
+            }
+        } else {
 #pragma unroll 4
-        for (int f = tid % TPR; f < a.F; f += TPR) s = fmaf((float)sf[r][f], (float)y[f] + (low ? (float)low[f] : 0.f), s);
+            for (int f = tid % TPR; f < a.F; f += TPR) s = fmaf((float)sf[r][f], (float)y[f] + (low ? (float)low[f] : 0.f), s);
+        }
     }
 #pragma unroll
     for (int o = 1; o < TPR; o <<= 1) s += __shfl_xor(s, o);
@@ -650,9 +687,8 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
         }
     }
 }
-// dK / dV of the tiles that runs share, in order, and zeros in the rows of no note: 16 rows a workgroup, counted from a note's first
+// dK / dV of the tiles that runs share, in order, and zeros in the rows of no note: 4 or 16 rows a workgroup, counted from a note's first
 // (blockIdx.y = B: the rows in front of the first note), a wave to a row.
-#define PA_JOIN_ROWS 16
 template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = pa_scalar((int)threadIdx.x >> 6);
@@ -660,13 +696,13 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const long long end = b == a.B ? note_span(a.spans, 0, a.rows, a.max_len).start : (b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows);
     int first;
     const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
-    for (long long r0 = (long long)blockIdx.x * PA_JOIN_ROWS; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * PA_JOIN_ROWS) {
+    for (long long r0 = (long long)blockIdx.x * a.join_rows; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * a.join_rows) {
         int u0 = 0, u1 = 0;  // the runs of this tile
         if (r0 < sp.len) {
             const int at = (first + (int)(r0 / PA_TILE)) * a.nQ;
             u0 = at / runs.per, u1 = (at + a.nQ - 1) / runs.per;
         }
-        for (long long r = r0 + w; r < r0 + PA_JOIN_ROWS; r += 4) {
+        for (long long r = r0 + w; r < r0 + a.join_rows; r += 4) {
             const long long row = sp.start + r;
             if (r < sp.len) {
                 if (u0 == u1) continue;
@@ -674,21 +710,33 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
                 const float* slab = a.dkv + (2LL * u0 * PA_TILE + r % PA_TILE) * W;
                 const int n = u1 - u0;
                 if (((a.E | a.F) & 3) == 0) {
-                    for (int c = 4 * lane; c < W; c += 256) {
-                        f32x4 s = *reinterpret_cast<const f32x4*>(slab + (long long)PA_TILE * W + c);
+                    f32x4 s[2];  // E + F <= 416: all of the row on its way at once
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) s[j] = *reinterpret_cast<const f32x4*>(slab + (long long)PA_TILE * W + min(4 * lane + 256 * j, W - 4));
 #pragma unroll 4
-                        for (int k = 1; k <= n; ++k) s += *reinterpret_cast<const f32x4*>(slab + 2LL * k * PA_TILE * W + c);
-                        if (c < a.E) pa_out<T>(s, (T*)a.dK + row * a.E, nullptr, c, a.E);
-                        else pa_out<T>(s, (T*)a.dV + row * a.F, nullptr, c - a.E, a.F);
+                    for (int k = 1; k <= n; ++k)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) s[j] += *reinterpret_cast<const f32x4*>(slab + 2LL * k * PA_TILE * W + min(4 * lane + 256 * j, W - 4));
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int c = 4 * lane + 256 * j;
+                        if (c < a.E) pa_out<T>(s[j], (T*)a.dK + row * a.E, nullptr, c, a.E);
+                        else if (c < W) pa_out<T>(s[j], (T*)a.dV + row * a.F, nullptr, c - a.E, a.F);
                     }
                     continue;
                 }
-                for (int c = lane; c < W; c += 64) {
-                    float s = slab[(long long)PA_TILE * W + c];
+                float s[7];
+#pragma unroll
+                for (int j = 0; j < 7; ++j) s[j] = slab[(long long)PA_TILE * W + min(lane + 64 * j, W - 1)];
 #pragma unroll 4
-                    for (int k = 1; k <= n; ++k) s += slab[2LL * k * PA_TILE * W + c];
-                    if (c < a.E) ((T*)a.dK)[row * a.E + c] = (T)s;
-                    else ((T*)a.dV)[row * a.F + c - a.E] = (T)s;
+                for (int k = 1; k <= n; ++k)
+#pragma unroll
+                    for (int j = 0; j < 7; ++j) s[j] += slab[2LL * k * PA_TILE * W + min(lane + 64 * j, W - 1)];
+#pragma unroll
+                for (int j = 0; j < 7; ++j) {
+                    const int c = lane + 64 * j;
+                    if (c < a.E) ((T*)a.dK)[row * a.E + c] = (T)s[j];
+                    else if (c < W) ((T*)a.dV)[row * a.F + c - a.E] = (T)s[j];
                 }
             } else if (row < end) {
                 for (int c = lane; c < a.E; c += 64) ((T*)a.dK)[row * a.E + c] = (T)0.f;
@@ -811,15 +859,32 @@ __global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
 #pragma unroll
     for (int j = 0; j < G::NE; ++j) pa_out<float>(dq[j], out, nullptr, 16 * j + 4 * g, a.E);
 }
-// dQ = sum of the slabs, in order.
-template <typename T, int ROWS>
-__global__ __launch_bounds__(256) void pa_q_join_kernel(PaArgs a) {
+// dQ = sum of the slabs, in a fixed order: a thread an element, or (G > 1, many slabs of few elements: 56 labels of 31, 258 slabs, 22 us
+// with one thread, 6 so) G waves share the slabs of 64 elements and join in LDS.
+template <typename T, int ROWS, int G>
+__global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_q_join_kernel(PaArgs a) {
+    __shared__ float sh[G][64];
     const int all = pa_unit<ROWS>(a, 0).all;
     const long long n = (long long)a.L * a.E;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        float s = 0.f;
+    if constexpr (G == 1) {
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+            float s = 0.f;
 #pragma unroll 4
-        for (int k = 0; k < all; ++k) s += a.dq[k * n + i];
+            for (int k = 0; k < all; ++k) s += a.dq[k * n + i];
+            ((T*)a.dQ)[i] = (T)s;
+        }
+    } else {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, per = (all + G - 1) / G;
+        const long long i = (long long)blockIdx.x * 64 + lane;
+        float s = 0.f;
+        if (i < n)
+#pragma unroll 8
+            for (int k = w * per; k < min(all, (w + 1) * per); ++k) s += a.dq[k * n + i];
+        sh[w][lane] = s;
+        __syncthreads();
+        if (w > 0 || i >= n) return;
+#pragma unroll
+        for (int k = 1; k < G; ++k) s += sh[k][lane];
         ((T*)a.dQ)[i] = (T)s;
     }
 }
@@ -857,10 +922,11 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
             hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 3, CAP, DROP>), dim3(p.units), dim3(PA_TILE * 4), lds, st, a);
         }
     }
-    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, PA_JOIN_ROWS) : 1, a.B + 1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, a.join_rows) : 1, a.B + 1), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_bwd_q_kernel<K, G, W, H, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * H * 64), 2 * H * G::TOK * 1024, st, a);
     const long long n = (long long)a.L * a.E;
-    hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS>), dim3((unsigned)(n < 256 * 4096 ? cdiv((long)n, 256) : 4096)), dim3(256), 0, st, a);
+    if (n <= 64 * 512 && a.B + a.extra > 32) hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS, 16>), dim3((unsigned)cdiv((long)n, 64)), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS, 1>), dim3((unsigned)(n < 256 * 4096 ? cdiv((long)n, 256) : 4096)), dim3(256), 0, st, a);
     GZSL_CHECK_LAUNCH();
     return 0;
 }
