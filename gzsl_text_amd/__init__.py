@@ -6,6 +6,7 @@ Layout:
   ops_hip.py   tensor-level ops, each one or two kernel launches
   engine.py    forward/backward orchestration of the base feature extractor
   gan_engine.py  WGAN-GP critic / generator iterations
+  packed.py    span tables of packed notes (operators: ops_hip.py, torch.ops.gzsl)
   parallel.py  label-dimension sharding over RCCL (one process per GPU)
   modules/     nn.Module mirrors of the reference's modules/ package (same classes, ctor signatures, state-dict keys)
 """

@@ -96,7 +96,8 @@ __device__ __forceinline__ void pa_emit(typename K::T (*sh)[P], char* img, int t
         pa_put<K, N>(img, i, pa_cut<K, G>(x), lane);
     }
 }
-// Blocks [0, B nT): a token tile (keys, values); then nQ blocks of queries.
+// Blocks [0, B nT): a token tile (keys, values); then nQ blocks of queries.  Memory-bound: reads each operand once, writes its image
+// (17404 tokens of 200 + 200 bf16: 8 us).
 template <class K, class G, bool BWD>
 __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
     typedef typename K::T T;
@@ -130,7 +131,8 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
 }
 // Backward: dO images of (note, label tile); behind the fragments, for each label, off and scale of its weights
 // P = exp2(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; scale 0 past the
-// last label) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.
+// last label) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.  Memory-bound
+// (16 x 1999 rows of 200 bf16: 67 MB in 14 us).
 template <class K, class G>
 __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
     typedef typename K::T T;
@@ -239,7 +241,8 @@ __device__ __forceinline__ void pa_fwd_begin(PaFwdState<K, G>& w, const PaArgs& 
 // KR: row fragments of the keys, VC: column fragments of the values; t0: the tile's first token, LAST: it may end behind the note (left
 // tokens are the note's).
 template <class K, class G, bool CAP, bool DROP, bool LAST>
-__device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left, int lane) {
+__device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left,
+                                            int lane) {
     typedef typename K::frag frag;
     constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
     const int g = lane >> 4;
@@ -327,7 +330,12 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
     for (int j = 0; j < G::NF; ++j) pa_out<T>(w.acc[j] * inv, out, low, 16 * j + 4 * g, a.F);
 }
 
-// Workgroup = WAVES x 16 labels of one note (or of one chunk of it), token tiles from the pre-pass's images.
+// Workgroup = WAVES x 16 labels of one note (or of one chunk of it), token tiles from the pre-pass's images.  An image is read by all
+// label workgroups of a note and comes from L2; a wave's 16 queries and its output tile stay in registers.  Bound by the matrix pipe
+// and, a third of the time in addition, by the softmax's vector instructions, two waves' of which overlap with other waves' matrix
+// instructions only in part: 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 840 TFLOP/s of the padded products (1255 is
+// what a large library product reaches); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
+// reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
 template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
@@ -382,7 +390,9 @@ __device__ __forceinline__ void pa_row_load(const T* row, int e0, int W, bool wi
 
 // The same for at most WAVES x 16 labels (one label workgroup a note or chunk): every token tile is then read by one workgroup
 // alone, which cuts its fragments itself: each wave loads the elements of its share of the next tile's fragments while it works on the
-// current one.  No images and one launch less.
+// current one.  No images and one launch less: 2 notes of 59 tokens in all x 70 labels 16 -> 13 us, 40003 tokens x 50 labels 58 -> 40.
+// With more labels every label workgroup would cut the fragments again.  What bounds it is latency: five tiles a workgroup at 256
+// workgroups (24 us for 48 MB); a second tile on its way changed nothing.
 template <class K, class G, int WAVES, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) {
     typedef typename K::T T;
@@ -461,7 +471,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) 
     pa_fwd_end(w, a, un, l0 + n, lane);
 }
 // Joins the chunks of a (note, label), in order: a workgroup of 4 rows of one wave each, or (G > 1, few rows over many chunks) of one
-// row whose chunks G waves share and join in LDS.  A lane weighs one chunk; a row's F values lie over the lanes.
+// row whose chunks G waves share and join in LDS.  A lane weighs one chunk; a row's F values lie over the lanes.  Latency-bound (50 rows
+// of 250 chunks: 9.6 us, 12.7 with the parts loaded behind the weights).
 template <typename T, int ROWS, int G>
 __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a) {
     __shared__ float so[G == 1 ? 4 : G][256], ss[G == 1 ? 4 : G], sM[G];
@@ -557,9 +568,11 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
     if (TH) ds *= fmaf(-th, th, 1.f);
 }
 
-// dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  PaX3 takes dV
-// and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a wave at two
-// waves a SIMD, and the scores a second time are a fifth of the products.
+// dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  Matrix pipe
+// and LDS reads both near their limit (PaBF, E, F = 200: 67 matrix instructions of 16 cycles and 55 KB a wave and step; one workgroup a
+// compute unit by its LDS): 17404 tokens x 1999 labels 88 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
+// PaX3 takes dV and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a
+// wave at two waves a SIMD, and the scores a second time are a fifth of the products.
 template <class K, class G, int PART, bool CAP, bool DROP>
 __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     typedef typename K::T T;
@@ -693,7 +706,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = pa_scalar((int)threadIdx.x >> 6);
     const NoteSpan sp = b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0};
-    const long long end = b == a.B ? note_span(a.spans, 0, a.rows, a.max_len).start : (b + 1 < a.B ? note_span(a.spans, b + 1, a.rows, a.max_len).start : a.rows);
+    const int next = b == a.B ? 0 : b + 1;  // the note that the gap behind this one ends at
+    const long long end = next < a.B ? note_span(a.spans, next, a.rows, a.max_len).start : a.rows;
     int first;
     const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
     for (long long r0 = (long long)blockIdx.x * a.join_rows; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * a.join_rows) {
@@ -747,7 +761,8 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
 }
 
 // dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.  H = 2: twice the
-// waves, which take turns at the token tiles and add up in LDS (few labels: half the way through the longest note).
+// waves, which take turns at the token tiles and add up in LDS (few labels: half the way through the longest note).  Bound as dK / dV is
+// (17404 tokens x 1999 labels of 200 bf16 70 us, 7339 x 9000 of 100 and 200 fp32 325).
 template <class K, class G, int WAVES, int H, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     typedef typename K::T T;
