@@ -26,7 +26,8 @@
 // them 16 bytes a lane at one address plus constants, free of bank conflicts without padding; odd widths, row pitches, alignment
 // and whatever lies between the notes (NaN included) end in the pre-pass.  The backward
 // takes the column fragments of bf16 pieces out of the row fragments with ds_read_b64_tr_b16, PaX3 all of them for lack of LDS, PaBF
-// those of the keys (dQ 87 -> 78 us at 17404 tokens x 1999 labels of 200; of the labels' tiles it was no gain).
+// those of the keys (dQ 87 -> 78 us at 17404 tokens x 1999 labels of 200; of the labels' tiles it was no gain).  A tenth to a third of
+// their LDS cycles are bank conflicts; lanes exchanged in the images to avoid them cost the 16-byte reads more (dK / dV 88 -> 111 us).
 #pragma once
 #include "packed.h"
 #include "rng.h"

@@ -332,9 +332,9 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
 
 // Workgroup = WAVES x 16 labels of one note (or of one chunk of it), token tiles from the pre-pass's images.  An image is read by all
 // label workgroups of a note and comes from L2; a wave's 16 queries and its output tile stay in registers.  Bound by the matrix pipe
-// and, a third of the time in addition, by the softmax's vector instructions, two waves' of which overlap with other waves' matrix
-// instructions only in part: 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 840 TFLOP/s of the padded products (1255 is
-// what a large library product reaches); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
+// (bf16 48 % busy, PaX3 70 %) and the softmax's vector instructions, which overlap with other waves' matrix instructions only in part:
+// 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 940 TFLOP/s of the padded products (1255 is what a large library product
+// reaches, whose clock is as low); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
 // reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
 template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
@@ -568,9 +568,10 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
     if (TH) ds *= fmaf(-th, th, 1.f);
 }
 
-// dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  Matrix pipe
-// and LDS reads both near their limit (PaBF, E, F = 200: 67 matrix instructions of 16 cycles and 55 KB a wave and step; one workgroup a
-// compute unit by its LDS): 17404 tokens x 1999 labels 88 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
+// dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  One
+// workgroup a compute unit by its LDS and registers, so two waves a SIMD: what they wait for one another, for fragments and at the
+// barrier of a step is what is left (PaBF, E, F = 200: matrix pipe 48 % busy, LDS 44 %; PaX3 63 and 45 to 53 %).  17404 tokens x 1999
+// labels bf16 88 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
 // PaX3 takes dV and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a
 // wave at two waves a SIMD, and the scores a second time are a fifth of the products.
 template <class K, class G, int PART, bool CAP, bool DROP>
