@@ -337,9 +337,9 @@ struct PaTile {
 };
 __device__ __forceinline__ int pa_tiles(int len) { return (int)(((uint32_t)len + PA_TILE - 1) / PA_TILE); }
 // Token tiles of all notes, and of those in front of note b.
-__device__ __forceinline__ int pa_all_tiles(const PaArgs& a, int b, int& before) {
+__device__ __forceinline__ long long pa_all_tiles(const PaArgs& a, int b, long long& before) {
     const int lane = threadIdx.x & 63;
-    int n = 0, m = 0;
+    long long n = 0, m = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         const int t = b0 + lane < a.B ? pa_tiles(note_span(a.spans, b0 + lane, a.rows, a.max_len).len) : 0;
         n += t;
@@ -378,8 +378,9 @@ __device__ __forceinline__ PaTile pa_tile(const PaArgs& a, int i) {
 }
 struct PaRuns {
     int steps, per, units;  // in all, of a run (the last may be shorter), runs
-    __device__ __forceinline__ PaRuns(int tiles, int nQ) {
-        steps = tiles * nQ;  // (the host has seen that it fits)
+    __device__ __forceinline__ PaRuns(long long tiles, int nQ) {
+        // The host has seen that the steps of disjoint notes fit; of a table that is not, nothing is done where they do not.
+        steps = tiles <= 0x7FFFFF00 / nQ ? (int)tiles * nQ : 0;
         per = max(PA_RUN, (steps - 1) / PA_UNITS + 1);
         units = (steps + per - 1) / per;
     }

@@ -50,7 +50,9 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
         if (tiles > d->rows / PA_TILE + d->B) tiles = d->rows / PA_TILE + d->B;
         const long long steps = tiles * p.nQ;  // at most: the runs are cut on the device
         if (steps > 0x7FFFFF00) return GZSL_ETOOBIG;
-        p.units = (int)((steps + PA_RUN - 1) / PA_RUN < PA_UNITS ? (steps + PA_RUN - 1) / PA_RUN : PA_UNITS);
+        // (of notes that overlap there may be more, as many as would fill B times max_len)
+        const long long most = (long long)d->B * cdiv(p.max_len, PA_TILE);
+        p.units = most >= PA_UNITS * PA_RUN || most * p.nQ >= PA_UNITS * PA_RUN ? PA_UNITS : (int)((most * p.nQ + PA_RUN - 1) / PA_RUN);
         p.dkv = up256(8LL * p.units * PA_TILE * (d->E + d->F));
     }
     p.bytes = p.kv + p.q + p.dO + p.part + p.ml + p.dq + p.dkv;

@@ -582,7 +582,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U, D = G::PL == 3 ? 2 : 4;
     constexpr bool DV = PART & 1, DK = PART & 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
-    int before;
+    long long before;
     const PaRuns runs(pa_all_tiles(a, 0, before), a.nQ);
     const int end = min(runs.steps, ((int)blockIdx.x + 1) * runs.per);
     const PaCap cap = pa_cap(a.cap);
@@ -709,12 +709,12 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const NoteSpan sp = b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0};
     const int next = b == a.B ? 0 : b + 1;  // the note that the gap behind this one ends at
     const long long end = next < a.B ? note_span(a.spans, next, a.rows, a.max_len).start : a.rows;
-    int first;
+    long long first;
     const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
     for (long long r0 = (long long)blockIdx.x * a.join_rows; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * a.join_rows) {
         int u0 = 0, u1 = 0;  // the runs of this tile
-        if (r0 < sp.len) {
-            const int at = (first + (int)(r0 / PA_TILE)) * a.nQ;
+        if (r0 < sp.len && runs.steps > 0) {
+            const int at = (int)(first + r0 / PA_TILE) * a.nQ;
             u0 = at / runs.per, u1 = (at + a.nQ - 1) / runs.per;
         }
         for (long long r = r0 + w; r < r0 + a.join_rows; r += 4) {

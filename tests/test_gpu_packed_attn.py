@@ -316,3 +316,18 @@ def test_a_wrong_table_is_clamped_to_the_rows(ops):
     O, lse, rest = ops.attn_packed_fwd(k, v, q, bad, 64)
     ref = attn_ref(k, v, q, [(0, 20), (30, 10), (40, 0), (3, 0)])
     within(O, ref['O'], 'O')
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+def test_notes_that_overlap_stay_inside_the_workspace(ops, dtype):
+    """A table of notes over the same rows: the forward and dQ, sums of whole notes, are right; dK and dV hold one note's or another's
+    part (the table has to be disjoint for them), and nothing around them is touched."""
+    k, v, q, do, _, _, _ = make([300], 40, 24, 70, dtype, seed=3)
+    spans = torch.tensor([[0, 300]] * 40, dtype=torch.int64, device=DEV)
+    do = do.expand(40, -1, -1).contiguous()
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, 300)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, 300)
+    ref = attn_ref(k, v, q, [(0, 300)] * 40, dout=do)
+    within(O, ref['O'], 'O')
+    within(dq, ref['dQ'], 'dQ')
+    assert dk.shape == k.shape and dv.shape == v.shape
