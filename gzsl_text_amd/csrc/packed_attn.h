@@ -11,9 +11,12 @@
 //          the six cross terms of weight >= 2^-16 of them (what is dropped is below 2^-24 of the product), each the same MFMA:
 //          6 x 16 cycles per 32 k against 8 x 32 of the fp32 MFMA.
 //   PaF32  fp32 tensors, E > 112 (three pieces of both tiles no longer fit LDS twice): v_mfma_f32_16x16x4_f32, exact.
-// Sums are fp32 in all of them.  P is rounded to bf16 for bf16 tensors' products (half a step of 2^-8, as the inputs' own
-// rounding); the softmax sum uses P before that.  dS sums to zero over a row, so its products cancel: as one bf16 piece it made
-// dK and dQ 1.6 times as far off as rounded results are, so it goes in two (16 bits, one more product).
+// Sums are fp32 in all of them.  For bf16 tensors a scoring call rounds P to bf16 for its product (half a step of 2^-8, as the inputs' own
+// rounding; O is 1.0 to 1.3 times as far off as a rounded exact result); the softmax sum uses P before that.  A forward that a backward
+// follows and the backward take P and dS in two bf16 pieces (16 bits, one more product each): dS sums to zero over a row, so its
+// products cancel, and delta = <dO, O> has to be that of the same P.  With one piece of each, dK and dQ were up to 2.4 times as far off
+// as rounded exact results, dV 1.4 times; so all are within a hundredth of them (17404 tokens x 1999 labels of 200: forward 50 -> 60
+// us, dK / dV 88 -> 98).
 //
 // Everything is moved as FRAGMENTS: 1 KB, 16 bytes a lane, exactly one operand of one matrix instruction (eight bf16 of a lane;
 // four fp32, which feed four instructions).  With n = lane & 15, g = lane >> 4:
@@ -327,8 +330,8 @@ __device__ __forceinline__ PaUnit pa_unit(const PaArgs& a, int ci, int want_b = 
 // dK / dV: the steps of the sweep, token tile by token tile (PA_TILE tokens x the label tiles), in PA_UNITS equal runs, one for each
 // compute unit (less where a run would be under PA_RUN steps): every compute unit works for the same time, and only the tiles at a run's
 // two ends are shared and go through slabs (2 u for one that the run begins inside of, 2 u + 1 for the one that it ends in).  With
-// equal parts of a tile instead, as many as a cost rule found best, 17404 tokens x 1999 labels of 200 bf16 took 99 us, so 88; x 9000
-// labels, with their slabs' join, 415 and 380.
+// equal parts of a tile instead, as many as a cost rule found best, 17404 tokens x 1999 labels of 200 bf16 (weights in one piece) took
+// 99 us, so 88; x 9000 labels, with their slabs' join, 415 and 380.
 #define PA_UNITS 256
 #define PA_RUN 2  // steps of a run, at least (of 4: 60 us against 35 of its two launches for 1000 tokens x 428 labels, fp32)
 struct PaTile {

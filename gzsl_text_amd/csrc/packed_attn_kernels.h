@@ -239,12 +239,12 @@ __device__ __forceinline__ void pa_fwd_begin(PaFwdState<K, G>& w, const PaArgs& 
     w.m = w.fixed ? 0.f : -INFINITY, w.sum = 0.f;
 }
 // KR: row fragments of the keys, VC: column fragments of the values; t0: the tile's first token, LAST: it may end behind the note (left
-// tokens are the note's).
-template <class K, class G, bool CAP, bool DROP, bool LAST>
+// tokens are the note's); TWO: the weights go in two bf16 pieces.
+template <class K, class G, bool CAP, bool DROP, bool TWO, bool LAST>
 __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left,
                                             int lane) {
     typedef typename K::frag frag;
-    constexpr int U = G::U, D = G::PL == 3 ? 2 : 4;
+    constexpr int U = G::U, D = G::PL == 3 ? 2 : (TWO && DROP ? 3 : 4);
     const int g = lane >> 4;
     f32x4 s[U];
 #pragma unroll
@@ -287,6 +287,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
             for (int r = 0; r < 4; ++r) y[u][r] = CAP ? y[u][r] - mi : fmaf(y[u][r], PA_LOG2E, -mi);
     }
     frag pf;
+    bf16x8 pl;
     {
         float p[U][4];
 #pragma unroll
@@ -298,8 +299,12 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
                 if (DROP) p[u][r] = gz_u32(w.key, (uint32_t)(t0 + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
             }
         pa_pack(p, pf);
+        if constexpr (TWO) pa_pack_low(p, pl);
     }
-    pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) { w.acc[j] = pa_mma(f, pf, w.acc[j]); });
+    pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) {
+        if constexpr (TWO) w.acc[j] = pa_mma(f, pl, w.acc[j]);
+        w.acc[j] = pa_mma(f, pf, w.acc[j]);
+    });
 }
 // Output rows, or a chunk's part of them.
 template <class K, class G>
@@ -336,7 +341,7 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
 // 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 940 TFLOP/s of the padded products (1255 is what a large library product
 // reaches, whose clock is as low); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
 // reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
-template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
+template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP, bool TWO>
 __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15;
@@ -362,7 +367,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     auto step = [&](int t, auto last) {
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
         if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)(t + 1) * G::FWD * 1024, sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
-        if (!idle) pa_fwd_tile<K, G, CAP, DROP, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, TWO, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         pa_arrive();
     };
     for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
@@ -393,7 +398,7 @@ __device__ __forceinline__ void pa_row_load(const T* row, int e0, int W, bool wi
 // current one.  No images and one launch less: 2 notes of 59 tokens in all x 70 labels 16 -> 13 us, 40003 tokens x 50 labels 58 -> 40.
 // With more labels every label workgroup would cut the fragments again.  What bounds it is latency: five tiles a workgroup at 256
 // workgroups (24 us for 48 MB); a second tile on its way changed nothing.
-template <class K, class G, int WAVES, bool CAP, bool DROP>
+template <class K, class G, int WAVES, bool CAP, bool DROP, bool TWO>
 __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) {
     typedef typename K::T T;
     constexpr int V = 16 / (int)sizeof(T), NR = (G::RE + WAVES - 1) / WAVES, NC = (G::NF + WAVES - 1) / WAVES;  // fragments of a wave
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) 
     __syncthreads();
     for (int t = t0; t < t1; ++t) {  // (the masked form for every tile: one copy of the code, whose first run is part of a short call)
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
-        if (!idle) pa_fwd_tile<K, G, CAP, DROP, true>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, TWO, true>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         if (t + 1 < t1) store(t + 1, sm + ((t - t0 + 1) & 1) * G::FWD * 1024);
         if (t + 2 < t1) load(t + 2);
         __syncthreads();
@@ -571,7 +576,7 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
 // dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  One
 // workgroup a compute unit by its LDS and registers, so two waves a SIMD: what they wait for one another, for fragments and at the
 // barrier of a step is what is left (PaBF, E, F = 200: matrix pipe 48 % busy, LDS 44 %; PaX3 63 and 45 to 53 %).  17404 tokens x 1999
-// labels bf16 88 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
+// labels of 200 bf16 98 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
 // PaX3 takes dV and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a
 // wave at two waves a SIMD, and the scores a second time are a fifth of the products.
 template <class K, class G, int PART, bool CAP, bool DROP>
@@ -579,7 +584,8 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     typedef typename K::T T;
     typedef typename K::frag frag;
     extern __shared__ __attribute__((aligned(16))) char sm[];
-    constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U, D = G::PL == 3 ? 2 : 4;
+    constexpr int BUF = (G::QRY + G::OUT) * 1024, WAVES = PA_TILE / 16, U = G::U;
+    constexpr int D = G::PL == 3 || (G::NE > 7 && (CAP || G::SZ == 4)) ? 2 : 4;  // (where four fragments ahead would spill)
     constexpr bool DV = PART & 1, DK = PART & 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15, g = lane >> 4;
     long long before;
@@ -664,12 +670,14 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
                     }
                 }
                 frag pf, sf;
-                bf16x8 sl;
+                bf16x8 pl, sl;  // (bf16: what rounding dropped)
                 if (DV) pa_pack(p, pf);
                 if (DK) pa_pack(ds, sf);
                 if constexpr (DK && sizeof(T) == 2) pa_pack_low(ds, sl);
+                if constexpr (DV && sizeof(T) == 2) pa_pack_low(p, pl);
                 pa_run_ring<NC>(ring, ldc, [&](int j, const frag& f) {
                     if (DV && j < G::NF) {
+                        if constexpr (sizeof(T) == 2) dv[DV ? j : 0] = pa_mma(f, pl, dv[DV ? j : 0]);
                         dv[DV ? j : 0] = pa_mma(f, pf, dv[DV ? j : 0]);
                     } else {
                         const int e = DK ? j - (DV ? G::NF : 0) : 0;
@@ -906,15 +914,15 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_q_join_kernel(PaArgs
 }
 
 // --------------------------------------------------------------------------------------------------------------- launch
-template <class K, class G, int W, int OCC, bool CAP, bool DROP>
+template <class K, class G, int W, int OCC, bool CAP, bool DROP, bool TWO>
 static int pa_fwd(PaArgs& a, hipStream_t st) {
     typedef typename K::T T;
     if constexpr (W == 8) if (a.nLT == 1) {
-        hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+        hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP, TWO>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (W != 8 || a.nLT > 1) {
         hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+        hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP, TWO>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (a.extra > 0) {
         if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 16>), dim3(a.B * a.L), dim3(1024), 0, st, a);
@@ -948,7 +956,9 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
 }
 template <class K, class G, int W, int OCC, bool CAP>
 static int pa_fwd_drop(PaArgs& a, hipStream_t st) {
-    return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true>(a, st) : pa_fwd<K, G, W, OCC, CAP, false>(a, st);
+    if constexpr (sizeof(typename K::T) == 2)
+        if (a.rest) return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true, true>(a, st) : pa_fwd<K, G, W, OCC, CAP, false, true>(a, st);
+    return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true, false>(a, st) : pa_fwd<K, G, W, OCC, CAP, false, false>(a, st);
 }
 // W waves, OCC waves a SIMD asked of the compiler
 template <class K, class G, int W, int OCC>
