@@ -13,11 +13,13 @@ def half_step(t):
     return torch.finfo(t).eps / 2
 
 
-def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=True):
+def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=True, two=False):
     """keys [R,E], values [R,F], queries [L,E] (any type, used as the numbers they hold), spans list of (start, n);
-    keep: list of [L,n] dropout factors or None; rest: the backward has what the rounding of O dropped.  Returns dict of name -> (value, bound): O, lse and, with dout [B,L,F],
-    dK, dV, dQ."""
+    keep: list of [L,n] dropout factors or None; rest: the backward has what the rounding of O dropped; two: P and dS enter their
+    products in two pieces of the tensors' type (off by half a step of what the first one dropped).  Returns dict of name ->
+    (value, bound): O, lse and, with dout [B,L,F], dK, dV, dQ."""
     step = half_step(values.dtype)
+    piece = (step * step if two else step) * (step > U)
     k, v, q = (x.detach().cpu().double() for x in (keys, values, queries))
     B, L, E, F, R = len(spans), q.shape[0], k.shape[1], v.shape[1], k.shape[0]
     z = lambda *s: torch.zeros(s, dtype=torch.float64)  # noqa: E731
@@ -45,7 +47,7 @@ def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=T
         D = 1.0 if keep is None else keep[b]
         Pd = P * D
         O = Pd @ vb
-        dO_ = (Pd * (rel + step * (step > U) + (n + 4) * U)) @ vb.abs()   # P is rounded to the tensors' type for the product
+        dO_ = (Pd * (rel + piece + (n + 4) * U)) @ vb.abs()   # P is rounded to the tensors' type for the product
         out['O'][0][b] = O
         out['O'][1][b] = dO_ + (O.abs() + dO_) * step
         if dout is None:
@@ -53,7 +55,7 @@ def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=T
         g = dout[b].detach().cpu().double()
         slabs += 1
         out['dV'][0][s0:s0 + n] = Pd.T @ g
-        out['dV'][1][s0:s0 + n] = (Pd * (rel + step * (step > U) + (L + 4) * U)).T @ g.abs()
+        out['dV'][1][s0:s0 + n] = (Pd * (rel + piece + (L + 4) * U)).T @ g.abs()
         dP = g @ vb.T
         ddP = (F + 2) * U * (g.abs() @ vb.T.abs())
         delta = (g * O).sum(1, keepdim=True)
@@ -65,7 +67,7 @@ def attn_ref(keys, values, queries, spans, cap=0.0, dout=None, keep=None, rest=T
         if cap > 0:
             dth = (dx / cap + 8 * U) * slope + 4 * U       # error of tanh, from x's error and its own
             ddS = ddS + P * inner.abs() * 2 * (th.abs() * dth + dth * dth + U)
-        ddS = ddS + dS.abs() * step * (step > U)
+        ddS = ddS + dS.abs() * piece
         out['dQ'][0] += dS @ kb
         out['dQ'][1] += (ddS + (n + 4) * U * dS.abs()) @ kb.abs()
         out['dK'][0][s0:s0 + n] = dS.T @ q

@@ -331,3 +331,16 @@ def test_notes_that_overlap_stay_inside_the_workspace(ops, dtype):
     within(O, ref['O'], 'O')
     within(dq, ref['dQ'], 'dQ')
     assert dk.shape == k.shape and dv.shape == v.shape
+
+
+@pytest.mark.parametrize('cap', [0.0, 10.0])
+@pytest.mark.parametrize('lens,E,F,L', [([40, 13, 1], 200, 200, 60), ([300, 517], 100, 200, 1), ([20], 30, 8, 300), ([700, 31], 200, 64, 150)])
+def test_16_bit_gradients_are_rounded_once(ops, lens, E, F, L, cap):
+    """A training call's bf16 results are the exact ones rounded, up to 32-bit sums and two-piece weights (2^-16): nothing in between is
+    rounded to 16 bits, whose errors the cancellation in dS would multiply."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, torch.bfloat16, seed=11)
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, cap)
+    got = (O, *ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, cap))
+    ref = attn_ref(k, v, q, sl, cap, do, two=True)
+    for name, x in zip(('O', 'dK', 'dV', 'dQ'), got):
+        within(x, ref[name], name)
