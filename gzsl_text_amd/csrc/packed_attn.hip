@@ -66,7 +66,10 @@ static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* w
     a.nLT = p.nLT, a.extra = p.extra, a.least = p.least;
     // few rows: one a wave, for the time of one row's parts to come in (1000 tokens x 428 labels: 31 us with four a wave, 12 so); many: four,
     // to share out what a workgroup has to find out first (17404 x 1999: 21 us with one a wave, 19 so)
-    a.join_rows = (long long)p.max_len * d.B <= 16384 ? 4 : 16;
+    // and few tiles of more than two runs each: one row for all four waves (500 tokens x 3917 labels, 51 runs a tile: 58 us with a row a
+    // wave, 7 so; 6000 x 1999, 5 runs: 19 and 29)
+    const long long at_most = (long long)p.max_len * d.B;
+    a.join_rows = at_most <= 4096 && p.units > 2LL * d.B * cdiv(p.max_len, PA_TILE) ? 1 : (at_most <= 16384 ? 4 : 16);
     char* w = (char*)work;
     a.TK = w, w += p.kv;
     a.Q = w, w += p.q;

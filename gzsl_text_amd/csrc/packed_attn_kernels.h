@@ -709,7 +709,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
         }
     }
 }
-// dK / dV of the tiles that runs share, in order, and zeros in the rows of no note: 4 or 16 rows a workgroup, counted from a note's first
+// dK / dV of the tiles that runs share, in order, and zeros in the rows of no note: 1, 4 or 16 rows a workgroup, counted from a note's first
 // (blockIdx.y = B: the rows in front of the first note), a wave to a row.
 template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
@@ -719,6 +719,35 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const long long end = next < a.B ? note_span(a.spans, next, a.rows, a.max_len).start : a.rows;
     long long first;
     const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
+    if (a.join_rows == 1) {  // few tiles of many runs each: the four waves share one row's parts and join in LDS
+        __shared__ float sh[4][7 * 64];
+        for (long long r = blockIdx.x; r < max((long long)sp.len, end - sp.start); r += gridDim.x) {
+            const long long row = sp.start + r;
+            float s[7] = {};  // E + F <= 416
+            if (r < sp.len) {
+                if (runs.steps == 0) continue;
+                const int at = (int)(first + r / PA_TILE) * a.nQ, u0 = at / runs.per, n = (at + a.nQ - 1) / runs.per - u0, per = n / 4 + 1;
+                if (n == 0) continue;
+                const float* slab = a.dkv + (2LL * u0 * PA_TILE + r % PA_TILE) * W;
+#pragma unroll 4
+                for (int k = w * per; k < min(n + 1, (w + 1) * per); ++k)
+#pragma unroll
+                    for (int j = 0; j < 7; ++j) s[j] += slab[(k > 0 ? 2LL * k : 1LL) * PA_TILE * W + min(lane + 64 * j, W - 1)];
+            } else if (row >= end) {
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 7; ++j) sh[w][lane + 64 * j] = s[j];
+            __syncthreads();
+            for (int c = threadIdx.x; c < W; c += 256) {
+                const T o = (T)(((sh[0][c] + sh[1][c]) + sh[2][c]) + sh[3][c]);
+                if (c < a.E) ((T*)a.dK)[row * a.E + c] = o;
+                else ((T*)a.dV)[row * a.F + c - a.E] = o;
+            }
+            __syncthreads();
+        }
+        return;
+    }
     for (long long r0 = (long long)blockIdx.x * a.join_rows; r0 < max((long long)sp.len, end - sp.start); r0 += (long long)gridDim.x * a.join_rows) {
         int u0 = 0, u1 = 0;  // the runs of this tile
         if (r0 < sp.len && runs.steps > 0) {

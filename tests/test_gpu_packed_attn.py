@@ -344,3 +344,15 @@ def test_16_bit_gradients_are_rounded_once(ops, lens, E, F, L, cap):
     ref = attn_ref(k, v, q, sl, cap, do, two=True)
     for name, x in zip(('O', 'dK', 'dV', 'dQ'), got):
         within(x, ref[name], name)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('lens,E,F,L', [([130, 7], 30, 156, 1500), ([129], 100, 200, 900), ([20, 0, 31], 200, 33, 2100)])
+def test_token_tiles_of_many_runs(ops, dtype, lens, E, F, L):
+    """Few tokens, many labels: a token tile's gradients come from many workgroups' parts, odd and even widths, rows between notes."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=13, pitch=140, tail=5, garbage=float('nan'))
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, 5.0)
+    got = (O, lse, *ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, 5.0))
+    ref = attn_ref(k, v, q, sl, 5.0, do)
+    for name, x in zip(('O', 'lse', 'dK', 'dV', 'dQ'), got):
+        within(x, ref[name], name)
