@@ -11,12 +11,12 @@
 //          the six cross terms of weight >= 2^-16 of them (what is dropped is below 2^-24 of the product), each the same MFMA:
 //          6 x 16 cycles per 32 k against 8 x 32 of the fp32 MFMA.
 //   PaF32  fp32 tensors, E > 112 (three pieces of both tiles no longer fit LDS twice): v_mfma_f32_16x16x4_f32, exact.
-// Sums are fp32 in all of them.  For bf16 tensors a scoring call rounds P to bf16 for its product (half a step of 2^-8, as the inputs' own
-// rounding; O is 1.0 to 1.3 times as far off as a rounded exact result); the softmax sum uses P before that.  A forward that a backward
-// follows and the backward take P and dS in two bf16 pieces (16 bits, one more product each): dS sums to zero over a row, so its
-// products cancel, and delta = <dO, O> has to be that of the same P.  With one piece of each, dK and dQ were up to 2.4 times as far off
-// as rounded exact results, dV 1.4 times; so all are within a hundredth of them (17404 tokens x 1999 labels of 200: forward 50 -> 60
-// us, dK / dV 88 -> 98).
+// Sums are fp32 in all of them.  P and dS of bf16 tensors enter their products in two bf16 pieces (16 bits, one more product each).  With
+// P in one, a score row whose pooled values cancel was off by many times its own rounding (values of both signs, 517 tokens: 3.3e-4 for
+// 0.8e-4), and O 1.0 to 1.3 times as far off as a rounded exact result where they do not; dS sums to zero over a row, so its products cancel
+// always, and delta = <dO, O> has to be that of the same P: dK and dQ were up to 2.4 times as far off, dV 1.4 times.  So all are within a
+// hundredth of rounded exact results (forward of 19309 tokens x 9000 labels 137 -> 173 us, of 17404 x 1999 labels of 200 50 -> 60, dK / dV
+// there 88 -> 98).
 //
 // Everything is moved as FRAGMENTS: 1 KB, 16 bytes a lane, exactly one operand of one matrix instruction (eight bf16 of a lane;
 // four fp32, which feed four instructions).  With n = lane & 15, g = lane >> 4:

@@ -239,11 +239,12 @@ __device__ __forceinline__ void pa_fwd_begin(PaFwdState<K, G>& w, const PaArgs& 
     w.m = w.fixed ? 0.f : -INFINITY, w.sum = 0.f;
 }
 // KR: row fragments of the keys, VC: column fragments of the values; t0: the tile's first token, LAST: it may end behind the note (left
-// tokens are the note's); TWO: the weights go in two bf16 pieces.
-template <class K, class G, bool CAP, bool DROP, bool TWO, bool LAST>
+// tokens are the note's).
+template <class K, class G, bool CAP, bool DROP, bool LAST>
 __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left,
                                             int lane) {
     typedef typename K::frag frag;
+    constexpr bool TWO = sizeof(typename K::T) == 2;  // the weights go in two bf16 pieces
     constexpr int U = G::U, D = G::PL == 3 ? 2 : (TWO && DROP ? 3 : 4);
     const int g = lane >> 4;
     f32x4 s[U];
@@ -341,7 +342,7 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
 // 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 940 TFLOP/s of the padded products (1255 is what a large library product
 // reaches, whose clock is as low); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
 // reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
-template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP, bool TWO>
+template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15;
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     auto step = [&](int t, auto last) {
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
         if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)(t + 1) * G::FWD * 1024, sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
-        if (!idle) pa_fwd_tile<K, G, CAP, DROP, TWO, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         pa_arrive();
     };
     for (int t = t0; t < t1 - 1; ++t) step(t, std::false_type{});
@@ -398,7 +399,7 @@ __device__ __forceinline__ void pa_row_load(const T* row, int e0, int W, bool wi
 // current one.  No images and one launch less: 2 notes of 59 tokens in all x 70 labels 16 -> 13 us, 40003 tokens x 50 labels 58 -> 40.
 // With more labels every label workgroup would cut the fragments again.  What bounds it is latency: five tiles a workgroup at 256
 // workgroups (24 us for 48 MB); a second tile on its way changed nothing.
-template <class K, class G, int WAVES, bool CAP, bool DROP, bool TWO>
+template <class K, class G, int WAVES, bool CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) {
     typedef typename K::T T;
     constexpr int V = 16 / (int)sizeof(T), NR = (G::RE + WAVES - 1) / WAVES, NC = (G::NF + WAVES - 1) / WAVES;  // fragments of a wave
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) 
     __syncthreads();
     for (int t = t0; t < t1; ++t) {  // (the masked form for every tile: one copy of the code, whose first run is part of a short call)
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
-        if (!idle) pa_fwd_tile<K, G, CAP, DROP, TWO, true>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
+        if (!idle) pa_fwd_tile<K, G, CAP, DROP, true>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         if (t + 1 < t1) store(t + 1, sm + ((t - t0 + 1) & 1) * G::FWD * 1024);
         if (t + 2 < t1) load(t + 2);
         __syncthreads();
@@ -943,15 +944,15 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_q_join_kernel(PaArgs
 }
 
 // --------------------------------------------------------------------------------------------------------------- launch
-template <class K, class G, int W, int OCC, bool CAP, bool DROP, bool TWO>
+template <class K, class G, int W, int OCC, bool CAP, bool DROP>
 static int pa_fwd(PaArgs& a, hipStream_t st) {
     typedef typename K::T T;
     if constexpr (W == 8) if (a.nLT == 1) {
-        hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP, TWO>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+        hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (W != 8 || a.nLT > 1) {
         hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP, TWO>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
+        hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (a.extra > 0) {
         if ((long long)a.B * a.L <= 1024) hipLaunchKernelGGL((pa_join_kernel<T, G::ROWS, 16>), dim3(a.B * a.L), dim3(1024), 0, st, a);
@@ -983,16 +984,11 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <class K, class G, int W, int OCC, bool CAP>
-static int pa_fwd_drop(PaArgs& a, hipStream_t st) {
-    if constexpr (sizeof(typename K::T) == 2)
-        if (a.rest) return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true, true>(a, st) : pa_fwd<K, G, W, OCC, CAP, false, true>(a, st);
-    return a.thresh ? pa_fwd<K, G, W, OCC, CAP, true, false>(a, st) : pa_fwd<K, G, W, OCC, CAP, false, false>(a, st);
-}
 // W waves, OCC waves a SIMD asked of the compiler
 template <class K, class G, int W, int OCC>
 static int pa_go_fwd(PaArgs& a, hipStream_t st) {
-    return a.cap > 0.f ? pa_fwd_drop<K, G, W, OCC, true>(a, st) : pa_fwd_drop<K, G, W, OCC, false>(a, st);
+    if (a.cap > 0.f) return a.thresh ? pa_fwd<K, G, W, OCC, true, true>(a, st) : pa_fwd<K, G, W, OCC, true, false>(a, st);
+    return a.thresh ? pa_fwd<K, G, W, OCC, false, true>(a, st) : pa_fwd<K, G, W, OCC, false, false>(a, st);
 }
 template <class K, class G, int W, int H>
 static int pa_go_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {

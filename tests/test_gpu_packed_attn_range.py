@@ -1,0 +1,36 @@
+"""Packed label attention over the range of its arguments."""
+import pytest
+import torch
+
+from tests.packed_ref import attn_ref, within
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+@pytest.fixture(scope='module')
+def ops():
+    from gzsl_text_amd.ops_hip import HipOps
+    return HipOps()
+
+
+def make(lens, E, F, L, dtype, seed, tail=0, scale=0.3):
+    from gzsl_text_amd.packed import note_spans
+    table, max_len, rows = note_spans(lens, None, DEV)
+    gen = torch.Generator().manual_seed(seed)
+    k, v = torch.randn(rows + tail, E, generator=gen), torch.randn(rows + tail, F, generator=gen)
+    q, do = scale * torch.randn(L, E, generator=gen), torch.randn(len(lens), L, F, generator=gen)
+    return [x.to(dtype).to(DEV) for x in (k, v, q, do)] + [table, max_len, [tuple(x) for x in table.tolist()]]
+
+
+@pytest.mark.parametrize('cap', [0.0, 10.0])
+@pytest.mark.parametrize('lens,E,F,L', [([40, 13, 1], 200, 200, 60), ([300, 517], 100, 200, 200), ([900], 30, 64, 9), ([70, 3], 36, 52, 1500)])
+def test_16_bit_scoring_is_rounded_once(ops, lens, E, F, L, cap):
+    """A call that no backward follows is as exact as one of a training step: the exact values rounded, up to 32-bit sums and weights in
+    two pieces (2^-16).  Values of both signs: where a row cancels, weights rounded to 8 bits show."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, torch.bfloat16, seed=4)
+    O, lse, _ = ops.attn_packed_fwd(k, v, q, spans, max_len, cap, need_grad=False)
+    ref = attn_ref(k, v, q, sl, cap, two=True)
+    within(O, ref['O'], 'O')
+    within(lse, ref['lse'], 'lse')
+    assert torch.equal(O, ops.attn_packed_fwd(k, v, q, spans, max_len, cap)[0])
