@@ -172,22 +172,26 @@ __device__ __forceinline__ float pa_far(float x, const PaCap& c) {  // cap log2(
     return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c.k1)), -2.f * c.c2, c.c2);
 }
 #define PA_NEAR 0.35f
-// Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself
-// (pa_over takes it as it is).  bf16 tensors take the closed form: exact limits at +-inf, absolute error of a few 2^-24.  fp32 tensors
-// take the odd series below |x / cap| = 0.35 (the next term is below 2^-26 of the value), for the relative accuracy that the products
-// of the gradient still have, and the closed form only where a wave's tile holds a larger one.  (For bf16 the series is the longer way:
-// 148 us against 138 for 19309 tokens x 9000 labels.)
-template <class K, bool CAP, int U, bool TH>
+// How scores are capped (the kernels' CAP):
+//   1  the closed form: exact limits at +-inf, absolute error of a few 2^-24 cap log2(e).  bf16 tensors with a cap of at most PA_CLOSED,
+//      whose weights it leaves as good as their two pieces do.
+//   2  the odd series below |x / cap| = 0.35 (the next term is below 2^-26 of the value) and the closed form only where a wave's tile
+//      holds a larger one: an error relative to the score, whatever the cap.  fp32 tensors, whose products of the gradient still have
+//      that accuracy, and larger caps, at which the closed form's error grows past the scores (at 1e6 weights were off by a fifth).
+//      For small caps of bf16 it is the longer way: 148 us against 138 for 19309 tokens x 9000 labels, weights in one piece.
+enum { PA_NONE = 0, PA_FORM = 1, PA_SERIES = 2 };
+#define PA_CLOSED 64.f
+// Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself.
+template <int CAP, int U, bool TH>
 __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, float (&y)[U][4], float (&th)[U][4]) {
-    constexpr bool SERIES = CAP && sizeof(typename K::T) == 4;
     float most = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if (!CAP) {
+            if (CAP == PA_NONE) {
                 y[u][r] = x[u][r];
-            } else if (!SERIES) {
+            } else if (CAP == PA_FORM) {
                 y[u][r] = pa_far(x[u][r], c);
             } else {
                 const float v = x[u][r] * c.inv, w = v * v;
@@ -197,7 +201,7 @@ __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, f
                 y[u][r] = x[u][r] * t;
             }
         }
-    if (SERIES && __any(most >= PA_NEAR)) {
+    if (CAP == PA_SERIES && __any(most >= PA_NEAR)) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -209,11 +213,6 @@ __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, f
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) th[u][r] = y[u][r] * c.kt;
-}
-// 2^(y - off)
-template <bool CAP>
-__device__ __forceinline__ float pa_over(float y, float off) {
-    return __builtin_amdgcn_exp2f(CAP ? y - off : fmaf(y, PA_LOG2E, -off));
 }
 
 // Copies KB KB of a tile image into LDS: 1 KB per wave instruction, spread over the workgroup's waves.  `src` and `wave` are scalars.

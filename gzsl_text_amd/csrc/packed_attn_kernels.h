@@ -240,12 +240,12 @@ __device__ __forceinline__ void pa_fwd_begin(PaFwdState<K, G>& w, const PaArgs& 
 }
 // KR: row fragments of the keys, VC: column fragments of the values; t0: the tile's first token, LAST: it may end behind the note (left
 // tokens are the note's).
-template <class K, class G, bool CAP, bool DROP, bool LAST>
+template <class K, class G, int CAP, bool DROP, bool LAST>
 __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a, const PaCap& cap, const char* KR, const char* VC, int t0, int left,
                                             int lane) {
     typedef typename K::frag frag;
     constexpr bool TWO = sizeof(typename K::T) == 2;  // the weights go in two bf16 pieces
-    constexpr int U = G::U, D = G::PL == 3 ? 2 : (TWO && DROP ? 3 : 4);
+    constexpr int U = G::U, D = G::PL == 3 || (TWO && CAP == PA_SERIES) ? 2 : (TWO && DROP ? 3 : 4);  // (where four ahead would spill)
     const int g = lane >> 4;
     f32x4 s[U];
 #pragma unroll
@@ -257,7 +257,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
     pa_run_ring<G::RE>(ring, ldk, [&](int i, const frag& f) { s[i % U] = pa_mma(f, w.qf[i / U], s[i % U]); });
     pa_fill_ring<G::NF>(ring, ldv);  // under way during the softmax
     float y[U][4], th[U][4];
-    pa_scores<K, CAP, U, false>(s, cap, y, th);
+    pa_scores<CAP, U, false>(s, cap, y, th);
     if (LAST) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -342,7 +342,7 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
 // 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 940 TFLOP/s of the padded products (1255 is what a large library product
 // reaches, whose clock is as low); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
 // reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
-template <class K, class G, int WAVES, int OCC, bool CAP, bool DROP>
+template <class K, class G, int WAVES, int OCC, int CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = pa_scalar(tid >> 6), n = lane & 15;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
     const bool idle = l0 >= a.L;  // (wave-uniform: copies and barriers only)
     const PaCap cap = pa_cap(a.cap);
     PaFwdState<K, G> w;
-    pa_fwd_begin(w, a, CAP, b, l0 + n);
+    pa_fwd_begin(w, a, CAP != PA_NONE, b, l0 + n);
     {
         const int c = min(l0, a.nQ * G::ROWS - 16);
         const char* img = a.Q + (long long)(c / G::ROWS) * G::PL * G::RE * 1024;
@@ -399,7 +399,7 @@ __device__ __forceinline__ void pa_row_load(const T* row, int e0, int W, bool wi
 // current one.  No images and one launch less: 2 notes of 59 tokens in all x 70 labels 16 -> 13 us, 40003 tokens x 50 labels 58 -> 40.
 // With more labels every label workgroup would cut the fragments again.  What bounds it is latency: five tiles a workgroup at 256
 // workgroups (24 us for 48 MB); a second tile on its way changed nothing.
-template <class K, class G, int WAVES, bool CAP, bool DROP>
+template <class K, class G, int WAVES, int CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) {
     typedef typename K::T T;
     constexpr int V = 16 / (int)sizeof(T), NR = (G::RE + WAVES - 1) / WAVES, NC = (G::NF + WAVES - 1) / WAVES;  // fragments of a wave
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void pa_fwd_direct_kernel(PaArgs a) 
     };
     if (t0 < t1) load(t0);
     PaFwdState<K, G> w;
-    pa_fwd_begin(w, a, CAP, b, l0 + n);
+    pa_fwd_begin(w, a, CAP != PA_NONE, b, l0 + n);
     {
         const T* row = (const T*)a.queries + (long long)min(l0 + n, a.L - 1) * a.ldq;
         const bool qwide = a.E % V == 0 && a.ldq % V == 0 && ((uintptr_t)a.queries & 15) == 0;
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
 
 // ------------------------------------------------------------------------------------------------------------- backward
 // P and dS of a tile: weights w = exp2(y - off) * scale, dropout factor keep.
-template <bool CAP, bool TH>
+template <int CAP, bool TH>
 __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, float scale, float delta, float keep, float& p, float& ds) {
     const float w = __builtin_amdgcn_exp2f(CAP ? y - off : fmaf(y, PA_LOG2E, -off)) * scale;
     p = w * keep;
@@ -580,7 +580,7 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
 // labels of 200 bf16 98 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
 // PaX3 takes dV and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a
 // wave at two waves a SIMD, and the scores a second time are a fifth of the products.
-template <class K, class G, int PART, bool CAP, bool DROP>
+template <class K, class G, int PART, int CAP, bool DROP>
 __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
     typedef typename K::T T;
     typedef typename K::frag frag;
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
                 auto ldc = [&](int j) { return DV && j < G::NF ? ldv(j) : ldk(j - (DV ? G::NF : 0)); };
                 pa_fill_ring<NC>(ring, ldc);
                 float p[U][4], ds[U][4], y[U][4], th[U][4];
-                pa_scores<K, CAP, U, DK>(s, cap, y, th);
+                pa_scores<CAP, U, DK>(s, cap, y, th);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const f32x4 off = *reinterpret_cast<const f32x4*>(aux + 16 * u + 4 * g), scale = *reinterpret_cast<const f32x4*>(aux + G::ROWS + 16 * u + 4 * g),
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
                             const uint32_t key = gz_row_key(a.seed, GZSL_STREAM_ATTN, (uint32_t)b * a.L_total + a.l_offset + l);
                             keep = gz_u32(key, (uint32_t)tok) >= a.thresh ? a.scale : 0.f;
                         }
-                        pa_grad<CAP, CAP && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
+                        pa_grad<CAP, CAP != PA_NONE && DK>(y[u][r], th[u][r], dp[u][r], off[r], scale[r], delta[r], keep, p[u][r], ds[u][r]);
                     }
                 }
                 frag pf, sf;
@@ -802,7 +802,7 @@ __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
 // dQ: workgroup = WAVES x 16 labels (label on the lane axis) over one note or one chunk of it; a slab per chunk.  H = 2: twice the
 // waves, which take turns at the token tiles and add up in LDS (few labels: half the way through the longest note).  Bound as dK / dV is
 // (17404 tokens x 1999 labels of 200 bf16 70 us, 7339 x 9000 of 100 and 200 fp32 325).
-template <class K, class G, int WAVES, int H, bool CAP, bool DROP>
+template <class K, class G, int WAVES, int H, int CAP, bool DROP>
 __global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     typedef typename K::T T;
     typedef typename K::frag frag;
@@ -866,14 +866,14 @@ __global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
             };
             pa_fill_ring<G::NE>(ring, ldc);
             float ds[U][4], y[U][4], th[U][4];
-            pa_scores<K, CAP, U, true>(s, cap, y, th);
+            pa_scores<CAP, U, true>(s, cap, y, th);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float keep = 1.f, p;
                     if (DROP) keep = gz_u32(key, (uint32_t)(t * G::ROWS + 16 * u + 4 * g + r)) >= a.thresh ? a.scale : 0.f;
-                    pa_grad<CAP, CAP>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
+                    pa_grad<CAP, CAP != PA_NONE>(y[u][r], th[u][r], dp[u][r], off, scale, delta, keep, p, ds[u][r]);
                 }
             if constexpr (decltype(last)::value) {  // (a key of zeros has the score 0, which may be far above the note's own)
                 const int left = len - t * G::ROWS;
@@ -944,7 +944,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_q_join_kernel(PaArgs
 }
 
 // --------------------------------------------------------------------------------------------------------------- launch
-template <class K, class G, int W, int OCC, bool CAP, bool DROP>
+template <class K, class G, int W, int OCC, int CAP, bool DROP>
 static int pa_fwd(PaArgs& a, hipStream_t st) {
     typedef typename K::T T;
     if constexpr (W == 8) if (a.nLT == 1) {
@@ -961,7 +961,7 @@ static int pa_fwd(PaArgs& a, hipStream_t st) {
     GZSL_CHECK_LAUNCH();
     return 0;
 }
-template <class K, class G, int W, int H, bool CAP, bool DROP>
+template <class K, class G, int W, int H, int CAP, bool DROP>
 static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     typedef typename K::T T;
     constexpr int lds = 2 * (G::QRY + G::OUT) * 1024;
@@ -984,14 +984,21 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     GZSL_CHECK_LAUNCH();
     return 0;
 }
+// f(how scores are capped, whether weights are dropped)
+template <class K, class F>
+static int pa_form(const PaArgs& a, F&& f) {
+    auto drop = [&](auto cap) { return a.thresh ? f(cap, std::true_type{}) : f(cap, std::false_type{}); };
+    if (a.cap == 0.f) return drop(std::integral_constant<int, PA_NONE>{});
+    if constexpr (sizeof(typename K::T) == 2)
+        if (a.cap <= PA_CLOSED) return drop(std::integral_constant<int, PA_FORM>{});
+    return drop(std::integral_constant<int, PA_SERIES>{});
+}
 // W waves, OCC waves a SIMD asked of the compiler
 template <class K, class G, int W, int OCC>
 static int pa_go_fwd(PaArgs& a, hipStream_t st) {
-    if (a.cap > 0.f) return a.thresh ? pa_fwd<K, G, W, OCC, true, true>(a, st) : pa_fwd<K, G, W, OCC, true, false>(a, st);
-    return a.thresh ? pa_fwd<K, G, W, OCC, false, true>(a, st) : pa_fwd<K, G, W, OCC, false, false>(a, st);
+    return pa_form<K>(a, [&](auto cap, auto drop) { return pa_fwd<K, G, W, OCC, decltype(cap)::value, decltype(drop)::value>(a, st); });
 }
 template <class K, class G, int W, int H>
 static int pa_go_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
-    if (a.cap > 0.f) return a.thresh ? pa_bwd<K, G, W, H, true, true>(a, p, st) : pa_bwd<K, G, W, H, true, false>(a, p, st);
-    return a.thresh ? pa_bwd<K, G, W, H, false, true>(a, p, st) : pa_bwd<K, G, W, H, false, false>(a, p, st);
+    return pa_form<K>(a, [&](auto cap, auto drop) { return pa_bwd<K, G, W, H, decltype(cap)::value, decltype(drop)::value>(a, p, st); });
 }

@@ -3,9 +3,11 @@ import pytest
 import torch
 
 from tests.packed_ref import attn_ref, within
+from tests.packed_ref_range import attn_ref_range
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
+BOTH = pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
 
 
 @pytest.fixture(scope='module')
@@ -23,6 +25,12 @@ def make(lens, E, F, L, dtype, seed, tail=0, scale=0.3):
     return [x.to(dtype).to(DEV) for x in (k, v, q, do)] + [table, max_len, [tuple(x) for x in table.tolist()]]
 
 
+def run(ops, k, v, q, do, spans, max_len, cap=0.0, **drop):
+    O, lse, rest = ops.attn_packed_fwd(k, v, q, spans, max_len, cap, **drop)
+    dk, dv, dq = ops.attn_packed_bwd(do, O, lse, rest, k, v, q, spans, max_len, cap, **drop)
+    return dict(O=O, lse=lse, dV=dv, dK=dk, dQ=dq)
+
+
 @pytest.mark.parametrize('cap', [0.0, 10.0])
 @pytest.mark.parametrize('lens,E,F,L', [([40, 13, 1], 200, 200, 60), ([300, 517], 100, 200, 200), ([900], 30, 64, 9), ([70, 3], 36, 52, 1500)])
 def test_16_bit_scoring_is_rounded_once(ops, lens, E, F, L, cap):
@@ -34,3 +42,24 @@ def test_16_bit_scoring_is_rounded_once(ops, lens, E, F, L, cap):
     within(O, ref['O'], 'O')
     within(lse, ref['lse'], 'lse')
     assert torch.equal(O, ops.attn_packed_fwd(k, v, q, spans, max_len, cap)[0])
+
+
+@BOTH
+@pytest.mark.parametrize('lens,E,F,L', [([150, 31, 1], 100, 200, 40), ([77, 0, 130], 200, 64, 150)])
+@pytest.mark.parametrize('cap', [1e2, 1e3, 1e5, 1e6, 1e8, 1e30])
+def test_caps_far_above_the_scores(ops, lens, E, F, L, dtype, cap):
+    """Scores of deviation 3 and more under caps up to the largest that is accepted: an error relative to the score, whatever the cap."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=6)
+    got, ref = run(ops, k, v, q, do, spans, max_len, cap), attn_ref_range(k, v, q, sl, cap, do)
+    for name, x in got.items():
+        within(x, ref[name], f'{name} at cap {cap:g}')
+
+
+@BOTH
+@pytest.mark.parametrize('cap', [1e-30, 1e-3, 64.0, 65.0, 300.0])
+def test_caps_below_and_about_the_scores(ops, dtype, cap):
+    """Scores up to twenty times the cap and far beyond it."""
+    k, v, q, do, spans, max_len, sl = make([130, 40], 36, 52, 41, dtype, seed=8, scale=20.0)
+    got, ref = run(ops, k, v, q, do, spans, max_len, cap), attn_ref_range(k, v, q, sl, cap, do)
+    for name in ('O', 'lse', 'dV'):
+        within(got[name], ref[name], f'{name} at cap {cap:g}')
