@@ -38,19 +38,13 @@ struct GsArgs {
     int ncg, nblk, TS, tiles, chunk, nch;    // channel groups of a workgroup, workgroups over the channels, threads over time, tiles of a chunk
 };
 
-// z = sigmoid(g), a = 1 - z = sigmoid(-g).  fp32: both to a few roundings of their own size (e^-|g| never overflows; its exponent
-// |g| log2(e) is rounded once: |g| half steps), which the backward's z a needs.  The forward of
-// bf16 tensors takes a as the difference, off by a few half steps of 1: it only multiplies the state.
-template <typename T, bool BWD>
+// z = sigmoid(g) = 1 / (1 + w), a = 1 - z = w z with w = e^-g, both to a few roundings of their own size (the exponent |g| log2(e) is rounded
+// once: |g| half steps): a difference 1 - z would be off by a half step of 1, which a far state multiplies.  w stops at 2^126, where its
+// reciprocal is still a normal number; a gate that is no number stays one.
 __device__ __forceinline__ void gs_gate(float g, float& z, float& a) {
-    if (sizeof(T) == 2 && !BWD) {
-        z = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -GS_LOG2E));
-        a = 1.f - z;
-    } else {
-        const float e = __builtin_amdgcn_exp2f(fabsf(g) * -GS_LOG2E), big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
-        z = g >= 0.f ? big : small;
-        a = g >= 0.f ? small : big;
-    }
+    const float w = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -GS_LOG2E, 126.f));
+    z = __builtin_amdgcn_rcpf(1.f + w);
+    a = w * z;
 }
 
 template <typename T, int V>
@@ -165,7 +159,7 @@ __global__ __launch_bounds__(GS_THREADS) void gs_chunk_kernel(GsArgs a) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float z, k;
-                gs_gate<T, BWD>(g[s][v], z, k);
+                gs_gate(g[s][v], z, k);
                 if (BWD) B[v] = k * (B[v] + (a.dh ? u[s][v] : 0.f));
                 else B[v] = fmaf(k, B[v], z * u[s][v]);
                 A[v] *= k;
@@ -313,7 +307,7 @@ __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gs_gate<T, BWD>(k[s][v], z[s][v], k[s][v]);
+                gs_gate(k[s][v], z[s][v], k[s][v]);
                 if (i0 + s >= sp.len) k[s][v] = 1.f, u[s][v] = c[s][v] = z[s][v] = 0.f;
                 if (BWD) {
                     B[v] = k[s][v] * (B[v] + u[s][v]);
@@ -372,7 +366,7 @@ __global__ __launch_bounds__(256) void gs_step_kernel(const T* g, const T* c, fl
     const int ch = (int)(i - b * H);
     if (active && !active[b]) return;
     float z, k;
-    gs_gate<T, false>((float)g[b * ldg + ch], z, k);
+    gs_gate((float)g[b * ldg + ch], z, k);
     state[i] = fmaf(k, state[i], z * (float)c[b * ldc + ch]);
 }
 
