@@ -281,15 +281,16 @@ std::tuple<Tensor, Tensor> packed_label_attention(const Tensor& keys, const Tens
 }
 
 struct GatedScan : public torch::autograd::Function<GatedScan> {
-    static GzslGatedScan describe(const Tensor& g, const Tensor& c, const Tensor& spans, int64_t max_len, const Tensor& h0, bool reverse) {
+    static GzslGatedScan describe(const Tensor& g, const Tensor& c, const Tensor& spans, int64_t max_len, const Tensor& h0, bool reverse, const Tensor& rest) {
         GzslGatedScan d{};
         d.gates = g.data_ptr(), d.cands = c.data_ptr(), d.spans = spans.data_ptr<int64_t>(), d.h0 = h0.defined() ? h0.data_ptr<float>() : nullptr;
         d.rows = g.size(0), d.ldg = pitch_of(g), d.ldc = pitch_of(c);
         d.B = (int)spans.size(0), d.max_len = (int)max_len, d.H = (int)g.size(1), d.reverse = reverse, d.dtype = type_of(g, "gates");
+        d.rest = rest.defined() ? rest.data_ptr() : nullptr;
         return d;
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& gates, const Tensor& cands, const Tensor& spans, int64_t max_len,
-                                 const c10::optional<Tensor>& h0_, bool reverse) {
+                                 const c10::optional<Tensor>& h0_, bool reverse, bool grad) {
         TORCH_CHECK(type_of(gates, "gates") == type_of(cands, "cands"), "gzsl: gates and cands must have one type");
         const Tensor g = rows_of(gates, "gates"), c = rows_of(cands, "cands");
         TORCH_CHECK(g.sizes() == c.sizes(), "gzsl: gates / cands shapes differ");
@@ -303,7 +304,9 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
             TORCH_CHECK(h0_->size(0) == spans.size(0) && h0_->size(1) == g.size(1) && h0_->device() == g.device(), "gzsl: h0 is [B, H] on the same device");
             h0 = h0_->contiguous();
         }
-        const GzslGatedScan d = describe(g, c, spans, max_len, h0, reverse);
+        Tensor rest;  // (what a backward needs of 16-bit states)
+        if (grad && g.scalar_type() == at::kBFloat16) rest = at::empty(g.sizes(), g.options());
+        const GzslGatedScan d = describe(g, c, spans, max_len, h0, reverse, rest);
         Tensor h = at::empty(g.sizes(), g.options()), last = at::empty({d.B, d.H}, g.options().dtype(at::kFloat));
         if (d.B == 0) {
             h.zero_();
@@ -311,7 +314,8 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
             const Tensor work = scratch(gzsl_gated_scan_work_bytes(&d, 0), g, "gated_scan");
             check_rc(gzsl_gated_scan_fwd(&d, h.data_ptr(), last.data_ptr<float>(), work.data_ptr(), work.numel(), cur_stream()), "gzsl_gated_scan_fwd");
         }
-        ctx->save_for_backward({g, c, spans, h, h0});
+        if (!grad) return {h, last};
+        ctx->save_for_backward({g, c, spans, h, h0, rest});
         ctx->saved_data["max_len"] = max_len;
         ctx->saved_data["reverse"] = reverse;
         ctx->set_materialize_grads(false);
@@ -320,9 +324,9 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         check_once("gated_scan");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &g = saved[0], &c = saved[1], &spans = saved[2], &h = saved[3], &h0 = saved[4];
+        const Tensor &g = saved[0], &c = saved[1], &spans = saved[2], &h = saved[3], &h0 = saved[4], &rest = saved[5];
         const c10::DeviceGuard guard(g.device());
-        const GzslGatedScan d = describe(g, c, spans, ctx->saved_data["max_len"].toInt(), h0, ctx->saved_data["reverse"].toBool());
+        const GzslGatedScan d = describe(g, c, spans, ctx->saved_data["max_len"].toInt(), h0, ctx->saved_data["reverse"].toBool(), rest);
         Tensor dg = at::empty(g.sizes(), g.options()), dc = at::empty(g.sizes(), g.options()), dh0;
         if (h0.defined()) dh0 = at::empty_like(h0);
         if (d.B == 0) {
@@ -334,12 +338,13 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
                                          dc.data_ptr(), h0.defined() ? dh0.data_ptr<float>() : nullptr, work.data_ptr(), work.numel(), cur_stream()),
                      "gzsl_gated_scan_bwd");
         }
-        return {dg, dc, Tensor(), Tensor(), dh0, Tensor()};
+        return {dg, dc, Tensor(), Tensor(), dh0, Tensor(), Tensor()};
     }
 };
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& gates, const Tensor& cands, const Tensor& spans, int64_t max_len, const c10::optional<Tensor>& h0,
                                       bool reverse) {
-    auto out = GatedScan::apply(gates, cands, spans, max_len, h0, reverse);
+    const bool grad = at::GradMode::is_enabled() && (gates.requires_grad() || cands.requires_grad() || (h0.has_value() && h0->requires_grad()));
+    auto out = GatedScan::apply(gates, cands, spans, max_len, h0, reverse, grad);
     return {out[0], out[1]};
 }
 

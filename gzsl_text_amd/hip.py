@@ -44,7 +44,7 @@ class GzslGatedScan(ctypes.Structure):
     """Mirror of `struct GzslGatedScan` (include/gzsl_hip.h)."""
     _fields_ = [('gates', c_void_p), ('cands', c_void_p), ('spans', c_void_p), ('h0', c_void_p),
                 ('rows', c_ll), ('ldg', c_ll), ('ldc', c_ll),
-                ('B', c_int), ('max_len', c_int), ('H', c_int), ('reverse', c_int), ('dtype', c_int)]
+                ('B', c_int), ('max_len', c_int), ('H', c_int), ('reverse', c_int), ('dtype', c_int), ('rest', c_void_p)]
 
 
 # name -> argtypes (every entry point include/gzsl_hip.h declares; tests check the export list against the header)
@@ -102,6 +102,7 @@ _PROTOS = {
     'gzsl_packed_attn_fwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 4 + [c_ll, c_void_p],
     'gzsl_packed_attn_bwd': [ctypes.POINTER(GzslPackedAttn)] + [c_void_p] * 8 + [c_ll, c_void_p],
     'gzsl_gated_scan_work_bytes': [ctypes.POINTER(GzslGatedScan), c_int],
+    'gzsl_gated_scan_rest_bytes': [ctypes.POINTER(GzslGatedScan)],
     'gzsl_gated_scan_fwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 3 + [c_ll, c_void_p],
     'gzsl_gated_scan_bwd': [ctypes.POINTER(GzslGatedScan)] + [c_void_p] * 7 + [c_ll, c_void_p],
     'gzsl_gated_scan_step': [c_void_p] * 4 + [c_int, c_int, c_ll, c_ll, c_int, c_void_p],

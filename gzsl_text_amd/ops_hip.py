@@ -550,7 +550,7 @@ class HipOps:
             raise RuntimeError(f'{name[:-len("_work_bytes")]}: unsupported arguments (GZSL_EINVAL)')
         return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
-    def _gated_scan(self, gates, cands, spans, max_len, h0, reverse):
+    def _gated_scan(self, gates, cands, spans, max_len, h0, reverse, rest=None):
         dt = self._dtype(gates, cands)
         gates, cands = self._rows(gates, 'gates'), self._rows(cands, 'cands')
         self._spans(spans, max_len)
@@ -560,29 +560,37 @@ class HipOps:
         if h0 is not None and tuple(h0.shape) != (spans.shape[0], gates.shape[1]):
             raise RuntimeError(f'h0 {tuple(h0.shape)} does not fit {(spans.shape[0], gates.shape[1])}')
         d = hip.GzslGatedScan(dptr(gates), dptr(cands), ptr(spans), ptr(h0), gates.shape[0], self._ld(gates), self._ld(cands),
-                              spans.shape[0], max_len, gates.shape[1], int(bool(reverse)), dt)
+                              spans.shape[0], max_len, gates.shape[1], int(bool(reverse)), dt, ptr(rest))
         return d, (gates, cands)
 
-    def gated_scan_fwd(self, gates, cands, spans, max_len, h0=None, reverse=False):
+    def gated_scan_fwd(self, gates, cands, spans, max_len, h0=None, reverse=False, need_grad=False):
         """(h [R,H], h_last [B,H] fp32): h_t = (1 - z_t) h_{t-1} + z_t cands_t with z = sigmoid(gates), through every note's
-        rows (backwards when `reverse`) from h0 [B,H] fp32 (None: zeros).  Rows of no note get zeros."""
-        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse)
+        rows (backwards when `reverse`) from h0 [B,H] fp32 (None: zeros).  Rows of no note get zeros.  need_grad: (h, h_last,
+        rest), rest being what gated_scan_bwd takes (bf16: what the rounding of h dropped; fp32: None)."""
+        rest = torch.empty(gates.shape, dtype=torch.bfloat16, device=gates.device) if need_grad and gates.dtype == torch.bfloat16 else None
+        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse, rest)
         h = torch.empty(gates.shape, dtype=gates.dtype, device=gates.device)
         last = torch.empty((d.B, d.H), dtype=torch.float32, device=gates.device)
         if d.B == 0:
-            return h.zero_(), last
-        work = self._work('gzsl_gated_scan_work_bytes', d, 0, gates.device)
-        call('gzsl_gated_scan_fwd', d, ptr(h), ptr(last), ptr(work), work.numel())
+            h.zero_()
+        else:
+            work = self._work('gzsl_gated_scan_work_bytes', d, 0, gates.device)
+            call('gzsl_gated_scan_fwd', d, ptr(h), ptr(last), ptr(work), work.numel())
         del hold
-        return h, last
+        return (h, last, rest) if need_grad else (h, last)
 
-    def gated_scan_bwd(self, dh, dlast, h, gates, cands, spans, max_len, h0=None, reverse=False):
-        """(dgates, dcands, dh0) of gated_scan_fwd; dh [R,H] or dlast [B,H] may be None (zeros)."""
-        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse)
-        self._dtype(gates, h, dh)
+    def gated_scan_bwd(self, dh, dlast, h, gates, cands, spans, max_len, h0=None, reverse=False, rest=None):
+        """(dgates, dcands, dh0) of gated_scan_fwd; dh [R,H] or dlast [B,H] may be None (zeros).  bf16 without the forward's rest:
+        the forward is run once more for it."""
+        if rest is None and gates.dtype == torch.bfloat16:
+            h, _, rest = self.gated_scan_fwd(gates, cands, spans, max_len, h0, reverse, need_grad=True)
+        d, hold = self._gated_scan(gates, cands, spans, max_len, h0, reverse, rest)
+        self._dtype(gates, h, dh, rest)
         _check_f32(dlast)
         if h.shape != gates.shape or (dh is not None and dh.shape != h.shape) or (dlast is not None and tuple(dlast.shape) != (d.B, d.H)):
             raise RuntimeError('gated_scan_bwd: h / dh / dlast do not fit the gates')
+        if rest is not None and rest.shape != h.shape:
+            raise RuntimeError('rest is not that of this call\'s forward')
         dg, dc = (torch.empty(gates.shape, dtype=gates.dtype, device=gates.device) for _ in range(2))
         dh0 = torch.empty((d.B, d.H), dtype=torch.float32, device=gates.device)
         if d.B == 0:

@@ -312,8 +312,13 @@ typedef struct GzslGatedScan {
     const float* h0;
     long long rows, ldg, ldc;
     int B, max_len, H, reverse, dtype;
+    void* rest; /* [rows, H] or NULL */
 } GzslGatedScan;
 long long gzsl_gated_scan_work_bytes(const GzslGatedScan* d, int backward);
+/* `rest` of a bf16 call: gzsl_gated_scan_rest_bytes(d) bytes (fp32: 0, not used) that the forward fills with what the rounding of h
+ * dropped and the backward takes.  Without it the backward works from the rounded h, whose rounding then enters dgates (2.7 times the
+ * error of a rounded result where the states settle near candidates of mean 3 and deviation 1). */
+long long gzsl_gated_scan_rest_bytes(const GzslGatedScan* d);
 int gzsl_gated_scan_fwd(const GzslGatedScan* d, void* h, float* h_last, void* work, long long work_bytes, void* stream);
 /* dgates, dcands [rows,H] written (zero in rows of no note), dh0 [B,H] written (may be NULL), from dh [rows,H] and dlast [B,H]
  * fp32 (either may be NULL: zero) and the forward's h. */

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.packed_ref import U, scan_ref, within
+from tests.packed_ref import U, half_step, scan_ref, within
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -30,6 +30,42 @@ def make(lens, H, dtype, seed, bias=-1.0, mean=0.0, first=1.0):
     g, c, h0, dh, dl = 1.5 * rnd(rows, H) + bias, rnd(rows, H) + mean, first * rnd(len(lens), H), rnd(rows, H), rnd(len(lens), H)
     return (g.to(dtype).to(DEV), c.to(dtype).to(DEV), table, max_len, h0.to(DEV), dh.to(dtype).to(DEV), dl.to(DEV),
             [tuple(x) for x in table.tolist()])
+
+
+def ref_once(g, c, sl, h0, reverse, dh, dl):
+    """scan_ref for results that are rounded to the tensors' type once, at the end: the bounds of the same numbers as fp32 tensors, that
+    rounding, and in dgates the state in front of a step as it is kept for the backward, in two pieces (off by half_step^2)."""
+    step = half_step(g.dtype)
+    ref = scan_ref(g.float(), c.float(), sl, h0, reverse, dh.float(), dl)
+    if g.dtype == torch.float32:
+        return ref
+    h, dc = ref['h'][0], ref['dc'][0]
+    before = torch.zeros_like(h)
+    for b, (s, n) in enumerate(sl):
+        if n:
+            rows = h[s:s + n].flip(0) if reverse else h[s:s + n]
+            x = torch.cat([h0[b:b + 1].cpu().double(), rows[:-1]])
+            before[s:s + n] = x.flip(0) if reverse else x
+    extra = dict(dg=dc.abs() * torch.sigmoid(-g.detach().cpu().double()) * before.abs() * step * step)
+    for name in ('h', 'dg', 'dc'):
+        val, err = ref[name]
+        err = err + extra.get(name, 0.0)
+        ref[name] = (val, err + (val.abs() + err) * step)
+    return ref
+
+
+@pytest.mark.parametrize('reverse', [False, True], ids=['ahead', 'back'])
+@pytest.mark.parametrize('lens,H,mean,bias', [([70, 0, 31], 40, 3.0, -1.0), ([300, 45], 7, 3.0, 1.0), ([700], 100, 0.0, -1.0), ([129, 64], 64, 10.0, 0.0),
+                                              ([2100], 16, 3.0, -1.0)])
+def test_16_bit_gradients_are_rounded_once(ops, ext, lens, H, mean, bias, reverse):
+    """Candidates off centre: the state settles near them, and c - h_{t-1} in the gate's gradient cancels."""
+    g, c, spans, max_len, h0, dh, dl, sl = make(lens, H, torch.bfloat16, 3, bias, mean)
+    ref = ref_once(g, c, sl, h0, reverse, dh, dl)
+    a = [x.clone().requires_grad_(True) for x in (g, c, h0)]
+    h, last = ext.gated_scan(a[0], a[1], spans, max_len, a[2], reverse)
+    torch.autograd.backward((h, last), (dh, dl))
+    for name, x in zip(('h', 'last', 'dg', 'dc', 'dh0'), (h, last, *[t.grad for t in a])):
+        within(x, ref[name], name)
 
 
 def test_a_far_state_through_open_gates(ops, ext):
