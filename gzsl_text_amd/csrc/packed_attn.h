@@ -243,14 +243,15 @@ struct PaArgs {
     const void *keys, *values, *queries;
     const int64_t* spans;
     long long rows, ldk, ldv, ldq;
-    int B, max_len, L, E, F, nT, nQ;  // nT: token tiles of the longest note, nQ: label tiles
+    int B, max_len, L, E, F, nT, nQ;  // nT: token tiles of the longest note (0: images by rows, see pa_images), nQ: label tiles
+    int slots;                        // token tiles that have an image
     float cap;
     uint32_t l_offset, L_total, seed, thresh;
     float scale;
     int join_rows;                    // rows of a workgroup of pa_kv_finish_kernel
     int nLT, extra, least;            // label workgroups of a note; token chunks beyond one a note (0: notes are not cut), their tokens at least
     // workspace
-    char *TK, *Q, *DO;  // images: token tiles [B][nT], queries [nQ], dO [B][nQ]
+    char *TK, *Q, *DO;  // images: token tiles [slots], queries [nQ], dO [B][nQ]
     float *part, *ml;  // forward, notes cut: unnormalised O [chunk][L][F] and (max, sum) [chunk][L][2]
     float *dq, *dkv;   // backward: [chunk][L][E]; [slab][PA_TILE][E + F]
     // results and the backward's inputs
@@ -260,6 +261,25 @@ struct PaArgs {
     const float *cLSE, *crest;
     void *dK, *dV, *dQ;
 };
+
+// ---- where a token tile's image lies.  [B][nT] where that is at most PA_WASTE times what disjoint notes can fill.  Otherwise, of notes of
+// very different lengths (512 notes of 200000 rows, one of 65536: 67 GB), by rows: a note's first tile at [b], its tile t behind B at
+// start / ROWS + t - 1.  Of disjoint notes no two meet there, in whatever order the table has them: the row in front of a tile t > 0 is
+// its own note's, and so is every row of ROWS in front, so no other tile t > 0 begins in the same ROWS rows.
+#define PA_WASTE 4
+struct PaImages {
+    const char *first, *rest;
+    long long bytes;
+    __device__ __forceinline__ const char* operator()(int t) const { return (t ? rest : first) + t * bytes; }
+};
+template <int ROWS>
+__device__ __forceinline__ PaImages pa_images(const PaArgs& a, int b, long long start, int kb) {
+    PaImages m;
+    m.bytes = 1024LL * kb;
+    m.rest = a.TK + (a.nT ? (long long)b * a.nT : a.B + start / ROWS - 1) * m.bytes;
+    m.first = a.nT ? m.rest : a.TK + b * m.bytes;
+    return m;
+}
 
 // ---- how the work is cut.  The host knows max_len, not the lengths: every wave works the cut out from the span table, so the
 // kernels agree on it without a table in memory.  Per 64 notes: one load and a few lane exchanges.
@@ -378,6 +398,32 @@ __device__ __forceinline__ PaTile pa_tile(const PaArgs& a, int i) {
     }
     return u;
 }
+// The token tile whose image is at `slot` (b = -1: none).
+template <int ROWS>
+__device__ __forceinline__ PaTile pa_slot(const PaArgs& a, int slot) {
+    PaTile u;
+    u.b = -1;
+    if (a.nT || slot < a.B) {
+        u.b = a.nT ? slot / a.nT : slot, u.tile = a.nT ? slot % a.nT : 0;
+        u.sp = note_span(a.spans, u.b, a.rows, a.max_len);
+        if ((long long)u.tile * ROWS >= u.sp.len) u.b = -1;
+        return u;
+    }
+    const int lane = threadIdx.x & 63;
+    const long long cell = slot - a.B + 1;
+    for (int b0 = 0; b0 < a.B && u.b < 0; b0 += 64) {
+        const NoteSpan sp = b0 + lane < a.B ? note_span(a.spans, b0 + lane, a.rows, a.max_len) : NoteSpan{0, 0};
+        const long long t = cell - sp.start / ROWS;
+        const unsigned long long hit = __ballot(t > 0 && t * ROWS < sp.len);
+        if (hit) {
+            const int src = __ffsll((long long)hit) - 1;
+            u.b = b0 + src;
+            u.sp = {pa_scalar(__shfl(sp.start, src)), pa_scalar(__shfl(sp.len, src))};
+            u.tile = (int)(cell - u.sp.start / ROWS);
+        }
+    }
+    return u;
+}
 struct PaRuns {
     int steps, per, units;  // in all, of a run (the last may be shorter), runs
     __device__ __forceinline__ PaRuns(long long tiles, int nQ) {
@@ -389,6 +435,7 @@ struct PaRuns {
 };
 
 struct PaPlan {
+    long long slots;
     int max_len, nT, nQ, kind, waves, extra, least, units, nLT;  // kind: 0 PaBF, 1 PaBF wide, 2 PaX3, 3 PaF32 (wide: E > 112)
     long long kv, q, dO, part, ml, dq, dkv, bytes;
 };

@@ -6,7 +6,10 @@ static inline long long up256(long long n) { return (n + 255) / 256 * 256; }
 template <class G>
 static void pa_sizes(PaPlan& p, const GzslPackedAttn& d, int backward) {
     p.nT = (int)(((long long)p.max_len + G::ROWS - 1) / G::ROWS), p.nQ = (int)(((long long)d.L + G::ROWS - 1) / G::ROWS);
-    p.kv = 1024LL * d.B * p.nT * (backward ? G::TOK : G::FWD);
+    const long long most = d.rows / G::ROWS + d.B;  // tiles that disjoint notes can have
+    p.slots = (long long)d.B * p.nT;
+    if (p.slots > PA_WASTE * most) p.slots = most, p.nT = 0;
+    p.kv = 1024LL * p.slots * (backward ? G::TOK : G::FWD);
     p.q = 1024LL * p.nQ * (backward ? G::QRY : G::PL * G::RE);
     p.dO = backward ? 1024LL * d.B * p.nQ * G::OUT : 0;
 }
@@ -38,7 +41,8 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
     p.extra = wgs > 0 && wgs < 256 && p.max_len > p.least ? cdiv(p.waves == 4 && !backward ? 512 : 256, p.nLT) : 0;
     if (p.extra > (long long)d->B * (p.max_len / p.least + 1)) p.extra = d->B * (p.max_len / p.least + 1);
     const long long chunks = d->B + p.extra;
-    if ((long long)d->B * p.nT + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
+    if (fits) p.kv = p.q = 0;
+    if (p.slots + p.nQ > 0x3FFFFFFF || chunks * p.nLT > 0x3FFFFFFF || (long long)d->B * p.nQ > 0x3FFFFFFF || (long long)d->B * d->L > 0x3FFFFFFF)
         return GZSL_ETOOBIG;
     if (!backward && p.extra > 0) {
         p.part = up256(4 * chunks * d->L * d->F);
@@ -55,13 +59,13 @@ static int pa_plan(const GzslPackedAttn* d, int backward, PaPlan& p) {
         p.units = most >= PA_UNITS * PA_RUN || most * p.nQ >= PA_UNITS * PA_RUN ? PA_UNITS : (int)((most * p.nQ + PA_RUN - 1) / PA_RUN);
         p.dkv = up256(8LL * p.units * PA_TILE * (d->E + d->F));
     }
-    p.bytes = p.kv + p.q + p.dO + p.part + p.ml + p.dq + p.dkv;
+    p.bytes = p.kv + p.q + p.dO + p.part + p.ml + p.dq + p.dkv + 256;
     return 0;
 }
 static void pa_fill(PaArgs& a, const GzslPackedAttn& d, const PaPlan& p, void* work) {
     a.keys = d.keys, a.values = d.values, a.queries = d.queries, a.spans = d.spans;
     a.rows = d.rows, a.ldk = d.ldk, a.ldv = d.ldv, a.ldq = d.ldq;
-    a.B = d.B, a.max_len = p.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ;
+    a.B = d.B, a.max_len = p.max_len, a.L = d.L, a.E = d.E, a.F = d.F, a.nT = p.nT, a.nQ = p.nQ, a.slots = (int)p.slots;
     a.cap = d.cap, a.l_offset = (uint32_t)d.l_offset, a.L_total = (uint32_t)d.L_total, a.seed = d.seed, a.thresh = d.drop_thresh, a.scale = d.drop_scale;
     a.nLT = p.nLT, a.extra = p.extra, a.least = p.least;
     // few rows: one a wave, for the time of one row's parts to come in (1000 tokens x 428 labels: 31 us with four a wave, 12 so); many: four,

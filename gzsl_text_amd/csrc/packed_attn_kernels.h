@@ -96,18 +96,19 @@ __device__ __forceinline__ void pa_emit(typename K::T (*sh)[P], char* img, int t
         pa_put<K, N>(img, i, pa_cut<K, G>(x), lane);
     }
 }
-// Blocks [0, B nT): a token tile (keys, values); then nQ blocks of queries.  Memory-bound: reads each operand once, writes its image
+// Blocks [0, slots): a token tile (keys, values); then nQ blocks of queries.  Memory-bound: reads each operand once, writes its image
 // (17404 tokens of 200 + 200 bf16: 8 us).
 template <class K, class G, bool BWD>
 __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
     typedef typename K::T T;
     constexpr int PE = G::SE * G::KK, PF = G::SF * G::KK;
     __shared__ __attribute__((aligned(16))) T se[G::ROWS][PE + 16 / sizeof(T)], sf[G::ROWS][PF + 16 / sizeof(T)];
-    const int id = blockIdx.x, nTok = a.B * a.nT, tid = threadIdx.x;
-    if (id < nTok) {
-        const int b = id / a.nT, t = id % a.nT;
-        const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len);
-        if (t * G::ROWS >= sp.len) return;
+    const int id = blockIdx.x, tid = threadIdx.x;
+    if (id < a.slots) {
+        const PaTile un = pa_slot<G::ROWS>(a, id);
+        if (un.b < 0) return;
+        const int t = un.tile;
+        const NoteSpan sp = un.sp;
         pa_stage<T, G::ROWS>(se, (const T*)a.keys + sp.start * a.ldk, a.ldk, t * G::ROWS, sp.len, a.E, tid);
         pa_stage<T, G::ROWS>(sf, (const T*)a.values + sp.start * a.ldv, a.ldv, t * G::ROWS, sp.len, a.F, tid);
         __syncthreads();
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
             if (!G::TRT) pa_emit<K, G, G::NE, 1, false>(se, img + G::PL * G::RF * 1024, tid);
         }
     } else {
-        const int q = id - nTok;
+        const int q = id - a.slots;
         pa_stage<T, G::ROWS>(se, (const T*)a.queries, a.ldq, q * G::ROWS, a.L, a.E, tid);
         __syncthreads();
         char* img = a.Q + (long long)q * (BWD ? G::QRY : G::PL * G::RE) * 1024;
@@ -362,12 +363,12 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void pa_fwd_kernel(PaArgs a) {
 #pragma unroll
         for (int s = 0; s < G::SE; ++s) w.qf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
     }
-    const char* tk = a.TK + (long long)b * a.nT * G::FWD * 1024;
-    if (t0 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)t0 * G::FWD * 1024, sm, wave, lane);
+    const PaImages tk = pa_images<G::ROWS>(a, b, un.sp.start, G::FWD);
+    if (t0 < t1) pa_dma<WAVES, G::FWD>(tk(t0), sm, wave, lane);
     pa_arrive();
     auto step = [&](int t, auto last) {
         const char* KR = sm + ((t - t0) & 1) * G::FWD * 1024;
-        if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk + (long long)(t + 1) * G::FWD * 1024, sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
+        if (t + 1 < t1) pa_dma<WAVES, G::FWD>(tk(t + 1), sm + ((t - t0 + 1) & 1) * G::FWD * 1024, wave, lane);
         if (!idle) pa_fwd_tile<K, G, CAP, DROP, decltype(last)::value>(w, a, cap, KR, KR + G::PL * G::RE * 1024, t * G::ROWS, len - t * G::ROWS, lane);
         pa_arrive();
     };
@@ -603,7 +604,7 @@ __global__ __launch_bounds__(PA_TILE * 4, 2) void pa_bwd_kv_kernel(PaArgs a) {
         frag kf[G::SE], vf[DK ? G::SF : 1];
         {
             const int c = min(tok0, (len - 1) / 16 * 16);
-            const char* img = a.TK + ((long long)b * a.nT + c / G::ROWS) * G::TOK * 1024;
+            const char* img = pa_images<G::ROWS>(a, b, un.sp.start, G::TOK)(pa_scalar(c / G::ROWS));
 #pragma unroll
             for (int s = 0; s < G::SE; ++s) kf[s] = pa_frag<K, G::RE>(img, (c % G::ROWS / 16) * G::SE + s, lane);
             if (DK)
@@ -834,9 +835,9 @@ __global__ __launch_bounds__(WAVES * H * 64, 2) void pa_bwd_q_kernel(PaArgs a) {
     f32x4 dq[G::NE];
 #pragma unroll
     for (int j = 0; j < G::NE; ++j) dq[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const char* tk = a.TK + (long long)b * a.nT * G::TOK * 1024;
+    const PaImages tk = pa_images<G::ROWS>(a, b, un.sp.start, G::TOK);
     auto fetch = [&](int t, int k) {
-        if (t < t1) pa_dma<WAVES, G::TOK>(tk + (long long)t * G::TOK * 1024, sm + (2 * h + (k & 1)) * G::TOK * 1024, wave, lane);
+        if (t < t1) pa_dma<WAVES, G::TOK>(tk(t), sm + (2 * h + (k & 1)) * G::TOK * 1024, wave, lane);
     };
     fetch(t0 + h, 0);
     pa_arrive();
@@ -951,7 +952,7 @@ static int pa_fwd(PaArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((pa_fwd_direct_kernel<K, G, W, CAP, DROP>), dim3(a.B + a.extra), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (W != 8 || a.nLT > 1) {
-        hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((pa_pack_kernel<K, G, false>), dim3(a.slots + a.nQ), dim3(256), 0, st, a);
         hipLaunchKernelGGL((pa_fwd_kernel<K, G, W, OCC, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * 64), 2 * G::FWD * 1024, st, a);
     }
     if (a.extra > 0) {
@@ -966,7 +967,7 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
     typedef typename K::T T;
     constexpr int lds = 2 * (G::QRY + G::OUT) * 1024;
     static_assert(lds <= 160 * 1024 && 2 * H * G::TOK <= 160 && 2 * G::FWD <= 160, "two buffers in LDS");
-    hipLaunchKernelGGL((pa_pack_kernel<K, G, true>), dim3(a.B * a.nT + a.nQ), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((pa_pack_kernel<K, G, true>), dim3(a.slots + a.nQ), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_pack_do_kernel<K, G>), dim3(a.nQ * a.B), dim3(256), 0, st, a);
     if (p.units > 0) {
         if constexpr (G::PL == 3) {
@@ -976,7 +977,9 @@ static int pa_bwd(PaArgs& a, const PaPlan& p, hipStream_t st) {
             hipLaunchKernelGGL((pa_bwd_kv_kernel<K, G, 3, CAP, DROP>), dim3(p.units), dim3(PA_TILE * 4), lds, st, a);
         }
     }
-    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(a.max_len > 0 ? cdiv(a.max_len, a.join_rows) : 1, a.B + 1), dim3(256), 0, st, a);
+    // (a workgroup's rows repeat every gridDim.x: of many notes and one long one most workgroups would find none)
+    const int gx = cdiv(a.max_len, a.join_rows), most = 65536 / (a.B + 1) + 1;
+    hipLaunchKernelGGL(pa_kv_finish_kernel<T>, dim3(gx < 1 ? 1 : (gx < most ? gx : most), a.B + 1), dim3(256), 0, st, a);
     hipLaunchKernelGGL((pa_bwd_q_kernel<K, G, W, H, CAP, DROP>), dim3(a.nLT * (a.B + a.extra)), dim3(W * H * 64), 2 * H * G::TOK * 1024, st, a);
     const long long n = (long long)a.L * a.E;
     if (n <= 64 * 512 && a.B + a.extra > 32) hipLaunchKernelGGL((pa_q_join_kernel<T, G::ROWS, 16>), dim3((unsigned)cdiv((long)n, 64)), dim3(1024), 0, st, a);

@@ -63,3 +63,16 @@ def test_caps_below_and_about_the_scores(ops, dtype, cap):
     got, ref = run(ops, k, v, q, do, spans, max_len, cap), attn_ref_range(k, v, q, sl, cap, do)
     for name in ('O', 'lse', 'dV'):
         within(got[name], ref[name], f'{name} at cap {cap:g}')
+
+
+@BOTH
+@pytest.mark.parametrize('E,L', [(36, 150), (113, 150), (200, 1100)])
+def test_one_long_note_among_many(ops, dtype, E, L):
+    """Notes of very different lengths: token images are numbered by rows, not by the longest note."""
+    gen = torch.Generator().manual_seed(3)
+    lens = [int(x) for x in torch.randint(0, 40, (70,), generator=gen)]
+    lens[41], lens[42] = 901, 64
+    k, v, q, do, spans, max_len, sl = make(lens, E, 52, L, dtype, seed=12, tail=3)
+    got, ref = run(ops, k, v, q, do, spans, max_len, 6.0), attn_ref_range(k, v, q, sl, 6.0, do)
+    for name, x in got.items():
+        within(x, ref[name], name)

@@ -188,3 +188,24 @@ def test_overlapping_tensors_are_found():
     for written, read in (([x, x], ()), ([x[:6], x[5:]], ()), ([x[2:4]], [x]), ([x], [x[9:]]), ([x[:1], x], [x])):
         with pytest.raises(RuntimeError, match='overlap'):
             HipOps._apart(written, read)
+
+
+@lib_built
+@pytest.mark.parametrize('E', [100, 200])
+@pytest.mark.parametrize('dtype', [hip.F32, hip.BF16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('B,rows,max_len,L', [(64, 103000, 40000, 300), (16, 55000, 40000, 300), (1000, 200000, 60000, 500)])
+def test_one_long_note_among_many_takes_workspace_for_the_rows_there_are(B, rows, max_len, L, dtype, E):
+    """Scratch for what is read and written: at most ten times the inputs, the output and its gradient, and the fixed shares of the
+    chip's workgroups (256 pieces of a [L, F] output; 512 of 128 tokens); sized for a padded batch it was up to 60 times."""
+    lib, F, w = hip.load(), 200, 4 if dtype == hip.F32 else 2
+    d = attn(rows=rows, ldk=E, ldv=F, ldq=E, B=B, max_len=max_len, L=L, E=E, F=F, dtype=dtype, L_total=L)
+    data = w * (rows * (E + F) + L * E + B * L * F)
+    for backward in (0, 1):
+        assert 0 < lib.gzsl_packed_attn_work_bytes(d, backward) < 10 * data + 4 * (256 + B) * L * max(E, F) + 8 * 256 * 128 * (E + F)
+
+
+@lib_built
+def test_few_labels_need_no_images():
+    lib = hip.load()
+    d = attn(rows=40000, B=1, max_len=40000, L=50, E=100, F=200, ldk=100, ldv=200, ldq=100, L_total=50)
+    assert lib.gzsl_packed_attn_work_bytes(d, 0) < 4 * 300 * 50 * 202 + 1024
