@@ -349,6 +349,9 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& gates, const Tensor& cands, 
 }
 
 void gated_scan_step_(const Tensor& gates, const Tensor& cands, const Tensor& state, const c10::optional<Tensor>& active) {
+    // autograd would take the state behind the step for the one in front of it, and miss the gates and candidates
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(gates.requires_grad() || cands.requires_grad() || state.requires_grad()),
+                "gzsl: gated_scan_step_ is not differentiable: call gated_scan, or the step under no_grad or on detached tensors");
     const int t = type_of(gates, "gates");
     TORCH_CHECK(type_of(cands, "cands") == t, "gzsl: gates and cands must have one type");
     check_f32_cuda(state, "state", 2);
@@ -477,7 +480,7 @@ TORCH_LIBRARY_IMPL(gzsl, Autograd, m) {
     m.impl("ldam_bce", ldam_bce);
     m.impl("packed_label_attention", packed_label_attention);
     m.impl("gated_scan", gated_scan);
-    m.impl("gated_scan_step_", gated_scan_step_);  // (in place and not differentiable: parameters may require grad)
+    m.impl("gated_scan_step_", gated_scan_step_);  // (in place and not differentiable: refused where a gradient would be missed)
     m.impl("clip_grad_norm_", clip_grad_norm_);
     m.impl("adamw_clip_step_", adamw_clip_step_);
 }

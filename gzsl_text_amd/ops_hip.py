@@ -602,7 +602,9 @@ class HipOps:
 
     def gated_scan_step_(self, gates, cands, state, active=None):
         """One token of every running note: state [B,H] fp32 <- (1 - z) state + z cands, z = sigmoid(gates); rows whose
-        `active` [B] (bool) is False keep theirs."""
+        `active` [B] (bool) is False keep theirs.  Not differentiable: raises where a gradient would be missed."""
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (gates, cands, state)):
+            raise RuntimeError('gated_scan_step_ is not differentiable: call gated_scan, or the step under no_grad or on detached tensors')
         dt = self._dtype(gates, cands)
         _check_f32(state)
         gates, cands = self._rows(gates, 'gates'), self._rows(cands, 'cands')

@@ -209,3 +209,22 @@ def test_few_labels_need_no_images():
     lib = hip.load()
     d = attn(rows=40000, B=1, max_len=40000, L=50, E=100, F=200, ldk=100, ldv=200, ldq=100, L_total=50)
     assert lib.gzsl_packed_attn_work_bytes(d, 0) < 4 * 300 * 50 * 202 + 1024
+
+
+@pytest.mark.parametrize('which', [0, 1, 2], ids=['gates', 'cands', 'state'])
+def test_a_step_that_autograd_would_miss_is_refused(ext, which):
+    """A leaf or a result that wants a gradient, in either binding; no_grad and detached tensors pass this check (and are then
+    refused for standing on the CPU)."""
+    from gzsl_text_amd.ops_hip import HipOps
+    for step in (ext.gated_scan_step_, HipOps().gated_scan_step_):
+        for result in (False, True):
+            t = [torch.zeros(2, 3) for _ in range(3)]
+            t[which].requires_grad_()
+            if result:
+                t[which] = t[which] * 2
+            with pytest.raises(RuntimeError, match='not differentiable'):
+                step(*t)
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match='GPU|CPU|cuda|device'):
+                step(*t)
+            with pytest.raises((RuntimeError, NotImplementedError), match='GPU|CPU|cuda|device'):
+                step(*[x.detach() for x in t])
