@@ -129,6 +129,20 @@ __device__ __forceinline__ void pa_split(float x, bf16& h, bf16& m, bf16& l) {  
     m = (bf16)r;
     l = (bf16)(r - (float)m);
 }
+// An input of any value.  An infinity as (+-1, 0, +-inf): it meets the other operand's first piece alone, whose sign is the number's, and
+// not the lower ones, which may be zero or of the other sign; two infinities meet twice, with one sign.  What would round to an
+// infinity is cut instead.
+#define PA_ROUNDS_OVER 0x1.ffp127f  // the least number that rounds to an infinite bf16
+__device__ __forceinline__ void pa_split_any(float x, bf16& h, bf16& m, bf16& l) {
+    if (fabsf(x) == INFINITY) {
+        h = (bf16)copysignf(1.f, x), m = (bf16)0.f, l = (bf16)x;
+    } else if (fabsf(x) >= PA_ROUNDS_OVER) {
+        const float c = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), r = x - c;
+        h = (bf16)c, m = (bf16)r, l = (bf16)(r - (float)m);
+    } else {
+        pa_split(x, h, m, l);
+    }
+}
 __device__ __forceinline__ void pa_pack(const float (&p)[2][4], PaPieces& out) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

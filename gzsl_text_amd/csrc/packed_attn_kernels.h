@@ -11,12 +11,21 @@ __device__ __forceinline__ typename K::frag pa_cut(const typename K::T (&x)[G::K
         return __builtin_bit_cast(typename K::frag, x);
     } else {
         PaPieces f;
+        float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             bf16 h, m, l;
             pa_split(x[j], h, m, l);
             f.p[0][j] = h, f.p[1][j] = m, f.p[2][j] = l;
+            top = fmaxf(top, fabsf(x[j]));
         }
+        if (__any(top >= PA_ROUNDS_OVER))
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                bf16 h, m, l;
+                pa_split_any(x[j], h, m, l);
+                f.p[0][j] = h, f.p[1][j] = m, f.p[2][j] = l;
+            }
         return f;
     }
 }

@@ -76,3 +76,38 @@ def test_one_long_note_among_many(ops, dtype, E, L):
     got, ref = run(ops, k, v, q, do, spans, max_len, 6.0), attn_ref_range(k, v, q, sl, 6.0, do)
     for name, x in got.items():
         within(x, ref[name], name)
+
+
+@BOTH
+@pytest.mark.parametrize('lens,E,F,L', [([150, 31, 1], 100, 64, 33), ([40, 70], 112, 52, 150), ([150, 31], 113, 52, 33), ([77, 0, 130], 200, 64, 300)])
+@pytest.mark.parametrize('value', ['lowest'])
+def test_tokens_masked_by_a_column_of_the_keys(ops, lens, E, F, L, dtype, value):
+    """A column in which every query has 1 and a masked token's key minus infinity or the type's lowest value: its weight and its gradients
+    are 0, those of the others the exact ones.  A note's last token, a note's first ones, every second one."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=14)
+    low = float('-inf') if value == 'infinite' else torch.finfo(dtype).min
+    q[:, -1], k[:, -1] = 1, 0
+    for s, n in sl:
+        k[s:s + n // 4, -1] = low
+        if n > 1:
+            k[s + n - 1, -1] = low
+        k[s + n // 2:s + 3 * n // 4:2, -1] = low
+    got, ref = run(ops, k, v, q, do, spans, max_len), attn_ref_range(k, v, q, sl, 0.0, do)
+    for name in ('O', 'lse', 'dV', 'dK'):
+        within(got[name], ref[name], name)
+    within(got['dQ'][:, :-1], [x[:, :-1] for x in ref['dQ']], 'dQ')  # (of the column: 0 times infinity)
+    out = k[:, -1] == low
+    assert not got['dK'][out].any() and not got['dV'][out].any()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32])
+@pytest.mark.parametrize('E,L', [(100, 33), (100, 200), (200, 33), (200, 200)])
+def test_infinite_values(ops, E, L, dtype):
+    """An infinite value makes its column of the note's rows infinite, and nothing else."""
+    k, v, q, do, spans, max_len, sl = make([70, 33], E, 40, L, dtype, seed=17)
+    v[5, 3], v[90, 11] = float('inf'), float('-inf')
+    O, lse, _ = ops.attn_packed_fwd(k, v, q, spans, max_len, 7.0, need_grad=False)
+    ref = attn_ref_range(k, v, q, sl, 7.0)
+    assert torch.isposinf(O[0, :, 3]).all() and torch.isneginf(O[1, :, 11]).all()
+    within(O, ref['O'], 'O')
+    within(lse, ref['lse'], 'lse')
