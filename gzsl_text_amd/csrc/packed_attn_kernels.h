@@ -39,9 +39,9 @@ __device__ __forceinline__ void pa_put(char* img, int i, const typename K::frag&
     }
 }
 // ------------------------------------------------------------------------------------------------------------- pre-pass
-// A tile's rows into LDS, zeros past nrows (at least 1) and past W (row stride P elements).  Addresses are clamped, not branched around,
+// A tile's rows into LDS, zeros past nrows (at least 1; REPEAT: its last row again) and past W (row stride P elements).  Addresses are clamped, not branched around,
 // and loaded in batches: a batch is on its way together.
-template <typename T, int ROWS, int P>
+template <typename T, int ROWS, bool REPEAT = false, int P>
 __device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld, int row0, int nrows, int W, int tid) {
     if (((uintptr_t)src & 15) == 0 && ld % (16 / sizeof(T)) == 0 && W % (16 / sizeof(T)) == 0) {
         constexpr int V = 16 / sizeof(T), C = P / V, N = (ROWS * C + 255) / 256;
@@ -55,7 +55,7 @@ __device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld,
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 256 * i, r = c / C, e = c % C * V;
-            if (!(row0 + r < nrows && e < W))
+            if (!((REPEAT || row0 + r < nrows) && e < W))
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[i][k] = (T)0.f;
             if (c < ROWS * C) *reinterpret_cast<vec*>(&sh[r][e]) = v[i];
@@ -73,7 +73,7 @@ __device__ __forceinline__ void pa_stage(T (*sh)[P], const T* src, long long ld,
 #pragma unroll
             for (int i = 0; i < D; ++i) {
                 const int c = tid + 256 * (i0 + i), r = c / P, e = c % P;
-                if (c < ROWS * P) sh[r][e] = row0 + r < nrows && e < W ? v[i] : (T)0.f;
+                if (c < ROWS * P) sh[r][e] = (REPEAT || row0 + r < nrows) && e < W ? v[i] : (T)0.f;
             }
         }
     }
@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
         }
     } else {
         const int q = id - a.slots;
-        pa_stage<T, G::ROWS>(se, (const T*)a.queries, a.ldq, q * G::ROWS, a.L, a.E, tid);
+        // (past the last label that label again, with weights scaled by 0: of zeros an infinite key would make a score that is no number)
+        pa_stage<T, G::ROWS, true>(se, (const T*)a.queries, a.ldq, q * G::ROWS, a.L, a.E, tid);
         __syncthreads();
         char* img = a.Q + (long long)q * (BWD ? G::QRY : G::PL * G::RE) * 1024;
         pa_emit<K, G, G::RE, G::SE, true>(se, img, tid);
@@ -140,8 +141,8 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
     }
 }
 // Backward: dO images of (note, label tile); behind the fragments, for each label, off and scale of its weights
-// P = exp2(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; scale 0 past the
-// last label) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.  Memory-bound
+// P = exp2(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; past the last label its
+// off again and scale 0) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.  Memory-bound
 // (16 x 1999 rows of 200 bf16: 67 MB in 14 us).
 template <class K, class G>
 __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
@@ -185,10 +186,10 @@ __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
     if (tid % TPR == 0) {
         float* aux = reinterpret_cast<float*>(img + (G::OUT - 1) * 1024);
         float off = 0.f, scale = 0.f;
-        if (l < a.L) {
-            if (a.crest) off = a.crest[2 * row], scale = a.crest[2 * row + 1];
-            else off = a.cLSE[row] * PA_LOG2E, scale = 1.f;
-        }
+        const long long at = min(row, (long long)b * a.L + a.L - 1);
+        if (a.crest) off = a.crest[2 * at], scale = a.crest[2 * at + 1];
+        else off = a.cLSE[at] * PA_LOG2E, scale = 1.f;
+        if (l >= a.L) scale = 0.f;
         aux[r] = off;
         aux[G::ROWS + r] = scale;
         aux[2 * G::ROWS + r] = s;

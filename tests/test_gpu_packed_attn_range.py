@@ -80,7 +80,7 @@ def test_one_long_note_among_many(ops, dtype, E, L):
 
 @BOTH
 @pytest.mark.parametrize('lens,E,F,L', [([150, 31, 1], 100, 64, 33), ([40, 70], 112, 52, 150), ([150, 31], 113, 52, 33), ([77, 0, 130], 200, 64, 300)])
-@pytest.mark.parametrize('value', ['lowest'])
+@pytest.mark.parametrize('value', ['infinite', 'lowest'])
 def test_tokens_masked_by_a_column_of_the_keys(ops, lens, E, F, L, dtype, value):
     """A column in which every query has 1 and a masked token's key minus infinity or the type's lowest value: its weight and its gradients
     are 0, those of the others the exact ones.  A note's last token, a note's first ones, every second one."""
@@ -98,6 +98,30 @@ def test_tokens_masked_by_a_column_of_the_keys(ops, lens, E, F, L, dtype, value)
     within(got['dQ'][:, :-1], [x[:, :-1] for x in ref['dQ']], 'dQ')  # (of the column: 0 times infinity)
     out = k[:, -1] == low
     assert not got['dK'][out].any() and not got['dV'][out].any()
+
+
+@BOTH
+@pytest.mark.parametrize('E,L', [(36, 32), (100, 33), (112, 200), (113, 33), (200, 200)])
+def test_infinite_keys_under_a_cap(ops, E, L, dtype):
+    """An infinite element of a key, or of a query, is a score of +-cap: everything but the gradients that multiply it is exact."""
+    k, v, q, do, spans, max_len, sl = make([70, 33], E, 40, L, dtype, seed=15)
+    for x in (k, q):
+        x[x == 0] = 0.5  # (0 times infinity is no number)
+    k[3, 1], k[40, 5], k[69, 1], k[80, 0] = float('inf'), float('-inf'), float('inf'), float('-inf')
+    ref = attn_ref_range(k, v, q, sl, 7.0, do)
+    got = run(ops, k, v, q, do, spans, max_len, 7.0)
+    rest = [e for e in range(E) if e not in (0, 1, 5)]
+    for name in ('O', 'lse', 'dV', 'dK'):
+        within(got[name], ref[name], name)
+    within(got['dQ'][:, rest], [x[:, rest] for x in ref['dQ']], 'dQ')
+    k, v, q, do, spans, max_len, sl = make([70, 33], E, 40, L, dtype, seed=16)
+    for x in (k, q):
+        x[x == 0] = 0.5
+    q[0, 2], q[L - 1, 2], q[L // 2, 4] = float('inf'), float('-inf'), float('-inf')
+    ref = attn_ref_range(k, v, q, sl, 7.0, do)
+    got = run(ops, k, v, q, do, spans, max_len, 7.0)
+    for name in ('O', 'lse', 'dV', 'dQ'):
+        within(got[name], ref[name], name + ' of infinite queries')
 
 
 @pytest.mark.parametrize('dtype', [torch.float32])
