@@ -151,6 +151,15 @@ __device__ __forceinline__ void pa_pack(const float (&p)[2][4], PaPieces& out) {
         out.p[0][j] = h, out.p[1][j] = m, out.p[2][j] = l;
     }
 }
+// Weights p >= 0 in two pieces that are positive where p is, so that an infinite value stays one: the first cut, not rounded, the
+// second with 2^-23 p on top (it stays within 2^-16 p).
+__device__ __forceinline__ void pa_pack_two(const float (&p)[2][4], bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = p[j >> 2][j & 3], c = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+        hi[j] = (bf16)c, lo[j] = (bf16)fmaf(x, 1.f + 0x1p-23f, -c);
+    }
+}
 // what rounding to bf16 dropped
 __device__ __forceinline__ void pa_pack_low(const float (&p)[2][4], bf16x8& out) {
 #pragma unroll

@@ -310,8 +310,8 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
                 w.sum += p[u][r];
                 if (DROP) p[u][r] = gz_u32(w.key, (uint32_t)(t0 + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
             }
-        pa_pack(p, pf);
-        if constexpr (TWO) pa_pack_low(p, pl);
+        if constexpr (TWO) pa_pack_two(p, pf, pl);
+        else pa_pack(p, pf);
     }
     pa_run_ring<G::NF>(ring, ldv, [&](int j, const frag& f) {
         if constexpr (TWO) w.acc[j] = pa_mma(f, pl, w.acc[j]);

@@ -124,7 +124,7 @@ def test_infinite_keys_under_a_cap(ops, E, L, dtype):
         within(got[name], ref[name], name + ' of infinite queries')
 
 
-@pytest.mark.parametrize('dtype', [torch.float32])
+@BOTH
 @pytest.mark.parametrize('E,L', [(100, 33), (100, 200), (200, 33), (200, 200)])
 def test_infinite_values(ops, E, L, dtype):
     """An infinite value makes its column of the note's rows infinite, and nothing else."""
