@@ -184,6 +184,12 @@ __device__ __forceinline__ void pa_fill_ring(F (&ring)[D], LD&& ld) {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+enum { PA_NONE = 0, PA_FORM = 1, PA_SERIES = 2 };  // how scores are capped: pa_scores
+// 2^ of a difference of scores: in units of log 2, or (no cap) of 1
+template <int CAP>
+__device__ __forceinline__ float pa_exp(float d) {
+    return __builtin_amdgcn_exp2f(CAP ? d : d * PA_LOG2E);
+}
 struct PaCap {
     float inv, k1, c2, kt;  // 1 / cap, 2 log2(e) / cap, cap log2(e), 1 / (cap log2(e))
 };
@@ -202,9 +208,9 @@ __device__ __forceinline__ float pa_far(float x, const PaCap& c) {  // cap log2(
 //      holds a larger one: an error relative to the score, whatever the cap.  fp32 tensors, whose products of the gradient still have
 //      that accuracy, and larger caps, at which the closed form's error grows past the scores (at 1e6 weights were off by a fifth).
 //      For small caps of bf16 it is the longer way: 148 us against 138 for 19309 tokens x 9000 labels, weights in one piece.
-enum { PA_NONE = 0, PA_FORM = 1, PA_SERIES = 2 };
 #define PA_CLOSED 64.f
-// Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself.
+// Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself, and
+// maxima stay in its units: in those of log 2 a row of the type's lowest values would run over.
 template <int CAP, int U, bool TH>
 __device__ __forceinline__ void pa_scores(const f32x4 (&x)[U], const PaCap& c, float (&y)[U][4], float (&th)[U][4]) {
     float most = 0.f;
@@ -279,7 +285,7 @@ struct PaArgs {
     float *dq, *dkv;   // backward: [chunk][L][E]; [slab][PA_TILE][E + F]
     // results and the backward's inputs
     void* O;
-    float *LSE, *rest;  // rest: (max in log 2, 1 / sum) [B][L][2], then for bf16 what the rounding of O dropped, [B][L][F]
+    float *LSE, *rest;  // rest: (max in the scores' units, 1 / sum) [B][L][2], then for bf16 what the rounding of O dropped, [B][L][F]
     const void *cO, *dO;
     const float *cLSE, *crest;
     void *dK, *dV, *dQ;

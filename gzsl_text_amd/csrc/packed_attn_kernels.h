@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void pa_pack_kernel(PaArgs a) {
     }
 }
 // Backward: dO images of (note, label tile); behind the fragments, for each label, off and scale of its weights
-// P = exp2(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; past the last label its
+// P = e^(y - off) * scale (from the forward's own maximum and sum; from LSE where the caller has only that; past the last label its
 // off again and scale 0) and delta = <dO_l, O_l> (with what the rounding of O dropped, where it is known).  TPR threads a row.  Memory-bound
 // (16 x 1999 rows of 200 bf16: 67 MB in 14 us).
 template <class K, class G>
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void pa_pack_do_kernel(PaArgs a) {
         float off = 0.f, scale = 0.f;
         const long long at = min(row, (long long)b * a.L + a.L - 1);
         if (a.crest) off = a.crest[2 * at], scale = a.crest[2 * at + 1];
-        else off = a.cLSE[at] * PA_LOG2E, scale = 1.f;
+        else if (a.cLSE[at] != -INFINITY) off = a.cLSE[at] * (a.cap > 0.f ? PA_LOG2E : 1.f), scale = 1.f;
         if (l >= a.L) scale = 0.f;
         aux[r] = off;
         aux[G::ROWS + r] = scale;
@@ -282,11 +282,10 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mt = fmaxf(mt, y[u][r]);
-        if (!CAP) mt *= PA_LOG2E;
-        if (__any(mt > w.m + 12.f)) {  // m is the same in the four lanes of a column
+        if (__any(mt > w.m + (CAP ? 12.f : 12.f * PA_LN2))) {  // m is the same in the four lanes of a column
             mt = fmaxf(mt, __shfl_xor(mt, 16));
             mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float mn = fmaxf(w.m, mt), alpha = mn == w.m ? 1.f : __builtin_amdgcn_exp2f(w.m - mn);
+            const float mn = fmaxf(w.m, mt), alpha = mn == w.m ? 1.f : pa_exp<CAP>(w.m - mn);
 #pragma unroll
             for (int j = 0; j < G::NF; ++j) w.acc[j] *= alpha;
             w.sum *= alpha;
@@ -296,7 +295,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[u][r] = CAP ? y[u][r] - mi : fmaf(y[u][r], PA_LOG2E, -mi);
+            for (int r = 0; r < 4; ++r) y[u][r] -= mi;
     }
     frag pf;
     bf16x8 pl;
@@ -306,7 +305,7 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[u][r] = __builtin_amdgcn_exp2f(y[u][r]);
+                p[u][r] = pa_exp<CAP>(y[u][r]);
                 w.sum += p[u][r];
                 if (DROP) p[u][r] = gz_u32(w.key, (uint32_t)(t0 + 16 * u + 4 * g + r)) >= a.thresh ? p[u][r] * a.scale : 0.f;
             }
@@ -318,7 +317,10 @@ __device__ __forceinline__ void pa_fwd_tile(PaFwdState<K, G>& w, const PaArgs& a
         w.acc[j] = pa_mma(f, pf, w.acc[j]);
     });
 }
-// Output rows, or a chunk's part of them.
+// Output rows, or a chunk's part of them.  A row without a finite score (sum 0) is one of no tokens.
+__device__ __forceinline__ float pa_lse(const PaArgs& a, float m, float sum) {
+    return sum == 0.f ? -INFINITY : fmaf(__builtin_amdgcn_logf(sum), PA_LN2, a.cap > 0.f ? m * PA_LN2 : m);
+}
 template <class K, class G>
 __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a, const PaUnit& un, int l, int lane) {
     typedef typename K::T T;
@@ -335,11 +337,10 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
         for (int j = 0; j < G::NF; ++j) pa_out<float>(w.acc[j], a.part + pr * a.F, nullptr, 16 * j + 4 * g, a.F);
         return;
     }
-    const bool some = un.sp.len > 0;
-    const float inv = some ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (g == 0) {
-        a.LSE[row] = some ? (w.m + __builtin_amdgcn_logf(sum)) * PA_LN2 : -INFINITY;
-        if (a.rest) a.rest[2 * row] = w.m, a.rest[2 * row + 1] = inv;
+        a.LSE[row] = pa_lse(a, w.m, sum);
+        if (a.rest) a.rest[2 * row] = sum == 0.f ? 0.f : w.m, a.rest[2 * row + 1] = inv;
     }
     T* out = (T*)a.O + row * a.F;
     bf16* low = sizeof(T) == 2 && a.rest ? reinterpret_cast<bf16*>(a.rest + 2LL * a.B * a.L) + row * a.F : nullptr;
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
         if ((b0 - c0) % 64 == 0) {
             const int c = min(b0 + lane, c1 - 1);
             const float s = b0 + lane < c1 ? ml[2LL * c * a.L + 1] : 0.f;
-            f = s != 0.f ? __builtin_amdgcn_exp2f(ml[2LL * c * a.L] - M) : 0.f;
+            f = s != 0.f ? __builtin_amdgcn_exp2f((ml[2LL * c * a.L] - M) * (a.cap > 0.f ? 1.f : PA_LOG2E)) : 0.f;
             sum = fmaf(f, s, sum);
         }
 #pragma unroll
@@ -559,10 +560,10 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
     sum = 0.f;
 #pragma unroll
     for (int q = 0; q < G; ++q) sum += ss[w0 + q];
-    const float inv = 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (f0 == 0) {
-        a.LSE[row] = (M + __builtin_amdgcn_logf(sum)) * PA_LN2;
-        if (a.rest) a.rest[2 * row] = M, a.rest[2 * row + 1] = inv;
+        a.LSE[row] = pa_lse(a, M, sum);
+        if (a.rest) a.rest[2 * row] = sum == 0.f ? 0.f : M, a.rest[2 * row + 1] = inv;
     }
     for (int f = f0; f < a.F; f += step) {
         float o = 0.f;
@@ -576,10 +577,10 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
 }
 
 // ------------------------------------------------------------------------------------------------------------- backward
-// P and dS of a tile: weights w = exp2(y - off) * scale, dropout factor keep.
+// P and dS of a tile: weights w = e^(y - off) * scale, dropout factor keep.
 template <int CAP, bool TH>
 __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, float scale, float delta, float keep, float& p, float& ds) {
-    const float w = __builtin_amdgcn_exp2f(CAP ? y - off : fmaf(y, PA_LOG2E, -off)) * scale;
+    const float w = pa_exp<CAP>(y - off) * scale;
     p = w * keep;
     ds = w * fmaf(dp, keep, -delta);
     if (TH) ds *= fmaf(-th, th, 1.f);

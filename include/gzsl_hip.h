@@ -277,7 +277,9 @@ int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long 
 /* Label-wise attention over packed notes (icd_modules.py:137-142 for notes of unequal length; the reference attends its
  * padding):  x = <q_l, k_t>, y = cap*tanh(x/cap) (cap = 0: y = x), softmax of y over the note's own tokens, dropout on the
  * weights (the masks of gzsl_label_attn_fwd, keyed on (b*L_total + l_offset + l, token index in the note)), pooling of the
- * values.  O [B,L,F] of the tensors' type, LSE [B,L] fp32 (natural units); a note of no tokens gives O = 0, LSE = -inf.
+ * values.  O [B,L,F] of the tensors' type, LSE [B,L] fp32 (natural units); a note of no tokens, or one whose scores
+ * for a label are all minus infinity, gives O = 0, LSE = -inf and gradients of 0.  Pooling sums are taken before they are divided by the
+ * weights' sum: values above 1e25 in magnitude may run over.
  * E, F <= 208; cap 0 or from 1e-30 to 1e30.  `work`: 16-byte aligned device scratch of gzsl_packed_attn_work_bytes(d, backward) bytes (-1: bad arguments),
  * its contents undefined before and after. */
 typedef struct GzslPackedAttn {

@@ -135,3 +135,44 @@ def test_infinite_values(ops, E, L, dtype):
     assert torch.isposinf(O[0, :, 3]).all() and torch.isneginf(O[1, :, 11]).all()
     within(O, ref['O'], 'O')
     within(lse, ref['lse'], 'lse')
+
+
+@BOTH
+@pytest.mark.parametrize('lens,E,F,L', [([70, 33, 40], 100, 40, 33), ([130, 33, 60], 112, 40, 150), ([70, 33], 113, 52, 33), ([40, 400, 1], 200, 64, 300), ([33, 900], 36, 20, 5)])
+@pytest.mark.parametrize('rest', [True, False], ids=['rest', 'lse'])
+def test_notes_whose_tokens_are_all_masked(ops, lens, E, F, L, dtype, rest):
+    """Of minus infinity nothing is left: like a note of no tokens, O = 0, lse = minus infinity and gradients of 0.  The lowest value is a
+    score like any other.  The other notes do not see it."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=18)
+    q[:, -1], k[:, -1] = 1, 0
+    s, n = sl[1]
+    other = [i for i in range(len(lens)) if i != 1]
+    outside = [(0, 0) if i == 1 else x for i, x in enumerate(sl)]
+    for low in (float('-inf'), torch.finfo(dtype).min):
+        k[s:s + n, -1] = low
+        O, lse, kept = ops.attn_packed_fwd(k, v, q, spans, max_len)
+        dk, dv, dq = ops.attn_packed_bwd(do, O, lse, kept if rest else None, k, v, q, spans, max_len)
+        ref = attn_ref_range(k, v, q, outside, 0.0, do)
+        within(O[other], [x[other] for x in ref['O']], 'O')
+        within(lse[other], [x[other] for x in ref['lse']], 'lse')
+        for i in other if rest else ():
+            r = slice(sl[i][0], sl[i][0] + sl[i][1])
+            within(dk[r], [x[r] for x in ref['dK']], 'dK')
+            within(dv[r], [x[r] for x in ref['dV']], 'dV')
+        if low == float('-inf'):
+            assert not O[1].any() and torch.isneginf(lse[1]).all() and not dk[s:s + n].any() and not dv[s:s + n].any()
+            assert not torch.isnan(dq[:, :-1]).any()
+            if rest:
+                within(dq[:, :-1], [x[:, :-1] for x in ref['dQ']], 'dQ')
+        else:
+            # A score of 3.4e38 is off by up to (E + 2) u of it, 2e33 and more, as any sum of E products is (two of these scores, equal in
+            # 64 bits, may differ by a rounding of 2e31): which tokens carry the weight is not determined, only that the weights
+            # are finite, not negative and sum to 1.  O lies among the note's values, and dV sums over the tokens to the sum of dO.
+            step, tol = torch.finfo(dtype).eps / 2, (2 * n + L + 20) * 2.0 ** -24 + 2.0 ** -16 * (dtype == torch.bfloat16)
+            vd, g = v[s:s + n].cpu().double(), do[1].cpu().double()
+            slack = (step + 2 * tol) * vd.abs().amax(0)
+            x = O[1].cpu().double()
+            assert (x >= vd.amin(0) - slack).all() and (x <= vd.amax(0) + slack).all()
+            if rest:
+                got, up = dv[s:s + n].cpu().double(), g.sum(0)
+                assert ((got.sum(0) - up).abs() <= tol * g.abs().sum(0) + step * got.abs().sum(0)).all()
