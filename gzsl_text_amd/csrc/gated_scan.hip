@@ -38,6 +38,7 @@ struct GsArgs {
     float* dh0;
     float* pair;                             // [B][nch][2][H]
     int joined;
+    int* ascending;                          // of many notes: whether the table lists them in ascending order
     int ncg, nblk, TS, tiles, chunk, nch;    // channel groups of a workgroup, workgroups over the channels, threads over time, tiles of a chunk
 };
 
@@ -226,14 +227,26 @@ __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
     const GsPlace p = gs_place(a, V);
     const NoteSpan sp = note_span(a.spans, p.b, a.rows, a.max_len);
     const long long first = (long long)p.k * a.chunk;
-    {   // rows of no note: those behind this note, shared out like its own rows, and those in front of note 0
-        const long long next = p.b + 1 < a.B ? note_span(a.spans, p.b + 1, a.rows, a.max_len).start : a.rows;
+    {   // rows of no note: those behind this note, shared out like its own rows, and those in front of all notes, shared out over note 0's
+        const bool known = a.ascending && *a.ascending;
+        const long long end = sp.start + sp.len;
+        const NoteSpan after = p.b + 1 < a.B ? note_span(a.spans, p.b + 1, a.rows, a.max_len) : NoteSpan{a.rows, 1};
+        const bool look = !known && !(after.start == end && after.len > 0), front = p.b == 0 && sp.start > 0;
+        __shared__ long long gap[2];
+        if (look || front) {
+            if (p.tid < 64) {  // (the last wave may be short of lanes)
+                const long long g0 = look ? note_gap(a.spans, a.B, a.rows, a.max_len, end) : 0, g1 = note_gap(a.spans, a.B, a.rows, a.max_len, -1);
+                if (p.tid == 0) gap[0] = g0, gap[1] = g1;
+            }
+            __syncthreads();
+        }
+        const long long next = look ? gap[0] : after.start;
         const long long lo = max(first, (long long)sp.len), hi = p.k == a.nch - 1 ? next - sp.start : min(first + a.chunk, next - sp.start);
         float zero[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) zero[v] = 0.f;
-        auto clear = [&](long long r0, long long r1) {
-            for (long long r = r0 + p.j; r < r1; r += a.TS) {
+        auto clear = [&](long long r0, long long r1, int step) {
+            for (long long r = r0 + p.j; r < r1; r += step) {
                 if (!p.on) break;
                 if (BWD) {
                     gs_store<T, V>((T*)a.dg + r * a.H + p.ch, zero);
@@ -243,8 +256,8 @@ __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
                 }
             }
         };
-        clear(sp.start + lo, sp.start + hi);
-        if (p.b == 0 && p.k == 0) clear(0, sp.start);
+        clear(sp.start + lo, sp.start + hi, a.TS);
+        if (front) clear((long long)p.k * a.TS, gap[1], a.nch * a.TS);
     }
     if (first >= sp.len && p.k > 0) return;
     const long long at = (long long)p.b * a.H + p.ch;
@@ -372,6 +385,18 @@ __global__ __launch_bounds__(GS_THREADS) void gs_apply_kernel(GsArgs a) {
         for (int v = 0; v < V; ++v) end[at + v] = x[v];
 }
 
+// Whether the notes stand in ascending order, disjoint: then a note's rows of no note end at the next one's start, and of many notes a
+// workgroup need not go through the whole table for them.
+__global__ __launch_bounds__(1024) void gs_order_kernel(GsArgs a) {
+    bool ok = true;
+    for (int b = threadIdx.x; b + 1 < a.B; b += 1024) {
+        const NoteSpan sp = note_span(a.spans, b, a.rows, a.max_len), next = note_span(a.spans, b + 1, a.rows, a.max_len);
+        ok = ok && sp.start + sp.len <= next.start;
+    }
+    ok = __syncthreads_and(ok);
+    if (threadIdx.x == 0) *a.ascending = ok;
+}
+
 // Its launch is its time (64 x 200: 4.4 us with the call).
 template <typename T>
 __global__ __launch_bounds__(256) void gs_step_kernel(const T* g, const T* c, float* state, const uint8_t* active, int H, long long ldg, long long ldc, long long n) {
@@ -427,12 +452,18 @@ static int gs_shape(GsArgs& a, int V) {
     return (long long)a.nch * a.B > 0x7FFFFFFF ? GZSL_ETOOBIG : 0;
 }
 
+static long long gs_pair_bytes(const GsArgs& a) { return a.nch > 1 ? 8LL * a.B * a.nch * a.H : 0; }
+// Up to 256 notes a workgroup finds its rows of no note in the table, four loads a wave; of more, a kernel looks at the order first.
+static long long gs_work(const GsArgs& a) { return gs_pair_bytes(a) + (a.B > 256 ? 16 : 0); }
+
 template <typename T, int V, bool BWD>
 static int gs_go(GsArgs& a, void* work, long long work_bytes, hipStream_t st) {
     constexpr int S = V == 8 ? 4 : 8;
     if (int e = gs_shape(a, V)) return e;
-    if (a.nch > 1 && (!work || ((uintptr_t)work & 15) || work_bytes < 8LL * a.B * a.nch * a.H)) return GZSL_EINVAL;
+    if (gs_work(a) > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < gs_work(a))) return GZSL_EINVAL;
     a.pair = (float*)work;
+    a.ascending = a.B > 256 ? (int*)((char*)work + gs_pair_bytes(a)) : nullptr;
+    if (a.ascending) hipLaunchKernelGGL(gs_order_kernel, dim3(1), dim3(1024), 0, st, a);
     const dim3 grid(a.nch * a.B, a.nblk), block(a.ncg * a.TS);
     const size_t lds = sizeof(float) * 2 * V * block.x;
     if (a.nch > 1) hipLaunchKernelGGL((gs_chunk_kernel<T, V, S, BWD>), grid, block, lds, st, a);
@@ -463,7 +494,7 @@ extern "C" long long gzsl_gated_scan_work_bytes(const GzslGatedScan* d, int back
     for (int V = 1; V <= 8; V <<= 1) {
         GsArgs a = gs_args(*d);
         if (V == 2 || gs_shape(a, V)) continue;
-        const long long n = a.nch > 1 ? 8LL * a.B * a.nch * a.H : 0;
+        const long long n = gs_work(a);
         most = n > most ? n : most;
     }
     return most;

@@ -728,8 +728,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void pa_kv_finish_kernel(PaArgs a) {
     const int b = blockIdx.y, W = a.E + a.F, lane = threadIdx.x & 63, w = pa_scalar((int)threadIdx.x >> 6);
     const NoteSpan sp = b < a.B ? note_span(a.spans, b, a.rows, a.max_len) : NoteSpan{0, 0};
-    const int next = b == a.B ? 0 : b + 1;  // the note that the gap behind this one ends at
-    const long long end = next < a.B ? note_span(a.spans, next, a.rows, a.max_len).start : a.rows;
+    const long long end = note_gap(a.spans, a.B, a.rows, a.max_len, b < a.B ? sp.start + sp.len : -1);  // of the gap behind this note
     long long first;
     const PaRuns runs(pa_all_tiles(a, b, first), a.nQ);
     if (a.join_rows == 1) {  // few tiles of many runs each: the four waves share one row's parts and join in LDS

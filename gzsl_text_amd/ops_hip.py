@@ -512,7 +512,7 @@ class HipOps:
     def attn_packed_fwd(self, keys, values, queries, spans, max_len, cap=0.0, l_offset=0, L_total=0, seed=0, p=0.0,
                         need_grad=True):
         """(O [B,L,F], lse [B,L], rest): label attention over packed notes (gzsl_packed_attn_fwd).  keys [R,E], values [R,F],
-        queries [L,E], all fp32 or all bf16; spans [B,2] int64 = (first row, rows) per note, ascending and disjoint.  `rest`
+        queries [L,E], all fp32 or all bf16; spans [B,2] int64 = (first row, rows) per note, disjoint, in any order.  `rest`
         is for attn_packed_bwd (softmax statistics; bf16: what the rounding of O dropped); None without need_grad."""
         d, hold = self._packed_attn(keys, values, queries, spans, max_len, cap, l_offset, L_total, seed, p)
         O = torch.empty((d.B, d.L, d.F), dtype=values.dtype, device=values.device)

@@ -268,8 +268,8 @@ int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long 
 
 /* ---- packed notes -----------------------------------------------------------------------------------------------
  * Notes of unequal length in one [rows, width] tensor: note b owns rows spans[2b] .. spans[2b] + spans[2b+1] - 1 (int64, on
- * the device, ascending and disjoint; a padded [B,T,width] batch is spans (b*T, length)).  `max_len` is at least the longest
- * count.  The kernels clamp every span to [0, rows) and max_len: a table that is neither ascending nor disjoint gives wrong numbers, never an
+ * the device, disjoint, in any order; a padded [B,T,width] batch is spans (b*T, length)).  `max_len` is at least the longest
+ * count.  The kernels clamp every span to [0, rows) and max_len: a table of notes that overlap gives wrong numbers, never an
  * access out of range.  Tensors are fp32 or bf16 (`dtype`), their rows `ld*`
  * elements apart with consecutive elements inside a row; sums, softmax statistics and states are fp32 for both. */
 #define GZSL_F32 0

@@ -80,3 +80,35 @@ def test_a_far_state_through_open_gates(ops, ext):
         gd, cd, s = g[:2].cpu().double(), c[:2].cpu().double(), h0.cpu().double()
         t1, t2 = torch.sigmoid(-gd) * s, torch.sigmoid(gd) * cd
         within(state, (t1 + t2, (8 + gd.abs()) * U * (t1.abs() + t2.abs()) + U * (t1 + t2).abs()), 'state')
+
+
+@pytest.mark.parametrize('reverse', [False, True], ids=['ahead', 'back'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('lens,H', [([130, 0, 33, 257, 0, 1], 200), ([70, 900, 0, 31], 5), ([12, 0, 3] * 24, 40), ([3, 0, 1, 0, 7] * 60 + [300], 7)])
+def test_a_table_in_any_order(ops, dtype, lens, H, reverse):
+    """Notes sorted by anything, more of them than a wave has lanes and than a workgroup looks through: every note's results are its
+    own, and rows of no note, which hold NaN, get zeros.  The same notes in ascending order give the same bits."""
+    from tests.test_gpu_packed_attn_range import any_order
+    spans, sl, R = any_order(lens, seed=4)
+    gen = torch.Generator().manual_seed(5)
+    g, c, dh = (torch.full((R, H), float('nan')) for _ in range(3))
+    for s, n in sl:
+        g[s:s + n], c[s:s + n], dh[s:s + n] = (torch.randn(n, H, generator=gen) for _ in range(3))
+    g, c, dh = (x.to(dtype).to(DEV) for x in (g, c, dh))
+    h0, dl = (torch.randn(len(lens), H, generator=gen).to(DEV) for _ in range(2))
+    own = torch.zeros(R, dtype=torch.bool)
+    for s, n in sl:
+        own[s:s + n] = True
+    ref = ref_once(g, c, sl, h0, reverse, torch.where(own.to(DEV)[:, None], dh, 0), dl)
+    order = sorted(range(len(sl)), key=lambda i: sl[i])
+    for at in (list(range(len(sl))), order):
+        t, h00, dl0 = spans[at].contiguous(), h0[at].contiguous(), dl[at].contiguous()
+        h, last, rest = ops.gated_scan_fwd(g, c, t, max(lens), h00, reverse, need_grad=True)
+        got = (h, last, *ops.gated_scan_bwd(dh, dl0, h, g, c, t, max(lens), h00, reverse, rest))
+        for name, x in zip(('h', 'last', 'dg', 'dc', 'dh0'), got):
+            within(x, [y[at] for y in ref[name]] if name in ('last', 'dh0') else ref[name], name)
+        for x in (got[0], got[2], got[3]):
+            assert not x[~own].any()
+        first = got if at is not order else first
+    for i in (0, 2, 3):
+        assert torch.equal(first[i], got[i])

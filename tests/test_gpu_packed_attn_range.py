@@ -176,3 +176,48 @@ def test_notes_whose_tokens_are_all_masked(ops, lens, E, F, L, dtype, rest):
             if rest:
                 got, up = dv[s:s + n].cpu().double(), g.sum(0)
                 assert ((got.sum(0) - up).abs() <= tol * g.abs().sum(0) + step * got.abs().sum(0)).all()
+
+
+def any_order(lens, seed, lead=5):
+    """A table of notes in no order, rows of no note in front, between and behind, notes of no tokens anywhere in it."""
+    from random import Random
+    r = Random(seed)
+    at, spans = lead, []
+    for n in lens:
+        spans.append((at, n))
+        at += n + r.choice([0, 0, 1, 7, 150])
+    spans = [(r.choice([0, at // 2, at, s]) if n == 0 else s, n) for s, n in spans]
+    r.shuffle(spans)
+    return torch.tensor(spans, dtype=torch.int64, device=DEV), spans, at + 11
+
+
+@BOTH
+@pytest.mark.parametrize('lens,E,L', [([130, 0, 33, 257, 0, 1], 100, 40), ([130, 0, 33, 257, 0, 1], 36, 300), ([64, 32, 128], 200, 33)])
+def test_a_table_in_any_order(ops, dtype, lens, E, L):
+    """Notes sorted by anything: every note's results are its own, and rows of no note, which hold NaN, get zeros."""
+    spans, sl, R = any_order(lens, seed=2)
+    gen = torch.Generator().manual_seed(5)
+    k, v = torch.full((R, E), float('nan')), torch.full((R, 52), float('nan'))
+    for s, n in sl:
+        k[s:s + n], v[s:s + n] = torch.randn(n, E, generator=gen), torch.randn(n, 52, generator=gen)
+    k, v, q, do = (x.to(dtype).to(DEV) for x in (k, v, 0.3 * torch.randn(L, E, generator=gen), torch.randn(len(lens), L, 52, generator=gen)))
+    got, ref = run(ops, k, v, q, do, spans, max(lens), 5.0), attn_ref_range(k, v, q, sl, 5.0, do)
+    for name, x in got.items():
+        within(x, ref[name], name)
+    own = torch.zeros(R, dtype=torch.bool)
+    for s, n in sl:
+        own[s:s + n] = True
+    assert not got['dK'][~own].any() and not got['dV'][~own].any()
+
+
+@BOTH
+def test_many_notes_in_any_order(ops, dtype):
+    """Hundreds of notes, images by rows: one of 700 tokens among them."""
+    gen = torch.Generator().manual_seed(7)
+    lens = [int(x) for x in torch.randint(0, 20, (300,), generator=gen)] + [700]
+    spans, sl, R = any_order(lens, seed=3)
+    k, v = torch.randn(R, 36, generator=gen).to(dtype).to(DEV), torch.randn(R, 20, generator=gen).to(dtype).to(DEV)
+    q, do = (0.3 * torch.randn(150, 36, generator=gen)).to(dtype).to(DEV), torch.randn(len(lens), 150, 20, generator=gen).to(dtype).to(DEV)
+    got, ref = run(ops, k, v, q, do, spans, 700), attn_ref_range(k, v, q, sl, 0.0, do)
+    for name, x in got.items():
+        within(x, ref[name], name)
