@@ -541,7 +541,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 64 * G) void pa_join_kernel(PaArgs a
 #pragma unroll
         for (int i = 0; i < D; ++i) {
             const float fi = __shfl(f, (b0 - c0) % 64 + i);
-            if (b0 + i < c1 && fi != 0.f)
+            if (b0 + i < c1)  // (a part that is no number stays one behind a weight of 0)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o4[k] = fmaf(fi, v[i][k], o4[k]);
         }

@@ -221,3 +221,16 @@ def test_many_notes_in_any_order(ops, dtype):
     got, ref = run(ops, k, v, q, do, spans, 700), attn_ref_range(k, v, q, sl, 0.0, do)
     for name, x in got.items():
         within(x, ref[name], name)
+
+
+@BOTH
+@pytest.mark.parametrize('lens,L', [([900], 9), ([400, 700], 150), ([70], 9)])
+def test_a_value_that_is_no_number_shows_wherever_its_weight_is(ops, lens, L, dtype):
+    """A weight of 0 times NaN is NaN, in a note that is cut into chunks as in one that is not: in every label's row, in that column."""
+    k, v, q, do, spans, max_len, sl = make(lens, 36, 20, L, dtype, seed=21)
+    q[:, -1], k[:, -1] = 1, 0
+    s, n = sl[0]
+    v[s + 3, 7] = float('nan')  # at a weight of e^-10000
+    k[s:s + n // 2, -1] = -1e4  # (and chunks of such weights alone)
+    O = ops.attn_packed_fwd(k, v, q, spans, max_len, need_grad=False)[0]
+    assert torch.isnan(O[0, :, 7]).all() and torch.isnan(O).sum() == L
