@@ -112,3 +112,16 @@ def test_a_table_in_any_order(ops, dtype, lens, H, reverse):
         first = got if at is not order else first
     for i in (0, 2, 3):
         assert torch.equal(first[i], got[i])
+
+
+@pytest.mark.parametrize('reverse', [False, True], ids=['ahead', 'back'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('lens,H', [([1100, 0, 33, 700, 64, 31, 1, 1057], 2048), ([1701, 700, 64, 1, 0, 33, 96, 1500], 257), ([1400, 96, 65, 31], 4100)])
+def test_chunks_of_several_tiles(ops, dtype, lens, H, reverse):
+    """Wide states make chunks of two tiles and more; notes end in a chunk's first tile, at its end, inside its last one."""
+    g, c, spans, max_len, h0, dh, dl, sl = make(lens, H, dtype, seed=8)
+    h, last, rest = ops.gated_scan_fwd(g, c, spans, max_len, h0, reverse, need_grad=True)
+    got = (h, last, *ops.gated_scan_bwd(dh, dl, h, g, c, spans, max_len, h0, reverse, rest))
+    ref = ref_once(g, c, sl, h0, reverse, dh, dl)
+    for name, x in zip(('h', 'last', 'dg', 'dc', 'dh0'), got):
+        within(x, ref[name], name)

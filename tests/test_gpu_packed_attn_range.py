@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.packed_ref import attn_ref, within
+from tests.packed_ref import attn_ref, dropout_keep, within
 from tests.packed_ref_range import attn_ref_range
 
 pytestmark = pytest.mark.gpu
@@ -234,3 +234,30 @@ def test_a_value_that_is_no_number_shows_wherever_its_weight_is(ops, lens, L, dt
     k[s:s + n // 2, -1] = -1e4  # (and chunks of such weights alone)
     O = ops.attn_packed_fwd(k, v, q, spans, max_len, need_grad=False)[0]
     assert torch.isnan(O[0, :, 7]).all() and torch.isnan(O).sum() == L
+
+
+@BOTH
+@pytest.mark.parametrize('cap', [0.0, 5.0, 100.0])
+@pytest.mark.parametrize('lens,E,F,L', [([130, 0, 33], 36, 52, 150), ([900, 70], 100, 64, 300), ([900, 70], 200, 200, 150), ([33, 500], 200, 61, 40),
+                                        ([40, 9], 113, 20, 1300)])
+def test_dropout_in_every_form(ops, lens, E, F, L, dtype, cap):
+    """Weights dropped by the counter hash, in the form of few labels and of many, at both key widths, in notes that are cut, with labels
+    that are a shard of more, under no cap, the closed form and the series."""
+    k, v, q, do, spans, max_len, sl = make(lens, E, F, L, dtype, seed=22)
+    drop = dict(l_offset=37, L_total=L + 50, seed=4321, p=0.2)
+    got = run(ops, k, v, q, do, spans, max_len, cap, **drop)
+    ref = attn_ref_range(k, v, q, sl, cap, do, dropout_keep(sl, L, 4321, 0.2, 37, L + 50))
+    for name, x in got.items():
+        within(x, ref[name], name)
+
+
+@BOTH
+@pytest.mark.parametrize('E,cap', [(36, 5.0), (200, 0.0), (200, 5.0)])
+def test_dropout_with_more_workgroups_than_the_chip_has_places(ops, dtype, E, cap):
+    gen = torch.Generator().manual_seed(6)
+    lens = [int(x) for x in torch.randint(0, 40, (65,), generator=gen)] + [133]
+    k, v, q, do, spans, max_len, sl = make(lens, E, 24, 1100, dtype, seed=23)
+    got = run(ops, k, v, q, do, spans, max_len, cap, seed=99, p=0.5)
+    ref = attn_ref_range(k, v, q, sl, cap, do, dropout_keep(sl, 1100, 99, 0.5))
+    for name, x in got.items():
+        within(x, ref[name], name)
