@@ -233,7 +233,7 @@ struct PackedLabelAttention : public torch::autograd::Function<PackedLabelAttent
         TORCH_CHECK(p_drop >= 0.0 && p_drop < 1.0, "gzsl: drop probability in [0, 1)");
         check_spans(spans, max_len, k);
         if (L_total <= 0) L_total = q.size(0);
-        TORCH_CHECK(l_offset >= 0 && l_offset + q.size(0) <= L_total && L_total < (1LL << 31), "gzsl: labels outside of L_total");
+        TORCH_CHECK(l_offset >= 0 && L_total < (1LL << 31) && l_offset <= L_total - q.size(0), "gzsl: labels outside of L_total");
         const c10::DeviceGuard guard(k.device());
         const GzslPackedAttn d = describe(k, v, q, spans, max_len, cap, p_drop, seed, l_offset, L_total);
         Tensor O = at::empty({d.B, d.L, d.F}, v.options()), lse = at::empty({d.B, d.L}, v.options().dtype(at::kFloat));

@@ -501,7 +501,7 @@ class HipOps:
             raise RuntimeError(f'drop probability {p} outside [0, 1)')
         L = queries.shape[0]
         L_total = L_total or L
-        if l_offset < 0 or l_offset + L > L_total:
+        if l_offset < 0 or l_offset + L > L_total or L_total > INT_MAX:
             raise RuntimeError(f'labels {l_offset} .. {l_offset + L} outside of {L_total}')
         th, sc = drop_params(p)
         d = hip.GzslPackedAttn(dptr(keys), dptr(values), dptr(queries), ptr(spans), keys.shape[0], self._ld(keys), self._ld(values),

@@ -261,3 +261,12 @@ def test_dropout_with_more_workgroups_than_the_chip_has_places(ops, dtype, E, ca
     ref = attn_ref_range(k, v, q, sl, cap, do, dropout_keep(sl, 1100, 99, 0.5))
     for name, x in got.items():
         within(x, ref[name], name)
+
+
+@pytest.mark.parametrize('l_offset,L_total', [(-1, 0), (1, 0), (3, 6), (2 ** 63 - 1, 0), (2 ** 63 - 4, 5), (0, 2 ** 31)])
+def test_labels_outside_of_their_range_are_refused(l_offset, L_total):
+    from gzsl_text_amd import torch_ext
+    torch_ext.load()
+    k, v, q, do, spans, max_len, sl = make([5], 8, 8, 4, torch.float32, seed=1)
+    with pytest.raises(RuntimeError, match='outside of L_total'):
+        torch.ops.gzsl.packed_label_attention(k, v, q, spans, max_len, 0.0, 0.0, 0, l_offset, L_total)

@@ -228,3 +228,12 @@ def test_a_step_that_autograd_would_miss_is_refused(ext, which):
                 step(*t)
             with pytest.raises((RuntimeError, NotImplementedError), match='GPU|CPU|cuda|device'):
                 step(*[x.detach() for x in t])
+
+
+@pytest.mark.parametrize('l_offset,L_total', [(-1, 0), (1, 0), (3, 6), (2 ** 63 - 1, 0), (0, 2 ** 31), (2 ** 32, 2 ** 32 + 4)])
+def test_labels_outside_of_their_range_are_refused(l_offset, L_total):
+    from gzsl_text_amd.ops_hip import HipOps
+    t, n, rows = note_spans([3, 4], device='cpu')
+    x = torch.zeros(rows, 8)
+    with pytest.raises(RuntimeError, match='outside of'):
+        HipOps().attn_packed_fwd(x, x, x[:4], t, n, l_offset=l_offset, L_total=L_total)
