@@ -630,6 +630,7 @@ __global__ __launch_bounds__(256) void gemm_shortk_kernel(GzslGemm g) {
             a[u] = *reinterpret_cast<const f32x4*>(ap + (long long)(k + u) * g.a_sk);
             b[u] = *reinterpret_cast<const f32x4*>(bp + (long long)(k + u) * g.b_sk);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (left alone, each k's loads wait behind the products of the one before: 6.2 us against 4.2 at K = 8 to 24)
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
