@@ -12,7 +12,7 @@
 //   3. gs_apply_kernel takes that state (or joins the pairs of the chunks before its own itself), then runs through its tiles:
 //      each thread's steps to a pair, a scan of the pairs over the tile's threads in LDS, the steps again from the state in front.
 // Memory-bound: 3 (6) tensors forward (backward), of which the first pass reads two once more (from the 256 MB last-level cache
-// where they fit).  81600 x 256 bf16 forward: 19 + 8 + 26 us (4.4 and 4.7 TB/s in the first and the third; a copy reaches 5.1); 18388 x
+// where they fit).  81600 x 256 bf16 forward: 21 + 8 + 28 us (4.0 and 4.5 TB/s in the first and the third; a copy reaches 5.1); 18388 x
 // 200 fp32: 10 + 12 us, backward 9 + 21.  A workgroup takes whole rows: of narrower pieces, for more workgroups, the third took 44 for 39.
 // The pairs meet in a fixed order, so results repeat bit for bit; tokens in front of a step never see it.
 #include "packed.h"

@@ -15,7 +15,7 @@
 // P in one, a score row whose pooled values cancel was off by many times its own rounding (values of both signs, 517 tokens: 3.3e-4 for
 // 0.8e-4), and O 1.0 to 1.3 times as far off as a rounded exact result where they do not; dS sums to zero over a row, so its products cancel
 // always, and delta = <dO, O> has to be that of the same P: dK and dQ were up to 2.4 times as far off, dV 1.4 times.  So all are within a
-// hundredth of rounded exact results (forward of 19309 tokens x 9000 labels 137 -> 173 us, of 17404 x 1999 labels of 200 50 -> 60, dK / dV
+// hundredth of rounded exact results (forward of 19309 tokens x 9000 labels 139 -> 172 us, of 17404 x 1999 labels of 200 50 -> 60, dK / dV
 // there 88 -> 98).
 //
 // Everything is moved as FRAGMENTS: 1 KB, 16 bytes a lane, exactly one operand of one matrix instruction (eight bf16 of a lane;
@@ -207,7 +207,7 @@ __device__ __forceinline__ float pa_far(float x, const PaCap& c) {  // cap log2(
 //   2  the odd series below |x / cap| = 0.35 (the next term is below 2^-26 of the value) and the closed form only where a wave's tile
 //      holds a larger one: an error relative to the score, whatever the cap.  fp32 tensors, whose products of the gradient still have
 //      that accuracy, and larger caps, at which the closed form's error grows past the scores (at 1e6 weights were off by a fifth).
-//      For small caps of bf16 it is the longer way: 148 us against 138 for 19309 tokens x 9000 labels, weights in one piece.
+//      For small caps of bf16 it is the longer way: 180 us against 176 for 19309 tokens x 9000 labels.
 #define PA_CLOSED 64.f
 // Scores x of a tile -> y = cap tanh(x / cap) in units of log 2, and th = tanh(x / cap) for the gradient.  Without a cap y is x itself, and
 // maxima stay in its units: in those of log 2 a row of the type's lowest values would run over.

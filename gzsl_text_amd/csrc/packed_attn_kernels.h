@@ -350,8 +350,8 @@ __device__ __forceinline__ void pa_fwd_end(PaFwdState<K, G>& w, const PaArgs& a,
 
 // Workgroup = WAVES x 16 labels of one note (or of one chunk of it), token tiles from the pre-pass's images.  An image is read by all
 // label workgroups of a note and comes from L2; a wave's 16 queries and its output tile stay in registers.  Bound by the matrix pipe
-// (bf16 48 % busy, PaX3 70 %) and the softmax's vector instructions, which overlap with other waves' matrix instructions only in part:
-// 19309 tokens x 9000 labels (100, 200; capped) bf16 124 us, 940 TFLOP/s of the padded products (1255 is what a large library product
+// (bf16 62 % busy, PaX3 70 %) and the softmax's vector instructions, which overlap with other waves' matrix instructions only in part:
+// 19309 tokens x 9000 labels (100, 200; capped) bf16 175 us, 1090 TFLOP/s of the padded products, the second pieces' among them (1255 is what a large library product
 // reaches, whose clock is as low); without the softmax 97.  Tried at that size and no faster: 32 labels a wave (half the LDS
 // reads), three tiles on their way instead of two, priorities by phase or by workgroup.  PaX3: 7339 x 9000 220 us.
 template <class K, class G, int WAVES, int OCC, int CAP, bool DROP>
@@ -588,7 +588,7 @@ __device__ __forceinline__ void pa_grad(float y, float th, float dp, float off, 
 
 // dK / dV: workgroup = one run of steps, 128 tokens of one note (16 a wave, tokens on the lane axis) by a label tile each.  One
 // workgroup a compute unit by its LDS and registers, so two waves a SIMD: what they wait for one another, for fragments and at the
-// barrier of a step is what is left (PaBF, E, F = 200: matrix pipe 48 % busy, LDS 44 %; PaX3 63 and 45 to 53 %).  17404 tokens x 1999
+// barrier of a step is what is left (PaBF, E, F = 200: matrix pipe 51 % busy, LDS 39 %; PaX3 62 to 64 and 42 to 52 %).  17404 tokens x 1999
 // labels of 200 bf16 98 us, 7339 x 9000 of 100 and 200 fp32 305 + 233.
 // PaX3 takes dV and dK in two launches (PART 1 and 2): the pieces of K and V and both accumulators are more than the 256 registers of a
 // wave at two waves a SIMD, and the scores a second time are a fifth of the products.

@@ -66,6 +66,11 @@ def test_16_bit_gradients_are_rounded_once(ops, ext, lens, H, mean, bias, revers
     torch.autograd.backward((h, last), (dh, dl))
     for name, x in zip(('h', 'last', 'dg', 'dc', 'dh0'), (h, last, *[t.grad for t in a])):
         within(x, ref[name], name)
+    # the explicit pair: with what the forward kept, and without it (the backward then runs the forward for it)
+    h, last, rest = ops.gated_scan_fwd(g, c, spans, max_len, h0, reverse, need_grad=True)
+    for kept in (rest, None):
+        for x, t in zip(ops.gated_scan_bwd(dh, dl, h, g, c, spans, max_len, h0, reverse, kept), a):
+            assert torch.equal(x, t.grad)
 
 
 def test_a_far_state_through_open_gates(ops, ext):
