@@ -279,7 +279,7 @@ int gzsl_adam_flat_step(float* p, const float* g, float* m, float* v, long long 
  * weights (the masks of gzsl_label_attn_fwd, keyed on (b*L_total + l_offset + l, token index in the note)), pooling of the
  * values.  O [B,L,F] of the tensors' type, LSE [B,L] fp32 (natural units); a note of no tokens, or one whose scores
  * for a label are all minus infinity, gives O = 0, LSE = -inf and gradients of 0.  Pooling sums are taken before they are divided by the
- * weights' sum: values above 1e25 in magnitude may run over.
+ * weights' sum: values above 1e20 in magnitude may run over.
  * E, F <= 208; cap 0 or from 1e-30 to 1e30.  `work`: 16-byte aligned device scratch of gzsl_packed_attn_work_bytes(d, backward) bytes (-1: bad arguments),
  * its contents undefined before and after. */
 typedef struct GzslPackedAttn {
